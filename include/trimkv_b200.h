@@ -649,6 +649,45 @@ int tkv_moe_route(const float* logits, int64_t logit_stride, const float* correc
 int tkv_moe_gemm(const void* a, int64_t a_stride, int64_t a_rows, const int32_t* src, const void* w, const int32_t* offsets,
                  void* out, int64_t max_rows, int experts, int n, int k, int act, int dtype, int32_t* status, tkv_stream_t stream);
 
+/* How evenly a router spreads its tokens: of n valid tokens (valid NULL: all; else bytes, 0 = not) with `top` choices each and
+ * p = softmax(logits), counts[e] = choices of expert e (entries outside [0, experts) count for none),
+ * loss = experts * sum_e counts[e] / (n top) * mean_t p_te (0 where n is 0).  load [experts + 1] keeps what the gradient needs:
+ * dlogits = grad * experts / n * p * (counts / (n top) - sum_j p_j counts_j / (n top)), 0 for tokens that are not valid; `grad` is one
+ * number in device memory.  logits and dlogits of one type, rows stride elements apart; choices of 32 or 64 bits; experts, top <= 1024. */
+int64_t tkv_moe_balance_workspace_bytes(int64_t tokens, int experts);
+int tkv_moe_balance(const void* logits, int64_t logit_stride, const void* choice, int64_t choice_stride, int choice_bits,
+                    const uint8_t* valid, int64_t valid_stride, int64_t tokens, int experts, int top, float* loss, int32_t* counts,
+                    float* load, void* workspace, int64_t workspace_bytes, int dtype, tkv_stream_t stream);
+int tkv_moe_balance_grad(const void* logits, int64_t logit_stride, const uint8_t* valid, int64_t valid_stride, const float* load,
+                         const float* grad, int64_t tokens, int experts, void* dlogits, int64_t dlogit_stride, int dtype,
+                         tkv_stream_t stream);
+
+/* Rotary positions of queries and keys [batch, heads, tokens, dim] (strides in elements, heads' elements consecutive; heads 0: none),
+ * out of place: the first 2 * pairs elements of a head turn by position * (f_hi + f_lo) and are scaled, the rest is copied.  layout 0:
+ * element i with pairs + i; 1: 2i with 2i + 1.  inverse: turned back (with the same scale), which is also the gradient.  Outputs are
+ * dense [batch, tokens, heads, dim]; positions of 32 or 64 bits [batch, tokens] with any strides. */
+int tkv_rotary(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_ss, void* q_out, int q_heads, const void* k, int64_t k_sb,
+               int64_t k_sh, int64_t k_ss, void* k_out, int k_heads, const void* pos, int pos_bits, int64_t pos_sb, int64_t pos_ss,
+               const float* freq_hi_lo, int batch, int tokens, int dim, int pairs, int layout, int inverse, float scale, int dtype,
+               tkv_stream_t stream);
+
+/* Softmax cross entropy of rows x [tokens, width] (rows x_stride elements apart) against the vocabulary of w [vocab, width], straight
+ * from w: the logits are never kept.  Tokens whose label is `ignore` do not count: loss 0, gradient 0, their rows are not read.  A label
+ * outside [0, vocab) makes the token's loss NaN, sets TKV_DEV_BAD_INDEX and leaves the token out of the gradients.
+ * tkv_vloss_forward: loss [tokens] fp32 and, for reduction 1 (mean over the counting tokens) or 2 (sum), one number in `reduced`; `plan`
+ * (tkv_vloss_plan_words int32) is what tkv_vloss_backward starts from.
+ * tkv_vloss_backward: grad is the gradient of the loss of every token (reduction 0; grad_stride elements apart) or of the reduced number;
+ * dx [tokens, width] and dw [vocab, width] dense, in the type of x and w, either may be NULL.
+ * Workspaces (16-byte aligned): tkv_vloss_workspace_bytes, -1 for sizes that are refused (2^24 tokens, vocabulary 2^23, width 65536). */
+int64_t tkv_vloss_plan_words(int64_t tokens);
+int64_t tkv_vloss_workspace_bytes(int64_t tokens, int64_t vocab, int width, int dtype, int backward, int want_dx);
+int tkv_vloss_forward(const void* x, int64_t x_stride, const void* w, const int64_t* labels, int64_t ignore, int64_t tokens,
+                      int64_t vocab, int width, int reduction, float* loss, float* reduced, int32_t* plan, void* workspace,
+                      int64_t workspace_bytes, int dtype, int32_t* status, tkv_stream_t stream);
+int tkv_vloss_backward(const void* x, int64_t x_stride, const void* w, const int32_t* plan, const float* grad, int64_t grad_stride,
+                       int reduction, int64_t tokens, int64_t vocab, int width, void* dx, void* dw, void* workspace,
+                       int64_t workspace_bytes, int dtype, int32_t* status, tkv_stream_t stream);
+
 /* Blocks until `stream` is idle, then returns *status (a TKV_DEV_* code) and clears it. */
 int tkv_read_status(int32_t* status, tkv_stream_t stream);
 

@@ -11,6 +11,8 @@ from .modeling_llama import TrimKVLlamaConfig, TrimKVLlamaForCausalLM, TrimKVLla
 from .modeling_phi3 import TrimKVPhi3Config, TrimKVPhi3ForCausalLM, TrimKVPhi3Model
 from .modeling_dafovik import DafovikConfig, DafovikForCausalLM, DafovikModel
 from .modeling_lonulix import LonulixConfig, LonulixForCausalLM, LonulixModel
+from .losses import expert_balance, linear_cross_entropy
+from .positions import apply_rotary
 from .registry import load_model, model_class
 from .state_cache import HybridStateCache
 
@@ -21,5 +23,5 @@ __all__ = [
     "TrimKVLlamaConfig", "TrimKVLlamaForCausalLM", "TrimKVLlamaModel",
     "TrimKVPhi3Config", "TrimKVPhi3ForCausalLM", "TrimKVPhi3Model",
     "DafovikConfig", "DafovikForCausalLM", "DafovikModel", "LonulixConfig", "LonulixForCausalLM", "LonulixModel",
-    "HybridStateCache", "load_model", "model_class",
+    "HybridStateCache", "load_model", "model_class", "apply_rotary", "expert_balance", "linear_cross_entropy",
 ]

@@ -89,6 +89,14 @@ SIGNATURES = {
     "tkv_latent_decode": (I, [P, L, L, P, L, L, P, P, I, P, P, F, P, L, L, P, L, I, I, I, I, I, I, P]),
     "tkv_moe_route": (I, [P, L, P, I, I, I, I, I, I, F, P, P, P, P, P, P, P]),
     "tkv_moe_gemm": (I, [P, L, L, P, P, P, P, L, I, I, I, I, I, P, P]),
+    "tkv_moe_balance_workspace_bytes": (L, [L, I]),
+    "tkv_moe_balance": (I, [P, L, P, L, I, P, L, L, I, I, P, P, P, P, L, I, P]),
+    "tkv_moe_balance_grad": (I, [P, L, P, L, P, P, L, I, P, L, I, P]),
+    "tkv_rotary": (I, [P, L, L, L, P, I, P, L, L, L, P, I, P, I, L, L, P, I, I, I, I, I, I, F, I, P]),
+    "tkv_vloss_plan_words": (L, [L]),
+    "tkv_vloss_workspace_bytes": (L, [L, L, I, I, I, I]),
+    "tkv_vloss_forward": (I, [P, L, P, P, L, L, L, I, I, P, P, P, P, L, I, P, P]),
+    "tkv_vloss_backward": (I, [P, L, P, P, P, L, I, L, L, I, P, P, P, L, I, P, P]),
     "tkv_read_status": (I, [P, P]),
 }
 

@@ -1,0 +1,485 @@
+// Cross entropy against a vocabulary (tkv_vloss.cuh): the plan, the joining of the tiles' shares, the gradients of the rows, the entry
+// points, and the form for every type, width and alignment, on the CUDA cores.
+//
+// The CUDA-core products take tiles of 128 x 128 over steps of 16 of the inner axis, 8 x 8 results a thread, the next step's operands in
+// registers meanwhile: bound by the fp32 multiply-adds.
+#include "tkv_vloss.cuh"
+
+namespace tkv {
+
+// ------------------------------------------------------------------------------------------------------------------ the plan
+constexpr int kPlanThreads = 1024, kPlanPer = 8;
+
+// Rows and labels of the tokens that count, in order; loss 0 for ignored ones, NaN for labels out of range (they do not count).
+__global__ void __launch_bounds__(kPlanThreads) vloss_plan_kernel(const int64_t* labels, int64_t ignore, int tokens, int64_t vocab, VlossPlan plan,
+                                                                  float* loss, int32_t* status) {
+  __shared__ int sums[kPlanThreads / 32 + 1];
+  __shared__ int bad_any;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  if (threadIdx.x == 0) bad_any = 0;
+  int base = 0;
+  bool bad = false;
+  __syncthreads();
+  for (int64_t t0 = 0; t0 < tokens; t0 += kPlanThreads * kPlanPer) {
+    int64_t y[kPlanPer];
+    int n = 0;
+    const int64_t t1 = t0 + (int64_t)threadIdx.x * kPlanPer;
+#pragma unroll
+    for (int i = 0; i < kPlanPer; ++i) {
+      y[i] = t1 + i < tokens ? labels[t1 + i] : ignore;
+      const bool off = y[i] != ignore && (y[i] < 0 || y[i] >= vocab);
+      if (t1 + i < tokens && (off || y[i] == ignore)) loss[t1 + i] = off ? __int_as_float(0x7fffffff) : 0.f;
+      bad |= off;
+      if (off) y[i] = ignore;
+      n += y[i] != ignore;
+    }
+    int total;
+    int at = base + block_exclusive_scan<kPlanThreads>(n, sums, &total);
+#pragma unroll
+    for (int i = 0; i < kPlanPer; ++i)
+      if (y[i] != ignore) { plan.rows[at] = (int32_t)(t1 + i); plan.label[at] = (int32_t)y[i]; ++at; }
+    base += total;
+  }
+  if (bad) { bad_any = 1; report(status, TKV_DEV_BAD_INDEX); }
+  __syncthreads();
+  if (threadIdx.x == 0) { plan.head[0] = base; plan.head[1] = bad_any; }
+}
+
+// --------------------------------------------------------------------------------------------------------------- the products
+constexpr int kVgThreads = 256, kVgTile = 128, kVgK = 16, kVgPitch = kVgTile + 4;
+
+enum { kVgStats, kVgLogitGrad, kVgShare, kVgOut };
+
+struct VgOperand {                                         // element (i, k): K-major p[row(i) * ld + k], else p[row(k) * ld + i]
+  const void* p; int64_t ld;
+  const int32_t* rows;                                     // of the axis that steps by ld, or NULL
+  int vec;                                                 // four elements may be read at once
+};
+struct VgProduct {
+  VgOperand a, b;
+  int64_t m, n, k;                                         // where the token axis is one of them, at most *count of it
+  const int32_t* count;
+  int token_axis;                                          // 0: m, 2: k
+  int64_t col0;                                            // column 0 is this of the vocabulary
+  int split; int64_t split_len;                            // share s covers k in [s split_len, ..)
+  int more;                                                // shares are added to what is there
+  Vloss l;
+};
+
+template <typename T> __device__ __forceinline__ void vg_load4(const T* p, int64_t left, bool vec, float* v) {
+  if (vec && left >= 4) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 x = *reinterpret_cast<const float4*>(p);
+      v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    } else {
+      alignas(8) T e[4];
+      *reinterpret_cast<uint2*>(e) = *reinterpret_cast<const uint2*>(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = to_f32<T>(e[i]);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = i < left ? to_f32<T>(p[i]) : 0.f;
+}
+// This thread's 8 of the 128 x 16 elements of a step.
+template <typename T, bool kKMajor> __device__ __forceinline__ void vg_fetch(const VgOperand& o, int64_t i0, int64_t ni, int64_t k0, int64_t k1, float* v) {
+  const T* base = reinterpret_cast<const T*>(o.p);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float* u = v + 4 * h;
+    if constexpr (kKMajor) {
+      const int64_t i = i0 + (threadIdx.x >> 2) + 64 * h, k = k0 + (threadIdx.x & 3) * 4;
+      if (i < ni && k < k1) vg_load4(base + (o.rows ? (int64_t)o.rows[i] : i) * o.ld + k, k1 - k, o.vec, u);
+      else u[0] = u[1] = u[2] = u[3] = 0.f;
+    } else {
+      const int64_t k = k0 + (threadIdx.x >> 4), i = i0 + (threadIdx.x & 15) * 4 + 64 * h;
+      if (k < k1 && i < ni) vg_load4(base + (o.rows ? (int64_t)o.rows[k] : k) * o.ld + i, ni - i, o.vec, u);
+      else u[0] = u[1] = u[2] = u[3] = 0.f;
+    }
+  }
+}
+template <bool kKMajor> __device__ __forceinline__ void vg_put(float (*s)[kVgPitch], const float* v) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if constexpr (kKMajor) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[(threadIdx.x & 3) * 4 + e][(threadIdx.x >> 2) + 64 * h] = v[4 * h + e];
+    } else {
+      *reinterpret_cast<float4*>(&s[threadIdx.x >> 4][(threadIdx.x & 15) * 4 + 64 * h]) = make_float4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
+    }
+  }
+}
+
+template <typename TA, bool kAK, typename TB, bool kBK, int kMode, typename TOut>
+__global__ void __launch_bounds__(kVgThreads, 2) vloss_any_kernel(const __grid_constant__ VgProduct p) {
+  __shared__ __align__(16) float a_s[2][kVgK][kVgPitch], b_s[2][kVgK][kVgPitch];
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int64_t count = *p.count;
+  const int64_t m = p.token_axis == 0 ? min(p.m, count) : p.m, kend = p.token_axis == 2 ? min(p.k, count) : p.k;
+  const int64_t m0 = (int64_t)blockIdx.x * kVgTile, n0 = (int64_t)blockIdx.y * kVgTile;
+  const int64_t k_first = (int64_t)blockIdx.z * p.split_len, k_last = min(kend, k_first + p.split_len);
+  if (m0 >= m) return;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  float2 acc[8][4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = make_float2(0.f, 0.f);
+  float fa[8], fb[8];
+  if (k_first < k_last) {
+    vg_fetch<TA, kAK>(p.a, m0, m, k_first, k_last, fa);
+    vg_fetch<TB, kBK>(p.b, n0, p.n, k_first, k_last, fb);
+    vg_put<kAK>(a_s[0], fa);
+    vg_put<kBK>(b_s[0], fb);
+  }
+  __syncthreads();
+  int buf = 0;
+  for (int64_t k0 = k_first; k0 < k_last; k0 += kVgK, buf ^= 1) {
+    const bool next = k0 + kVgK < k_last;
+    if (next) {
+      vg_fetch<TA, kAK>(p.a, m0, m, k0 + kVgK, k_last, fa);
+      vg_fetch<TB, kBK>(p.b, n0, p.n, k0 + kVgK, k_last, fb);
+    }
+#pragma unroll
+    for (int k = 0; k < kVgK; ++k) {
+      const float4 a0 = *reinterpret_cast<const float4*>(&a_s[buf][k][ty * 4]), a1 = *reinterpret_cast<const float4*>(&a_s[buf][k][64 + ty * 4]);
+      const float4 b0 = *reinterpret_cast<const float4*>(&b_s[buf][k][tx * 4]), b1 = *reinterpret_cast<const float4*>(&b_s[buf][k][64 + tx * 4]);
+      const float av[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
+      const float2 bv[4] = {make_float2(b0.x, b0.y), make_float2(b0.z, b0.w), make_float2(b1.x, b1.y), make_float2(b1.z, b1.w)};
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = fma2(make_float2(av[i], av[i]), bv[j], acc[i][j]);
+    }
+    if (next) {
+      vg_put<kAK>(a_s[buf ^ 1], fa);
+      vg_put<kBK>(b_s[buf ^ 1], fb);
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t row = m0 + (i < 4 ? ty * 4 + i : 64 + ty * 4 + i - 4);
+    const bool live = row < m;
+    float v[8];
+    int64_t col[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[j] = j & 1 ? acc[i][j >> 1].y : acc[i][j >> 1].x;
+      col[j] = n0 + (j < 4 ? tx * 4 + j : 64 + tx * 4 + j - 4);
+    }
+    if constexpr (kMode == kVgStats) {
+      const int64_t label = live ? (int64_t)p.l.plan.label[row] : -1;
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (live && col[j] == label) p.l.mine[row] = v[j];
+        if (col[j] < p.n) top = fmaxf(top, v[j]);
+      }
+#pragma unroll
+      for (int o = 8; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum += col[j] < p.n ? vl_weight(v[j], top) : 0.f;
+#pragma unroll
+      for (int o = 8; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (live && tx == 0) p.l.part[row * p.l.tiles + blockIdx.y] = make_float2(top, sum);
+    } else if (live) {
+      if constexpr (kMode == kVgLogitGrad) {
+        const float2 lse = p.l.plan.lse[row];
+        const float g = p.l.g[row];
+        const int64_t label = (int64_t)p.l.plan.label[row] - p.col0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (col[j] < p.n) reinterpret_cast<float*>(p.l.dl)[row * p.l.piece + col[j]] = g * (exp2f(fmaf(v[j] - lse.x, kLog2e, -lse.y)) - (col[j] == label ? 1.f : 0.f));
+      } else if constexpr (kMode == kVgShare) {
+        float* out = p.l.acc + ((int64_t)blockIdx.z * p.l.tokens + row) * p.n;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (col[j] < p.n) out[col[j]] = p.more ? out[col[j]] + v[j] : v[j];
+      } else {
+        const float back = p.l.g_scale[1];
+        TOut* out = reinterpret_cast<TOut*>(p.l.dw) + (p.col0 + row) * p.n;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (col[j] < p.n) out[col[j]] = from_f32<TOut>(v[j] * back);
+      }
+    }
+  }
+}
+
+template <typename TA, bool kAK, typename TB, bool kBK, int kMode, typename TOut> static int vg_launch(const VgProduct& p, cudaStream_t st) {
+  const int64_t mt = (p.m + kVgTile - 1) / kVgTile, nt = (p.n + kVgTile - 1) / kVgTile;
+  if (nt > 65535 || mt > INT32_MAX) return fail(TKV_ERR_UNSUPPORTED, "tkv_vloss: %lld x %lld tiles", (long long)mt, (long long)nt);
+  cudaError_t e = launch_pdl(vloss_any_kernel<TA, kAK, TB, kBK, kMode, TOut>, dim3((unsigned)mt, (unsigned)nt, p.split), dim3(kVgThreads), 0, st, p);
+  if (e != cudaSuccess) return fail(TKV_ERR_LAUNCH, "tkv_vloss: %s", cudaGetErrorString(e));
+  return check_launch("tkv_vloss");
+}
+
+static bool vec4(const void* p, int64_t ld, int size) { return ((uintptr_t)p | (uintptr_t)(ld * size)) % (size * 4) == 0; }
+
+template <typename T> static int vloss_any_forward(Vloss l, cudaStream_t st) {
+  VgProduct p = {};
+  p.a = {l.x, l.x_stride, l.plan.rows, vec4(l.x, l.x_stride, sizeof(T))};
+  p.b = {l.w, l.width, nullptr, vec4(l.w, l.width, sizeof(T))};
+  p.m = l.tokens; p.n = l.vocab; p.k = l.width; p.count = l.plan.head; p.token_axis = 0;
+  p.split = 1; p.split_len = l.width; p.l = l;
+  return vg_launch<T, true, T, true, kVgStats, T>(p, st);
+}
+
+// Pieces of the vocabulary: up to 64 MB of dL, whole tiles.
+static int64_t any_piece(int tokens, int64_t vocab) {
+  int64_t n = ((int64_t)64 << 20) / (4 * (int64_t)(tokens > 0 ? tokens : 1)) / kVgTile * kVgTile;
+  if (n < 1024) n = 1024;
+  return n < vocab ? n : vl_round(vocab, 4);
+}
+// Shares of dx's inner axis, so that its few tiles of [tokens, width] fill the GPU.
+static int any_slots(int tokens, int width, int64_t piece) {
+  const int64_t tiles = ((tokens + kVgTile - 1) / kVgTile) * (int64_t)((width + kVgTile - 1) / kVgTile);
+  int64_t s = (2 * 148 + tiles - 1) / (tiles > 0 ? tiles : 1), most = (piece + 255) / 256;
+  if (s > most) s = most;
+  return (int)(s < 1 ? 1 : s > 32 ? 32 : s);
+}
+
+template <typename T> static int vloss_any_backward(Vloss l, bool want_dx, cudaStream_t st) {
+  for (int64_t v0 = 0; v0 < l.vocab; v0 += l.piece) {
+    const int64_t n = l.vocab - v0 < l.piece ? l.vocab - v0 : l.piece;
+    const T* w = reinterpret_cast<const T*>(l.w) + v0 * l.width;
+    VgProduct p = {};
+    p.count = l.plan.head; p.col0 = v0; p.l = l; p.split = 1;
+    const VgOperand x = {l.x, l.x_stride, l.plan.rows, vec4(l.x, l.x_stride, sizeof(T))}, wk = {w, l.width, nullptr, vec4(w, l.width, sizeof(T))},
+                    dl = {l.dl, l.piece, nullptr, vec4(l.dl, l.piece, 4)};
+    p.a = x; p.b = wk; p.m = l.tokens; p.n = n; p.k = p.split_len = l.width; p.token_axis = 0;
+    int rc = vg_launch<T, true, T, true, kVgLogitGrad, T>(p, st);
+    if (rc == TKV_OK && want_dx) {
+      p.a = dl; p.b = wk; p.m = l.tokens; p.n = l.width; p.k = n; p.token_axis = 0;
+      p.split = l.slots; p.split_len = vl_round((n + l.slots - 1) / l.slots, kVgK); p.more = v0 > 0;
+      rc = vg_launch<float, true, T, false, kVgShare, T>(p, st);
+    }
+    if (rc == TKV_OK && l.dw) {
+      p.a = dl; p.b = x; p.m = n; p.n = l.width; p.k = p.split_len = l.tokens; p.token_axis = 2; p.split = 1;
+      rc = vg_launch<float, false, T, false, kVgOut, T>(p, st);
+    }
+    if (rc != TKV_OK) return rc;
+  }
+  return TKV_OK;
+}
+
+// ---------------------------------------------------------------------------------------------- joining, gradients of the rows
+constexpr int kJoinThreads = 128;
+
+// A CTA per token that counts: lse from the tiles' maxima and sums, loss.
+__global__ void __launch_bounds__(kJoinThreads) vloss_join_kernel(Vloss p, float* loss) {
+  __shared__ float red[2][kJoinThreads / 32];
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (row >= p.plan.head[0]) return;
+  const float2* part = p.part + (int64_t)row * p.tiles;
+  float top = -INFINITY, sum = 0.f;
+  for (int i = threadIdx.x; i < p.tiles; i += kJoinThreads) {
+    const float2 x = part[i];
+    const float next = fmaxf(top, x.x);
+    sum = sum * vl_weight(top, next) + x.y * vl_weight(x.x, next);
+    top = next;
+  }
+  float all = top;
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
+  if (lane == 0) red[0][warp] = all;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / 32; ++w) all = fmaxf(all, red[0][w]);
+  sum = warp_add(sum * vl_weight(top, all));
+  if (lane == 0) red[1][warp] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinThreads / 32; ++w) sum += red[1][w];
+    p.plan.lse[row] = make_float2(all, log2f(sum));
+    loss[p.plan.rows[row]] = (all - p.mine[row]) + logf(sum);   // maximum and label first: they are often the same number
+  }
+}
+
+constexpr int kSumThreads = 1024;
+
+// Sum (reduction 2) or mean (1) of the losses, in fp64, in a fixed order.
+__global__ void __launch_bounds__(kSumThreads) vloss_sum_kernel(const float* loss, int tokens, VlossPlan plan, int reduction, float* out) {
+  __shared__ double red[kSumThreads / 32];
+  grid_dependency_wait();
+  grid_launch_dependents();
+  double s = 0.0;
+  for (int t = threadIdx.x; t < tokens; t += kSumThreads) s += (double)loss[t];
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = 0.0;
+    for (int w = 0; w < kSumThreads / 32; ++w) s += red[w];
+    *out = (float)(reduction == 1 ? s / (double)plan.head[0] : s);
+  }
+}
+
+// Gradient of every counting row's loss, times a power of two that brings the largest to about 2^14: fp16 keeps what is small beside it
+// (a mean over many tokens makes all of them small), and exponents of bf16 and fp32 are only shifted.
+__global__ void __launch_bounds__(kSumThreads) vloss_rows_grad_kernel(const float* grad, int64_t stride, int reduction, VlossPlan plan, float* g, float* scale) {
+  __shared__ float red[kSumThreads / 32];
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int n = plan.head[0];
+  const float by = reduction == 1 ? 1.0f / (float)n : 1.0f;
+  float top = 0.f;
+  for (int i = threadIdx.x; i < n; i += kSumThreads) top = fmaxf(top, fabsf(grad[(int64_t)plan.rows[i] * stride] * by));
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kSumThreads / 32; ++w) top = fmaxf(top, red[w]);
+  int e = 0;
+  if (top > 0.f && top < INFINITY) e = min(max(14 - ilogbf(top), -100), 100);
+  const float s = ldexpf(1.f, e);
+  for (int i = threadIdx.x; i < n; i += kSumThreads) g[i] = grad[(int64_t)plan.rows[i] * stride] * by * s;
+  if (threadIdx.x == 0) { scale[0] = s; scale[1] = ldexpf(1.f, -e); }
+}
+
+constexpr int kDxThreads = 256;
+
+// dx: the shares of a row added up in order, in the caller's type and place; zeros for tokens that do not count.  The rows of the plan are
+// in order, so a token finds itself there by halving.
+template <typename T> __global__ void __launch_bounds__(kDxThreads) vloss_dx_kernel(Vloss p, T* dx) {
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int t = blockIdx.x, n = p.plan.head[0];
+  int lo = 0, hi = n;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (p.plan.rows[mid] < t) lo = mid + 1; else hi = mid;
+  }
+  const bool live = lo < n && p.plan.rows[lo] == t;
+  const float back = p.g_scale[1];
+  T* out = dx + (int64_t)t * p.width;
+  if (p.width % 8 == 0) {
+    for (int c = threadIdx.x * 8; c < p.width; c += kDxThreads * 8) {
+      float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (live)
+        for (int i = 0; i < p.slots; ++i) {
+          float v[8];
+          load_vec<8>(p.acc + ((int64_t)i * p.tokens + lo) * p.width + c, v);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) s[e] += v[e];
+        }
+      alignas(16) T e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(s[i] * back);
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) st16(reinterpret_cast<char*>(out + c) + 16 * i, *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(e) + 16 * i));
+    }
+    return;
+  }
+  for (int c = threadIdx.x; c < p.width; c += kDxThreads) {
+    float s = 0.f;
+    if (live)
+      for (int i = 0; i < p.slots; ++i) s += p.acc[((int64_t)i * p.tokens + lo) * p.width + c];
+    out[c] = from_f32<T>(s * back);
+  }
+}
+
+template <typename... A> static int vl_launch(const char* what, void (*kernel)(A...), dim3 grid, int threads, cudaStream_t st, A... args) {
+  cudaError_t e = launch_pdl(kernel, grid, dim3(threads), 0, st, args...);
+  if (e != cudaSuccess) return fail(TKV_ERR_LAUNCH, "%s: %s", what, cudaGetErrorString(e));
+  return check_launch(what);
+}
+
+static int64_t pad256(int64_t bytes) { return vl_round(bytes, 256); }
+static int64_t any_forward_bytes(int tokens, int64_t vocab) { return (int64_t)tokens * ((vocab + kVgTile - 1) / kVgTile) * 8; }
+static int64_t any_backward_bytes(int tokens, int64_t vocab, int width, bool dx) {
+  const int64_t piece = any_piece(tokens, vocab);
+  return pad256((int64_t)tokens * piece * 4) + (dx ? (int64_t)any_slots(tokens, width, piece) * tokens * width * 4 : 0);
+}
+static int check_sizes(const char* what, int64_t tokens, int64_t vocab, int width, int64_t x_stride, int dtype) {
+  if (tokens < 0 || vocab < 1 || width < 1 || elem_size(dtype) == 0 || (tokens > 1 && x_stride < width))
+    return fail(TKV_ERR_ARG, "%s: tokens=%lld vocab=%lld width=%d rows %lld apart dtype=%d", what, (long long)tokens, (long long)vocab, width, (long long)x_stride, dtype);
+  if (tokens > (1 << 24) || vocab > (1 << 23) || width > 65536)
+    return fail(TKV_ERR_UNSUPPORTED, "%s: tokens=%lld (at most 2^24) vocab=%lld (2^23) width=%d (65536)", what, (long long)tokens, (long long)vocab, width);
+  return TKV_OK;
+}
+
+}  // namespace tkv
+
+extern "C" int64_t tkv_vloss_plan_words(int64_t tokens) { return 4 + 4 * (tokens > 0 ? tokens : 0); }
+
+extern "C" int64_t tkv_vloss_workspace_bytes(int64_t tokens, int64_t vocab, int width, int dtype, int backward, int want_dx) {
+  using namespace tkv;
+  if (check_sizes("tkv_vloss_workspace_bytes", tokens, vocab, width, width, dtype) != TKV_OK) return -1;
+  const int t = (int)tokens;
+  return 512 + pad256((int64_t)t * 4) + (backward ? any_backward_bytes(t, vocab, width, want_dx != 0) : any_forward_bytes(t, vocab));
+}
+
+extern "C" int tkv_vloss_forward(const void* x, int64_t x_stride, const void* w, const int64_t* labels, int64_t ignore, int64_t tokens,
+                                 int64_t vocab, int width, int reduction, float* loss, float* reduced, int32_t* plan, void* workspace,
+                                 int64_t workspace_bytes, int dtype, int32_t* status, tkv_stream_t stream) {
+  using namespace tkv;
+  const int rc0 = check_sizes("tkv_vloss_forward", tokens, vocab, width, x_stride, dtype);
+  if (rc0 != TKV_OK) return rc0;
+  if (reduction < 0 || reduction > 2) return fail(TKV_ERR_ARG, "tkv_vloss_forward: reduction=%d", reduction);
+  if (!plan || !workspace || (reduction && !reduced) || (tokens && (!x || !w || !labels || !loss))) return fail(TKV_ERR_ARG, "tkv_vloss_forward: NULL pointer argument");
+  if (!aligned16(workspace) || workspace_bytes < tkv_vloss_workspace_bytes(tokens, vocab, width, dtype, 0, 0))
+    return fail(TKV_ERR_ARG, "tkv_vloss_forward: workspace of %lld bytes", (long long)workspace_bytes);
+  cudaStream_t st = (cudaStream_t)stream;
+  Vloss p = {};
+  p.x = x; p.x_stride = x_stride; p.w = w; p.vocab = vocab; p.tokens = (int)tokens; p.width = width; p.dtype = dtype;
+  p.plan = vloss_plan(plan, tokens); p.status = status;
+  p.mine = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + 512);
+  void* rest = reinterpret_cast<char*>(p.mine) + pad256(tokens * 4);
+  int rc = vl_launch("tkv_vloss_forward", vloss_plan_kernel, dim3(1), kPlanThreads, st, labels, ignore, p.tokens, vocab, p.plan, loss, status);
+  if (rc == TKV_OK && tokens) {
+    p.part = reinterpret_cast<float2*>(rest);
+    p.tiles = (int)((vocab + kVgTile - 1) / kVgTile);
+    rc = dtype == TKV_F32 ? vloss_any_forward<float>(p, st) : dtype == TKV_BF16 ? vloss_any_forward<__nv_bfloat16>(p, st) : vloss_any_forward<__half>(p, st);
+    if (rc == TKV_OK) rc = vl_launch("tkv_vloss_forward", vloss_join_kernel, dim3((unsigned)tokens), kJoinThreads, st, p, loss);
+  }
+  if (rc == TKV_OK && reduction) rc = vl_launch("tkv_vloss_forward", vloss_sum_kernel, dim3(1), kSumThreads, st, (const float*)loss, p.tokens, p.plan, reduction, reduced);
+  return rc;
+}
+
+extern "C" int tkv_vloss_backward(const void* x, int64_t x_stride, const void* w, const int32_t* plan, const float* grad, int64_t grad_stride,
+                                  int reduction, int64_t tokens, int64_t vocab, int width, void* dx, void* dw, void* workspace,
+                                  int64_t workspace_bytes, int dtype, int32_t* status, tkv_stream_t stream) {
+  using namespace tkv;
+  const int rc0 = check_sizes("tkv_vloss_backward", tokens, vocab, width, x_stride, dtype);
+  if (rc0 != TKV_OK) return rc0;
+  if (reduction < 0 || reduction > 2) return fail(TKV_ERR_ARG, "tkv_vloss_backward: reduction=%d", reduction);
+  cudaStream_t st = (cudaStream_t)stream;
+  if (tokens == 0) {
+    if (dw && cudaMemsetAsync(dw, 0, (size_t)vocab * width * elem_size(dtype), st) != cudaSuccess) return check_launch("tkv_vloss_backward");
+    return TKV_OK;
+  }
+  if (!plan || !workspace || !w || !grad || (!dx && !dw) || !x) return fail(TKV_ERR_ARG, "tkv_vloss_backward: NULL pointer argument");
+  if (!aligned16(workspace) || workspace_bytes < tkv_vloss_workspace_bytes(tokens, vocab, width, dtype, 1, dx != nullptr))
+    return fail(TKV_ERR_ARG, "tkv_vloss_backward: workspace of %lld bytes", (long long)workspace_bytes);
+  if (dx && width % 8 == 0 && !aligned16(dx)) return fail(TKV_ERR_ARG, "tkv_vloss_backward: dx must be 16-byte aligned");
+  Vloss p = {};
+  p.x = x; p.x_stride = x_stride; p.w = w; p.vocab = vocab; p.tokens = (int)tokens; p.width = width; p.dtype = dtype;
+  p.plan = vloss_plan(const_cast<int32_t*>(plan), tokens); p.status = status; p.dw = dw;
+  float* scale = reinterpret_cast<float*>(workspace);
+  float* g = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + 512);
+  char* rest = reinterpret_cast<char*>(g) + pad256(tokens * 4);
+  p.g = g; p.g_scale = scale;
+  int rc = vl_launch("tkv_vloss_backward", vloss_rows_grad_kernel, dim3(1), kSumThreads, st, grad, grad_stride, reduction, p.plan, g, scale);
+  if (rc != TKV_OK) return rc;
+  p.piece = any_piece(p.tokens, vocab);
+  p.slots = any_slots(p.tokens, width, p.piece);
+  p.dl = rest;
+  p.acc = reinterpret_cast<float*>(rest + pad256(tokens * p.piece * 4));
+  rc = dtype == TKV_F32 ? vloss_any_backward<float>(p, dx != nullptr, st)
+                        : dtype == TKV_BF16 ? vloss_any_backward<__nv_bfloat16>(p, dx != nullptr, st) : vloss_any_backward<__half>(p, dx != nullptr, st);
+  if (rc != TKV_OK || dx == nullptr) return rc;
+  if (dtype == TKV_F32) return vl_launch("tkv_vloss_backward", vloss_dx_kernel<float>, dim3((unsigned)tokens), kDxThreads, st, p, (float*)dx);
+  if (dtype == TKV_BF16) return vl_launch("tkv_vloss_backward", vloss_dx_kernel<__nv_bfloat16>, dim3((unsigned)tokens), kDxThreads, st, p, (__nv_bfloat16*)dx);
+  return vl_launch("tkv_vloss_backward", vloss_dx_kernel<__half>, dim3((unsigned)tokens), kDxThreads, st, p, (__half*)dx);
+}

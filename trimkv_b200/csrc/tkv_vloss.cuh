@@ -1,0 +1,48 @@
+// Cross entropy of hidden rows x [tokens, width] against the vocabulary of w [vocab, width], without keeping the logits.
+//   s = x w^T,  lse_t = log sum_v exp(s_tv),  loss_t = lse_t - s_t,label
+//   dL_tv = g_t (exp(s_tv - lse_t) - [v = label_t]),  dx = dL w,  dw = dL^T x
+// The tokens that count are moved together first (their places, labels and lse are the "plan" that the backward pass starts from), so
+// that ignored ones cost nothing and nothing of them, NaN included, gets anywhere.  Then the vocabulary goes by in tiles: the forward pass
+// keeps a maximum and a sum per (token, tile), the backward pass computes the logits of a piece of the vocabulary again, turns them into
+// the piece of dL, and multiplies that with w and x.  lse is kept as the largest logit and the base-2 logarithm of the sum of the weights
+// beside it: their sum in fp32 would lose the digits that a nearly certain token's loss and gradient consist of.
+#pragma once
+#include "tkv_elem.cuh"
+
+namespace tkv {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kVlRowTile = 256;                            // workspaces hold whole tiles of rows
+
+// int32 words: [0] tokens that count, [1] is 1 if a label was out of range, then lse (two fp32), rows and labels of the tokens that count.
+struct VlossPlan {
+  int32_t* head; float2* lse; int32_t* rows; int32_t* label;
+};
+inline __host__ __device__ VlossPlan vloss_plan(int32_t* p, int64_t tokens) {
+  return {p, reinterpret_cast<float2*>(p + 4), p + 4 + 2 * tokens, p + 4 + 3 * tokens};
+}
+
+// exp(x - top) of a logit or a maximum x <= top; nothing counts for nothing where there is no maximum yet.
+__device__ __forceinline__ float vl_weight(float x, float top) { return x == -INFINITY ? 0.f : exp2f((x - top) * kLog2e); }
+
+struct Vloss {
+  const void* x; int64_t x_stride;                         // rows of the caller
+  const void* w;
+  int64_t vocab;
+  int tokens, width, dtype;
+  VlossPlan plan;
+  int32_t* status;
+  // forward
+  float2* part; int tiles;                                 // [tokens][tiles] largest logit of a tile, sum of the weights beside it
+  float* mine;                                             // [tokens] logit of the label
+  // backward
+  const float* g;                                          // [tokens] gradient of each counting row's loss, times g_scale
+  const float* g_scale;                                    // [2] scale and its inverse
+  void* dl; int64_t piece;                                 // [tokens][piece]
+  float* acc; int slots;                                   // [slots][tokens][width] shares of dx
+  void* dw;
+};
+
+inline int64_t vl_round(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+}  // namespace tkv

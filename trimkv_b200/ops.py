@@ -5,6 +5,7 @@ CUDA kernels of libtrimkv_b200.so.
 """
 from __future__ import annotations
 
+import contextlib
 from array import array
 from typing import Optional
 
@@ -780,6 +781,13 @@ def latent_decode(q_abs, q, rot_dim: int, freq, ring, batch, scale: float, out, 
 def moe_route(logits, correction, identity: int, top: int, groups: int, keep: int, scale: float):
     """``(place [T, top], weight [T, top], src [T * top], offsets)`` of fp32 router logits (see tkv_moe_route in the header)."""
     T, E = logits.shape
+    place, _, weight, src, offsets = moe_route_choice(logits, correction, identity, top, groups, keep, scale)
+    return place, weight, src, offsets
+
+
+def moe_route_choice(logits, correction, identity: int, top: int, groups: int, keep: int, scale: float):
+    """:func:`moe_route` with the experts chosen ``[T, top]`` behind the places."""
+    T, E = logits.shape
     dev = logits.device
     ints = torch.empty(3 * T * top + E - identity + 1, dtype=torch.int32, device=dev)
     place, choice, src, offsets = ints[:T * top].view(T, top), ints[T * top:2 * T * top], ints[2 * T * top:3 * T * top], ints[3 * T * top:]
@@ -789,7 +797,7 @@ def moe_route(logits, correction, identity: int, top: int, groups: int, keep: in
                               weight.data_ptr(), choice.data_ptr(), place.data_ptr(), src.data_ptr(), _ptr(counts), offsets.data_ptr(),
                               _stream(logits)), "tkv_moe_route")
     _count(2 if T > 128 else 1)
-    return place, weight, src, offsets
+    return place, choice, weight, src, offsets
 
 
 def moe_gemm(a, w, offsets, out, src=None, act: str = "none", status=None) -> None:
@@ -798,3 +806,105 @@ def moe_gemm(a, w, offsets, out, src=None, act: str = "none", status=None) -> No
                              w.shape[0], w.shape[1], w.shape[2], {"none": 0, "gelu": 1}[act], dtype_code(a.dtype), _ptr(status),
                              _stream(a)), "tkv_moe_gemm")
     _count(1)
+
+
+# --------------------------------------------------------------------------------------------------------------------
+# Operators of scoring and training passes (``positions.apply_rotary``, ``losses``): these launch on the tensors' device, whatever the
+# current one is.
+
+_here = contextlib.nullcontext()
+
+
+def on_device_of(t: torch.Tensor):
+    """A context in which ``t``'s device is the current one."""
+    if not t.is_cuda:
+        raise _lib.TrimKVNativeError("trimkv_b200 runs on CUDA tensors only (no CPU path)")
+    return _here if t.get_device() == torch.cuda.current_device() else torch.cuda.device_of(t)
+
+
+def rotary(q, k, positions, freq, layout: int, inverse: bool, scale: float):
+    """``(q', k')`` of q and k ``[B, H, S, D]`` (one of them may be None), stored token by token; see ``positions.apply_rotary``, which
+    checks the arguments."""
+    x = q if q is not None else k
+    b, _, s, d = x.shape
+    if q is not None and q.stride(3) != 1:
+        q = q.contiguous()
+    if k is not None and k.stride(3) != 1:
+        k = k.contiguous()
+    with on_device_of(x):
+        out, args = [], []
+        for t in (q, k):
+            if t is None:
+                out.append(None)
+                args += [None, 0, 0, 0, None, 0]
+                continue
+            h = t.shape[1]
+            y = torch.empty(b, s, h, d, dtype=t.dtype, device=t.device)
+            out.append(y.transpose(1, 2))
+            sb, sh, ss, _ = t.stride()
+            args += [t.data_ptr(), sb, sh, ss, y.data_ptr(), h]
+        check(lib().tkv_rotary(*args, positions.data_ptr(), _POS_BITS[positions.dtype], positions.stride(0), positions.stride(1),
+                               freq.data_ptr(), b, s, d, freq.shape[0], layout, int(inverse), float(scale), dtype_code(x.dtype), _stream(x)),
+              "tkv_rotary")
+    _count(1)
+    return out
+
+
+VLOSS_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def vloss_forward(x, w, labels, ignore: int, reduction: int, status=None):
+    """``(loss [T], reduced or None, plan)`` of rows ``x [T, H]`` against ``w [V, H]``; see ``losses.linear_cross_entropy``."""
+    (t, h), v, dt = x.shape, w.shape[0], dtype_code(x.dtype)
+    with on_device_of(x):
+        loss = torch.empty(t, dtype=torch.float32, device=x.device)
+        reduced = torch.empty((), dtype=torch.float32, device=x.device) if reduction else None
+        plan = torch.empty(lib().tkv_vloss_plan_words(t), dtype=torch.int32, device=x.device)
+        need = lib().tkv_vloss_workspace_bytes(t, v, h, dt, 0, 0)
+        ws = torch.empty(max(need, 0), dtype=torch.uint8, device=x.device)
+        check(lib().tkv_vloss_forward(x.data_ptr(), x.stride(0), w.data_ptr(), labels.data_ptr(), ignore, t, v, h, reduction, loss.data_ptr(),
+                                      _ptr(reduced), plan.data_ptr(), ws.data_ptr(), need, dt, _ptr(status), _stream(x)), "tkv_vloss_forward")
+    _count(3 + (reduction != 0))
+    return loss, reduced, plan
+
+
+def vloss_backward(x, w, plan, grad, reduction: int, want_dx: bool, want_dw: bool, status=None):
+    """``(dx or None, dw or None)``; ``grad`` fp32 ``[T]`` of every token's loss, or one number of the reduced loss."""
+    (t, h), v, dt = x.shape, w.shape[0], dtype_code(x.dtype)
+    with on_device_of(x):
+        dx = torch.empty(t, h, dtype=x.dtype, device=x.device) if want_dx else None
+        dw = torch.empty(v, h, dtype=w.dtype, device=x.device) if want_dw else None
+        need = lib().tkv_vloss_workspace_bytes(t, v, h, dt, 1, int(want_dx))
+        ws = torch.empty(max(need, 0), dtype=torch.uint8, device=x.device)
+        check(lib().tkv_vloss_backward(x.data_ptr(), x.stride(0), w.data_ptr(), plan.data_ptr(), grad.data_ptr(),
+                                       grad.stride(0) if grad.dim() else 0, reduction, t, v, h, _ptr(dx), _ptr(dw), ws.data_ptr(), need, dt,
+                                       _ptr(status), _stream(x)), "tkv_vloss_backward")
+    _count(2 + want_dx + want_dw)
+    return dx, dw
+
+
+def moe_balance(logits, choice, valid):
+    """``(loss, counts [E] int32, load)`` of router logits ``[T, E]``; ``load`` is what :func:`moe_balance_grad` takes."""
+    T, E = logits.shape
+    with on_device_of(logits):
+        dev = logits.device
+        loss, load = torch.empty((), dtype=torch.float32, device=dev), torch.empty(E + 1, dtype=torch.float32, device=dev)
+        counts = torch.empty(E, dtype=torch.int32, device=dev)
+        need = lib().tkv_moe_balance_workspace_bytes(T, E)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        check(lib().tkv_moe_balance(logits.data_ptr(), logits.stride(0), choice.data_ptr(), choice.stride(0), _POS_BITS[choice.dtype], _ptr(valid),
+                                    0 if valid is None else valid.stride(0), T, E, choice.shape[1], loss.data_ptr(), counts.data_ptr(),
+                                    load.data_ptr(), ws.data_ptr(), need, dtype_code(logits.dtype), _stream(logits)), "tkv_moe_balance")
+    _count(2 if T > 32 else 1)
+    return loss, counts, load
+
+
+def moe_balance_grad(logits, valid, load, grad):
+    T, E = logits.shape
+    with on_device_of(logits):
+        out = torch.empty(T, E, dtype=logits.dtype, device=logits.device)
+        check(lib().tkv_moe_balance_grad(logits.data_ptr(), logits.stride(0), _ptr(valid), 0 if valid is None else valid.stride(0), load.data_ptr(),
+                                         grad.data_ptr(), T, E, out.data_ptr(), E, dtype_code(logits.dtype), _stream(logits)),
+              "tkv_moe_balance_grad")
+    _count(1)
+    return out
