@@ -43,7 +43,7 @@ __global__ void __launch_bounds__(kPlanThreads) vloss_plan_kernel(const int64_t*
   }
   if (bad) { bad_any = 1; report(status, TKV_DEV_BAD_INDEX); }
   __syncthreads();
-  if (threadIdx.x == 0) { plan.head[0] = base; plan.head[1] = bad_any; }
+  if (threadIdx.x == 0) { plan.head[0] = base; plan.head[1] = bad_any; plan.head[2] = plan.head[3] = 0; }
 }
 
 // --------------------------------------------------------------------------------------------------------------- the products
@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(kJoinThreads) vloss_join_kernel(Vloss p, float
 #pragma unroll
     for (int w = 0; w < kJoinThreads / 32; ++w) sum += red[1][w];
     p.plan.lse[row] = make_float2(all, log2f(sum));
-    loss[p.plan.rows[row]] = (all - p.mine[row]) + logf(sum);   // maximum and label first: they are often the same number
+    loss[p.plan.rows[row]] = p.plan.head[2] ? __int_as_float(0x7fffffff) : (all - p.mine[row]) + logf(sum);   // maximum and label first: they are often the same number
   }
 }
 
@@ -361,7 +361,7 @@ template <typename T> __global__ void __launch_bounds__(kDxThreads) vloss_dx_ker
     if (p.plan.rows[mid] < t) lo = mid + 1; else hi = mid;
   }
   const bool live = lo < n && p.plan.rows[lo] == t;
-  const float back = p.g_scale[1];
+  const float back = p.plan.head[2] ? __int_as_float(0x7fffffff) : p.g_scale[1];
   T* out = dx + (int64_t)t * p.width;
   if (p.width % 8 == 0) {
     for (int c = threadIdx.x * 8; c < p.width; c += kDxThreads * 8) {
@@ -395,6 +395,7 @@ template <typename... A> static int vl_launch(const char* what, void (*kernel)(A
   return check_launch(what);
 }
 
+static bool use_tc(const Vloss& p) { return vloss_tc_shape(p.tokens, p.vocab, p.width, p.dtype) && aligned16(p.w) && (p.dw == nullptr || aligned16(p.dw)); }
 static int64_t pad256(int64_t bytes) { return vl_round(bytes, 256); }
 static int64_t any_forward_bytes(int tokens, int64_t vocab) { return (int64_t)tokens * ((vocab + kVgTile - 1) / kVgTile) * 8; }
 static int64_t any_backward_bytes(int tokens, int64_t vocab, int width, bool dx) {
@@ -417,7 +418,12 @@ extern "C" int64_t tkv_vloss_workspace_bytes(int64_t tokens, int64_t vocab, int 
   using namespace tkv;
   if (check_sizes("tkv_vloss_workspace_bytes", tokens, vocab, width, width, dtype) != TKV_OK) return -1;
   const int t = (int)tokens;
-  return 512 + pad256((int64_t)t * 4) + (backward ? any_backward_bytes(t, vocab, width, want_dx != 0) : any_forward_bytes(t, vocab));
+  int64_t n = backward ? any_backward_bytes(t, vocab, width, want_dx != 0) : any_forward_bytes(t, vocab);
+  if (vloss_tc_shape(t, vocab, width, dtype)) {            // which form runs is known with the addresses: room for either
+    const int64_t tc = backward ? vloss_tc_backward_bytes(t, vocab, width, want_dx != 0) : vloss_tc_forward_bytes(t, vocab, width);
+    n = n > tc ? n : tc;
+  }
+  return 512 + pad256((int64_t)t * 4) + n;
 }
 
 extern "C" int tkv_vloss_forward(const void* x, int64_t x_stride, const void* w, const int64_t* labels, int64_t ignore, int64_t tokens,
@@ -440,7 +446,7 @@ extern "C" int tkv_vloss_forward(const void* x, int64_t x_stride, const void* w,
   if (rc == TKV_OK && tokens) {
     p.part = reinterpret_cast<float2*>(rest);
     p.tiles = (int)((vocab + kVgTile - 1) / kVgTile);
-    rc = dtype == TKV_F32 ? vloss_any_forward<float>(p, st) : dtype == TKV_BF16 ? vloss_any_forward<__nv_bfloat16>(p, st) : vloss_any_forward<__half>(p, st);
+    rc = use_tc(p) ? vloss_tc_forward(p, rest, st) : dtype == TKV_F32 ? vloss_any_forward<float>(p, st) : dtype == TKV_BF16 ? vloss_any_forward<__nv_bfloat16>(p, st) : vloss_any_forward<__half>(p, st);
     if (rc == TKV_OK) rc = vl_launch("tkv_vloss_forward", vloss_join_kernel, dim3((unsigned)tokens), kJoinThreads, st, p, loss);
   }
   if (rc == TKV_OK && reduction) rc = vl_launch("tkv_vloss_forward", vloss_sum_kernel, dim3(1), kSumThreads, st, (const float*)loss, p.tokens, p.plan, reduction, reduced);
@@ -472,12 +478,16 @@ extern "C" int tkv_vloss_backward(const void* x, int64_t x_stride, const void* w
   p.g = g; p.g_scale = scale;
   int rc = vl_launch("tkv_vloss_backward", vloss_rows_grad_kernel, dim3(1), kSumThreads, st, grad, grad_stride, reduction, p.plan, g, scale);
   if (rc != TKV_OK) return rc;
-  p.piece = any_piece(p.tokens, vocab);
-  p.slots = any_slots(p.tokens, width, p.piece);
-  p.dl = rest;
-  p.acc = reinterpret_cast<float*>(rest + pad256(tokens * p.piece * 4));
-  rc = dtype == TKV_F32 ? vloss_any_backward<float>(p, dx != nullptr, st)
+  if (use_tc(p)) {
+    rc = vloss_tc_backward(p, rest, dx != nullptr, st);
+  } else {
+    p.piece = any_piece(p.tokens, vocab);
+    p.slots = any_slots(p.tokens, width, p.piece);
+    p.dl = rest;
+    p.acc = reinterpret_cast<float*>(rest + pad256(tokens * p.piece * 4));
+    rc = dtype == TKV_F32 ? vloss_any_backward<float>(p, dx != nullptr, st)
                         : dtype == TKV_BF16 ? vloss_any_backward<__nv_bfloat16>(p, dx != nullptr, st) : vloss_any_backward<__half>(p, dx != nullptr, st);
+  }
   if (rc != TKV_OK || dx == nullptr) return rc;
   if (dtype == TKV_F32) return vl_launch("tkv_vloss_backward", vloss_dx_kernel<float>, dim3((unsigned)tokens), kDxThreads, st, p, (float*)dx);
   if (dtype == TKV_BF16) return vl_launch("tkv_vloss_backward", vloss_dx_kernel<__nv_bfloat16>, dim3((unsigned)tokens), kDxThreads, st, p, (__nv_bfloat16*)dx);

@@ -14,7 +14,7 @@ namespace tkv {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kVlRowTile = 256;                            // workspaces hold whole tiles of rows
 
-// int32 words: [0] tokens that count, [1] is 1 if a label was out of range, then lse (two fp32), rows and labels of the tokens that count.
+// int32 words: [0] tokens that count, [1] is 1 if a label was out of range, [2] if a wait ran out, then lse (two fp32), rows and labels of the tokens that count.
 struct VlossPlan {
   int32_t* head; float2* lse; int32_t* rows; int32_t* label;
 };
@@ -44,5 +44,12 @@ struct Vloss {
 };
 
 inline int64_t vl_round(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+// The form on the tensor cores (tkv_vloss_tc.cu): 16-bit types, widths of whole 16-byte vectors, w and dw on 16 bytes; x of any alignment.
+bool vloss_tc_shape(int tokens, int64_t vocab, int width, int dtype);
+int64_t vloss_tc_forward_bytes(int tokens, int64_t vocab, int width);
+int64_t vloss_tc_backward_bytes(int tokens, int64_t vocab, int width, bool dx);
+int vloss_tc_forward(Vloss& p, void* ws, cudaStream_t st);                   // fills part and mine, sets tiles
+int vloss_tc_backward(Vloss& p, void* ws, bool want_dx, cudaStream_t st);    // fills dw and acc, sets slots
 
 }  // namespace tkv

@@ -1,0 +1,507 @@
+// Cross entropy against a vocabulary (tkv_vloss.cuh) on tcgen05 + TMEM, for 16-bit types:
+//   kVtStats  : logits of 256 tokens x up to 256 words -> largest logit and sum of weights of every token, logit of its label;
+//   kVtLogits : the same logits again -> a tile of dL in the type of the operands;
+//   kVtGrads  : dx shares (dL w, both read along the vocabulary) and dw (dL^T x, both read along the tokens) of a piece, one launch.
+//
+// Bound by the tensor cores.  A tile belongs to a pair of CTAs (cta_group::2): each holds 128 of its 256 rows and, of every stage of 64
+// along the inner axis, its rows of A and half of B, 32 KB; the products read the other half from the neighbour, so that a CTA fetches
+// 32 KB for the work for which a CTA alone fetches 48.  Six stages; two accumulators of 256 TMEM columns, so that a tile's epilogue runs
+// beside the next tile's products.  One pair per two SMs, tiles in turn: row tiles innermost, in groups whose rows stay in L2, so that a
+// tile of w comes from HBM once per group.
+// What is stored along the inner axis (x, w in the logits; dL for dx) is read K-major, what is stored across it MN-major: nothing is
+// transposed in memory.
+//
+// Copies of both CTAs complete on the even CTA's barriers; it issues the products; their completion is told to both.  Every wait is
+// bounded; a CTA whose wait runs out records TKV_DEV_TIMEOUT, in the plan too (losses and dx become NaN), and tells its neighbour; both
+// drain and free their TMEM.
+#include <cuda.h>
+#include "tkv_vloss.cuh"
+#include "tkv_tc.cuh"
+
+namespace tkv {
+
+constexpr int kVtThreads = 192;                            // warp 0: copies, warp 1: products, warps 2-5: epilogue
+constexpr int kVtK = 64, kVtRows = 256, kVtCols = 256, kVtStages = 6;
+constexpr int kVtABytes = 128 * kVtK * 2, kVtBBytes = 128 * kVtK * 2, kVtStage = kVtABytes + kVtBBytes;
+constexpr int kVtGroup = 32;                               // row tiles that share a pass over w
+constexpr int kVtPairs = 74;
+
+enum { kVtStats, kVtLogits, kVtGrads };
+
+struct VtSmem {
+  uint64_t full[kVtStages], empty[kVtStages], acc_full[2], acc_empty[2];
+  uint32_t tmem_base;
+  int abort_flag;
+};
+constexpr int kVtSmemBytes = kVtStages * kVtStage + (int)sizeof(VtSmem);
+
+struct VtParams {
+  Vloss l;
+  int cols;                                                // of a tile (a multiple of 16)
+  int64_t v0, piece_cols;                                  // the vocabulary from v0 (kVtStats: all of it)
+  int64_t piece_pitch;
+  int want_dx, want_dw, more, split_steps;                 // kVtGrads: stages of a share of dx
+};
+
+// ---- instructions for pairs of CTAs
+__device__ __forceinline__ uint32_t vt_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ uint32_t vt_of_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void vt_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void vt_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+               ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void vt_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accum) : "memory");
+}
+__device__ __forceinline__ void vt_commit(uint64_t* bar) {  // to both CTAs
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ void vt_arrive(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ void vt_raise(uint32_t cluster_addr) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(1) : "memory");
+}
+// kind::f16 of a pair: D fp32, M = 256, N = n; which operands lie across the inner axis.
+__device__ __forceinline__ uint32_t vt_idesc(int bf16, int a_mn, int b_mn, int n) {
+  return (1u << 4) | ((uint32_t)bf16 << 7) | ((uint32_t)bf16 << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | (16u << 24);
+}
+
+// A pair's tiles in order; every role keeps its own.
+struct VtTile {
+  int dx;                                                  // kVtGrads: 1 for a share of dx, 0 for dw
+  int row0, col0, slot, step0, steps;                      // of 256 rows and `cols` columns; stages of the inner axis
+};
+template <int kMode> struct VtTiles {
+  const VtParams& p;
+  int n, tile, count, dx_count, mt, nt, ht, vt, slots;
+  __device__ __forceinline__ VtTiles(const VtParams& q, int pair) : p(q) {
+    n = q.l.plan.head[0];
+    tile = pair - kVtPairs;
+    mt = (n + kVtRows - 1) / kVtRows;
+    if (kMode == kVtGrads) {
+      ht = (q.l.width + kVtCols - 1) / kVtCols;
+      vt = (int)((q.piece_cols + kVtRows - 1) / kVtRows);
+      slots = q.l.slots;
+      dx_count = q.want_dx ? mt * ht * slots : 0;
+      count = dx_count + (q.want_dw ? vt * ht : 0);
+    } else {
+      nt = (int)((q.piece_cols + q.cols - 1) / q.cols);
+      count = mt * nt;
+    }
+  }
+  __device__ __forceinline__ bool next(VtTile& t) {
+    tile += kVtPairs;
+    if (tile >= count) return false;
+    if (kMode == kVtGrads) {
+      t.dx = tile < dx_count;
+      const int i = t.dx ? tile : tile - dx_count;
+      t.col0 = i % ht * kVtCols;
+      const int r = i / ht;
+      if (t.dx) {
+        t.row0 = r / slots * kVtRows;
+        t.slot = r % slots;
+        t.step0 = t.slot * p.split_steps;
+        t.steps = max(0, min(p.split_steps, (int)((p.piece_cols + kVtK - 1) / kVtK) - t.step0));
+      } else {
+        t.row0 = r * kVtRows;
+        t.slot = t.step0 = 0;
+        t.steps = (n + kVtK - 1) / kVtK;
+      }
+    } else {
+      const int per = kVtGroup * nt, g = tile / per, r = tile - g * per, rows = min(kVtGroup, mt - g * kVtGroup);
+      t.dx = t.slot = t.step0 = 0;
+      t.row0 = (g * kVtGroup + r % rows) * kVtRows;
+      t.col0 = r / rows * p.cols;
+      t.steps = (p.l.width + kVtK - 1) / kVtK;
+    }
+    return true;
+  }
+};
+
+template <typename T> __device__ __forceinline__ uint32_t vt_pack(float a, float b) {
+  if constexpr (sizeof(T) == 2 && __is_same(T, __half)) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+// Maps: a, b of the logits (x, w, K-major); of the gradients dL along and across (a, a2), w across (b), x across (b2).
+template <int kMode, typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kVtThreads, 1)
+vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_a2,
+                const __grid_constant__ CUtensorMap map_b2, const __grid_constant__ VtParams p) {
+  extern __shared__ __align__(1024) uint8_t base[];
+  VtSmem* sm = reinterpret_cast<VtSmem*>(base + kVtStages * kVtStage);
+  const int tid = threadIdx.x, warp = warp_uniform(tid >> 5), lane = tid & 31;
+  const int rank = (int)vt_rank(), pair = blockIdx.x >> 1;
+  volatile int* abort_flag = &sm->abort_flag;
+  const uint32_t peer_abort = vt_of_rank(smem_u32(&sm->abort_flag), rank ^ 1);
+  if (tid == 0) {
+    for (int s = 0; s < kVtStages; ++s) { mbar_init(&sm->full[s], 1); mbar_init(&sm->empty[s], 1); }
+    for (int s = 0; s < 2; ++s) { mbar_init(&sm->acc_full[s], 1); mbar_init(&sm->acc_empty[s], 8); }
+    sm->abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm->tmem_base)), "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+  }
+  grid_dependency_wait();
+  grid_launch_dependents();
+  tc_fence_before();
+  __syncthreads();
+  vt_cluster_sync();                                       // both CTAs' barriers are there
+  tc_fence_after();
+  const uint32_t tmem = sm->tmem_base;
+  auto give_up = [&]() {
+    if (*abort_flag == 0) { report(p.l.status, TKV_DEV_TIMEOUT); p.l.plan.head[2] = 1; }
+    *abort_flag = 1;
+    vt_raise(peer_abort);
+  };
+  if ((smem_u32(base) & 1023u) != 0 && tid == 0) give_up();   // the swizzled tiles need the alignment; the launch gives it
+  __syncthreads();
+  VtTiles<kMode> tiles(p, pair);
+  VtTile t;
+  int copies = 0;                                          // stages whose copies this CTA has started
+
+  if (warp == 0) {
+    bool ok = (bool)__all_sync(0xffffffffu, *abort_flag == 0);
+    int it = 0;
+    while (ok && tiles.next(t)) {
+      const bool a_mn = kMode == kVtGrads && !t.dx, b_mn = kMode == kVtGrads;
+      const int half = kMode == kVtGrads ? kVtCols / 2 : p.cols / 2;
+      const uint32_t bytes = 2 * (kVtABytes + half * kVtK * 2);          // of both CTAs
+      const int arow = t.row0 + rank * 128, brow = t.col0 + rank * half;
+      for (int k = t.step0; k < t.step0 + t.steps; ++k, ++it) {
+        const int s = it % kVtStages;
+        ok = warp_wait(&sm->empty[s], ((it / kVtStages) & 1) ^ 1, abort_flag);
+        if (!ok) break;
+        if (elect_one()) {
+          const uint32_t bar = vt_of_rank(smem_u32(&sm->full[s]), 0), a = smem_u32(base + s * kVtStage), b = a + kVtABytes;
+          if (rank == 0) mbar_expect_tx(&sm->full[s], bytes);
+          if (a_mn) {
+            vt_load(a, &map_a2, bar, arow, k * kVtK);
+            vt_load(a + kVtABytes / 2, &map_a2, bar, arow + 64, k * kVtK);
+          } else {
+            vt_load(a, &map_a, bar, k * kVtK, arow);
+          }
+          if (b_mn) {
+            const CUtensorMap* mb = t.dx ? &map_b : &map_b2;
+            const int y = k * kVtK + (t.dx ? (int)p.v0 : 0);
+            vt_load(b, mb, bar, brow, y);
+            vt_load(b + kVtBBytes / 2, mb, bar, brow + 64, y);
+          } else {
+            vt_load(b, &map_b, bar, k * kVtK, (int)p.v0 + brow);
+          }
+        }
+        __syncwarp();
+      }
+    }
+    // the last stages' products are told to this CTA before it may leave
+    for (int i = max(0, it - kVtStages); ok && i < it; ++i) ok = warp_wait(&sm->empty[i % kVtStages], (i / kVtStages) & 1, abort_flag);
+    if (!ok && lane == 0) give_up();
+    copies = it;
+  } else if (warp == 1) {
+    if (rank == 0) {
+      const uint32_t tm = warp_uniform(tmem);
+      const int bf16 = !__is_same(T, __half);
+      const uint64_t k_desc = make_desc(smem_u32(base), 16, 1024, 2), mn_desc = make_desc(smem_u32(base), kVtABytes / 2, 1024, 2);
+      int it = 0, acc = 0;
+      bool ok = (bool)__all_sync(0xffffffffu, *abort_flag == 0);
+      while (ok && tiles.next(t)) {
+        const bool a_mn = kMode == kVtGrads && !t.dx, b_mn = kMode == kVtGrads;
+        const uint32_t idesc = vt_idesc(bf16, a_mn, b_mn, kMode == kVtGrads ? kVtCols : p.cols);
+        const int buf = acc & 1;
+        ok = warp_wait(&sm->acc_empty[buf], ((acc >> 1) & 1) ^ 1, abort_flag);
+        tc_fence_after();
+        for (int k = 0; k < t.steps && ok; ++k, ++it) {
+          const int s = it % kVtStages;
+          ok = warp_wait(&sm->full[s], (it / kVtStages) & 1, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t at = (uint32_t)s * (kVtStage >> 4);
+            const uint64_t a = (a_mn ? mn_desc : k_desc) + at, b = (b_mn ? mn_desc : k_desc) + at + (kVtABytes >> 4);
+            const uint32_t da = a_mn ? 128 : 2, db = b_mn ? 128 : 2;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) vt_mma(tm + buf * kVtCols, a + q * da, b + q * db, idesc, (k > 0 || q > 0));
+            vt_commit(&sm->empty[s]);
+            if (k == t.steps - 1) vt_commit(&sm->acc_full[buf]);
+          }
+          __syncwarp();
+        }
+        if (ok && t.steps == 0) {                          // a share without stages: its epilogue writes zeros
+          if (elect_one()) vt_commit(&sm->acc_full[buf]);
+          __syncwarp();
+        }
+        ++acc;
+      }
+      if (!ok && lane == 0) give_up();
+    }
+    __syncwarp();
+  } else {
+    // ---- epilogue: thread = row of the CTA's half of the tile
+    const int quarter = warp & 3, row_in = quarter * 32 + lane;
+    const uint32_t acc_empty0 = vt_of_rank(smem_u32(&sm->acc_empty[0]), 0);
+    int acc = 0;
+    bool ok = *abort_flag == 0;
+    while (ok && tiles.next(t)) {
+      const int buf = acc & 1;
+      ok = (bool)__all_sync(0xffffffffu, mbar_wait_or_abort(&sm->acc_full[buf], (acc >> 1) & 1, abort_flag));
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + buf * kVtCols;
+      const int row = t.row0 + rank * 128 + row_in;
+      if constexpr (kMode == kVtStats) {
+        const bool live = row < tiles.n;
+        const int left = (int)min((int64_t)p.cols, p.piece_cols - t.col0);        // columns that exist
+        if (t.row0 + rank * 128 + quarter * 32 < tiles.n) {
+          const int label = live ? p.l.plan.label[row] - t.col0 : -1;
+          float top = -INFINITY, sum = 0.f;
+          for (int c = 0; c < left; c += 32) {
+            float v[32];
+            tmem_ld32(from + c, v);
+            if ((unsigned)(label - c) < 32u && label < left) {
+              float mine = 0.f;
+#pragma unroll
+              for (int i = 0; i < 32; ++i) mine = i == label - c ? v[i] : mine;
+              p.l.mine[row] = mine;
+            }
+            __syncwarp();
+            if (c + 32 > left) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = c + i < left ? v[i] : -INFINITY;
+            }
+            float next = top;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) next = fmaxf(next, v[i]);
+            const float from0 = next == -INFINITY ? 0.f : next;
+            float part = 0.f;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) part += exp2_weight((v[i] - from0) * kLog2e);
+            sum = fmaf(sum, exp2_weight((top - from0) * kLog2e), part);
+            top = next;
+          }
+          if (live) p.l.part[(int64_t)row * p.l.tiles + t.col0 / p.cols] = make_float2(top, sum);
+        }
+      } else if constexpr (kMode == kVtLogits) {
+        const bool live = row < tiles.n;
+        const int label = live ? (int)(p.l.plan.label[row] - p.v0 - t.col0) : -1;
+        const float2 lse = live ? p.l.plan.lse[row] : make_float2(0.f, 0.f);
+        const float g = live ? p.l.g[row] : 0.f;
+        const int left = (int)min((int64_t)p.cols, p.piece_cols - t.col0);
+        T* out = reinterpret_cast<T*>(p.l.dl) + (int64_t)row * p.piece_pitch + t.col0;
+        for (int c = 0; c < p.cols; c += 32) {
+          float v[32];
+          tmem_ld32(from + c, v);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float d = exp2_weight(fmaf(v[i] - lse.x, kLog2e, -lse.y)) - (i == label - c ? 1.f : 0.f);
+            v[i] = live && c + i < left ? g * d : 0.f;     // rows and columns that do not exist are zeros for the products to come
+          }
+#pragma unroll
+          for (int i = 0; i < 32; i += 8)
+            st16(out + c + i, make_uint4(vt_pack<T>(v[i], v[i + 1]), vt_pack<T>(v[i + 2], v[i + 3]), vt_pack<T>(v[i + 4], v[i + 5]), vt_pack<T>(v[i + 6], v[i + 7])));
+        }
+      } else {
+        const int left = p.l.width - t.col0;               // a multiple of 8
+        const bool live = t.dx ? row < tiles.n : row < p.piece_cols;
+        const float back = t.dx ? 0.f : p.l.g_scale[1];
+        float* share = p.l.acc + ((int64_t)t.slot * p.l.tokens + row) * p.l.width + t.col0;
+        T* out = reinterpret_cast<T*>(p.l.dw) + (p.v0 + row) * p.l.width + t.col0;
+        for (int c = 0; c < kVtCols && c < left; c += 32) {
+          float v[32];
+          if (t.steps > 0) tmem_ld32(from + c, v);
+          else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = 0.f;
+          }
+          if (live && t.dx) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              if (c + i < left) {
+                float4 w = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                if (p.more) {
+                  const float4 o = *reinterpret_cast<const float4*>(share + c + i);
+                  w.x += o.x; w.y += o.y; w.z += o.z; w.w += o.w;
+                }
+                *reinterpret_cast<float4*>(share + c + i) = w;
+              }
+            }
+          } else if (live) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8)
+              if (c + i < left)
+                st16(out + c + i, make_uint4(vt_pack<T>(v[i] * back, v[i + 1] * back), vt_pack<T>(v[i + 2] * back, v[i + 3] * back),
+                                             vt_pack<T>(v[i + 4] * back, v[i + 5] * back), vt_pack<T>(v[i + 6] * back, v[i + 7] * back)));
+          }
+          __syncwarp();
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) vt_arrive(acc_empty0 + buf * 8);
+      ++acc;
+    }
+    if (!ok && lane == 0) give_up();
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (tid == 0 && rank == 0 && *abort_flag != 0)           // copies in flight, the neighbour's too, land before the shared memory is released
+    for (int i = max(0, copies - kVtStages); i < copies; ++i) mbar_wait(&sm->full[i % kVtStages], (i / kVtStages) & 1);
+  __syncthreads();
+  vt_cluster_sync();                                       // nobody reads or signals a CTA that has left
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+}
+
+// -------------------------------------------------------------------------------------------------- rows that count, together
+constexpr int kVtGatherThreads = 256;
+
+// Row i of xc is the row of the i-th token that counts; zeros up to the end of the last tile of rows.
+template <bool kVec> __global__ void __launch_bounds__(kVtGatherThreads) vloss_gather_kernel(const uint16_t* x, int64_t x_stride, VlossPlan plan, int width, uint16_t* xc) {
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int n = plan.head[0];
+  const int64_t i = blockIdx.x;
+  if (i >= ((int64_t)n + kVtRows - 1) / kVtRows * kVtRows) return;
+  uint16_t* out = xc + i * width;
+  if (i >= n) {
+    for (int c = threadIdx.x * 8; c < width; c += kVtGatherThreads * 8) st16(out + c, make_uint4(0, 0, 0, 0));
+    return;
+  }
+  const uint16_t* in = x + (int64_t)plan.rows[i] * x_stride;
+  if (kVec) {
+    for (int c = threadIdx.x * 8; c < width; c += kVtGatherThreads * 8) st16(out + c, ld16_stream(in + c));
+  } else {
+    for (int c = threadIdx.x; c < width; c += kVtGatherThreads) out[c] = in[c];
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------------ the host
+bool vloss_tc_shape(int tokens, int64_t vocab, int width, int dtype) { return (dtype == TKV_BF16 || dtype == TKV_F16) && width % 8 == 0 && tokens > 0; }
+
+static int64_t vt_rows(int tokens) { return vl_round(tokens, kVtRows); }
+// Columns of a tile: the fewest that keep the number of rounds over the pairs that 256 columns need (few tokens: a last round that is
+// nearly empty costs as much as a whole one).
+static int vt_tile_cols(int tokens, int64_t vocab) {
+  const int64_t mt = vt_rows(tokens) / kVtRows, nt = (vocab + kVtCols - 1) / kVtCols, rounds = (mt * nt + kVtPairs - 1) / kVtPairs;
+  if (rounds > 16) return kVtCols;
+  int64_t most = rounds * kVtPairs / mt;                   // tiles of columns that fit those rounds
+  if (most < 1) most = 1;
+  const int64_t cols = vl_round((vocab + most - 1) / most, 16);
+  return (int)(cols < 32 ? 32 : cols > kVtCols ? kVtCols : cols);
+}
+// The vocabulary in equal pieces, of at most 256 MB of dL where that is not fewer than 8192 words.
+static int64_t vt_piece(int tokens, int64_t vocab) {
+  int64_t n = ((int64_t)256 << 20) / (2 * vt_rows(tokens)) / kVtCols * kVtCols;
+  if (n < 8192) n = 8192;
+  const int64_t pieces = (vocab + n - 1) / n;
+  return vl_round((vocab + pieces - 1) / pieces, kVtCols);
+}
+// Shares of dx: a tile of dx is as long as the piece, so where few tiles of the launch are, it is cut until it is a third of a pair's part.
+static int vt_slots(int tokens, int width, int64_t piece) {
+  const int64_t mt = vt_rows(tokens) / kVtRows, ht = (width + kVtCols - 1) / kVtCols, ks = piece / kVtK;
+  const int64_t total = mt * ht * ks;                      // stages of dx alone: it may be asked for alone
+  const int64_t part = (total + kVtPairs - 1) / kVtPairs;
+  int64_t s = (3 * ks + part - 1) / (part > 0 ? part : 1);
+  if (s > ks / 8) s = ks / 8;
+  if (mt * ht >= 2 * kVtPairs || s < 1) s = 1;
+  return (int)(s > 32 ? 32 : s);
+}
+static int64_t vt_pad(int64_t bytes) { return vl_round(bytes, 1024); }
+
+int64_t vloss_tc_forward_bytes(int tokens, int64_t vocab, int width) {
+  const int cols = vt_tile_cols(tokens, vocab);
+  return 1024 + vt_pad(vt_rows(tokens) * width * 2) + (int64_t)tokens * ((vocab + cols - 1) / cols) * 8;
+}
+int64_t vloss_tc_backward_bytes(int tokens, int64_t vocab, int width, bool dx) {
+  const int64_t piece = vt_piece(tokens, vocab);
+  return 1024 + vt_pad(vt_rows(tokens) * width * 2) + vt_pad(vt_rows(tokens) * piece * 2) + (dx ? (int64_t)vt_slots(tokens, width, piece) * tokens * width * 4 : 0);
+}
+
+static int vt_gather(const Vloss& p, void* xc, cudaStream_t st) {
+  const bool vec = aligned16(p.x) && p.x_stride % 8 == 0;
+  cudaError_t e = launch_pdl(vec ? vloss_gather_kernel<true> : vloss_gather_kernel<false>, dim3((unsigned)vt_rows(p.tokens)), dim3(kVtGatherThreads), 0, st,
+                             reinterpret_cast<const uint16_t*>(p.x), p.x_stride, p.plan, p.width, reinterpret_cast<uint16_t*>(xc));
+  if (e != cudaSuccess) return fail(TKV_ERR_LAUNCH, "tkv_vloss: %s", cudaGetErrorString(e));
+  return check_launch("tkv_vloss");
+}
+
+template <int kMode, typename T> static int vt_launch(const CUtensorMap* m, const VtParams& p, cudaStream_t st) {
+  static bool allowed[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev < 0 || dev >= 64 || !allowed[dev])) {
+    e = cudaFuncSetAttribute(vloss_tc_kernel<kMode, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kVtSmemBytes);
+    if (e == cudaSuccess && dev >= 0 && dev < 64) allowed[dev] = true;
+  }
+  if (e == cudaSuccess) e = launch_pdl(vloss_tc_kernel<kMode, T>, dim3(2 * kVtPairs), dim3(kVtThreads), (size_t)kVtSmemBytes, st, m[0], m[1], m[2], m[3], p);
+  if (e != cudaSuccess) return fail(TKV_ERR_LAUNCH, "tkv_vloss: %s", cudaGetErrorString(e));
+  return check_launch("tkv_vloss");
+}
+
+static void* vt_align(void* p) { return reinterpret_cast<void*>(((uintptr_t)p + 1023) & ~(uintptr_t)1023); }
+
+int vloss_tc_forward(Vloss& l, void* ws, cudaStream_t st) {
+  void* xc = vt_align(ws);
+  VtParams p = {};
+  p.cols = vt_tile_cols(l.tokens, l.vocab);
+  l.part = reinterpret_cast<float2*>(reinterpret_cast<char*>(xc) + vt_pad(vt_rows(l.tokens) * l.width * 2));
+  l.tiles = (int)((l.vocab + p.cols - 1) / p.cols);
+  p.l = l; p.v0 = 0; p.piece_cols = l.vocab;
+  CUtensorMap m[4];
+  int rc = vt_gather(l, xc, st);
+  if (rc == TKV_OK) rc = make_map_2d(&m[0], xc, l.width, vt_rows(l.tokens), kVtK, 128, l.dtype);
+  if (rc == TKV_OK) rc = make_map_2d(&m[1], l.w, l.width, l.vocab, kVtK, p.cols / 2, l.dtype);
+  if (rc != TKV_OK) return rc;
+  m[2] = m[3] = m[0];
+  return l.dtype == TKV_BF16 ? vt_launch<kVtStats, __nv_bfloat16>(m, p, st) : vt_launch<kVtStats, __half>(m, p, st);
+}
+
+int vloss_tc_backward(Vloss& l, void* ws, bool want_dx, cudaStream_t st) {
+  char* xc = reinterpret_cast<char*>(vt_align(ws));
+  const int64_t rows = vt_rows(l.tokens), piece = vt_piece(l.tokens, l.vocab);
+  l.dl = xc + vt_pad(rows * l.width * 2);
+  l.piece = piece;
+  l.acc = reinterpret_cast<float*>(reinterpret_cast<char*>(l.dl) + vt_pad(rows * piece * 2));
+  l.slots = vt_slots(l.tokens, l.width, piece);
+  CUtensorMap a[4], g[4];
+  int rc = vt_gather(l, xc, st);
+  if (rc == TKV_OK) rc = make_map_2d(&a[0], xc, l.width, rows, kVtK, 128, l.dtype);
+  if (rc == TKV_OK) rc = make_map_2d(&a[1], l.w, l.width, l.vocab, kVtK, 128, l.dtype);
+  if (rc == TKV_OK) rc = make_map_2d(&g[0], l.dl, piece, rows, kVtK, 128, l.dtype);
+  if (rc == TKV_OK) rc = make_map_2d(&g[1], l.w, l.width, l.vocab, 64, kVtK, l.dtype);
+  if (rc == TKV_OK) rc = make_map_2d(&g[2], l.dl, piece, rows, 64, kVtK, l.dtype);
+  if (rc == TKV_OK) rc = make_map_2d(&g[3], xc, l.width, rows, 64, kVtK, l.dtype);
+  if (rc != TKV_OK) return rc;
+  a[2] = a[3] = a[0];
+  VtParams p = {};
+  p.cols = kVtCols; p.piece_pitch = piece; p.want_dx = want_dx; p.want_dw = l.dw != nullptr; p.l = l;
+  p.split_steps = (int)((piece / kVtK + l.slots - 1) / l.slots);
+  for (int64_t v0 = 0; v0 < l.vocab && rc == TKV_OK; v0 += piece) {
+    p.v0 = v0; p.piece_cols = l.vocab - v0 < piece ? l.vocab - v0 : piece; p.more = v0 > 0;
+    if (l.dtype == TKV_BF16) {
+      rc = vt_launch<kVtLogits, __nv_bfloat16>(a, p, st);
+      if (rc == TKV_OK) rc = vt_launch<kVtGrads, __nv_bfloat16>(g, p, st);
+    } else {
+      rc = vt_launch<kVtLogits, __half>(a, p, st);
+      if (rc == TKV_OK) rc = vt_launch<kVtGrads, __half>(g, p, st);
+    }
+  }
+  return rc;
+}
+
+}  // namespace tkv
