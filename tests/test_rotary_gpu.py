@@ -202,3 +202,12 @@ def test_another_stream():
         got, _ = apply_rotary(q * 1, None, pos, freq)
     torch.cuda.current_stream().wait_stream(side)
     _close(got, *_want(q, pos[None], freq, "half", 1.0))
+
+
+def test_gradient_of_the_gradient():
+    q = torch.randn(1, 2, 4, 16, device="cuda", requires_grad=True)
+    pos, freq, g = torch.arange(4, device="cuda"), _table(8), torch.randn(1, 2, 4, 16, device="cuda", requires_grad=True)
+    d, = torch.autograd.grad(apply_rotary(q, None, pos, freq, scale=0.5)[0], q, g, create_graph=True)
+    v = torch.randn_like(q)
+    back, = torch.autograd.grad(d, g, v)                            # of a linear map: the map itself
+    _close(back, *_want(v, pos[None], freq, "half", 0.5))

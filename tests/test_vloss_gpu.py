@@ -263,3 +263,11 @@ def test_two_streams_at_once():
                 got[i] = linear_cross_entropy(*z, reduction="none")
     torch.cuda.synchronize()
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_no_gradient_of_the_gradient():
+    x, w, y = _inputs(10, 90, 16, SF)
+    x.requires_grad_()
+    dx, = torch.autograd.grad(linear_cross_entropy(x, w, y), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()

@@ -1,14 +1,15 @@
 // How evenly a router spreads its tokens over the experts.  Of n valid tokens with k choices each and p_t = softmax(z_t):
 //   c_e = choices of expert e,  f_e = c_e / (n k),  P_e = sum_t p_te / n,  loss = E sum_e f_e P_e
 //   d loss / d z_te = (E / n) p_te (f_e - sum_j p_tj f_j)          (the counts have no gradient)
-// Both passes read the logits once and recompute the softmax: a warp per token, its experts in the lanes' registers, so HBM (or, for
-// few tokens, the launches) is the bound.  The sums over tokens stay in registers, lane by lane, and are added up in a fixed order:
+// Both passes read the logits once and recompute the softmax: a few lanes or a warp per token, its experts in their registers, so HBM (or,
+// for few tokens, the launches) is the bound.  The sums over tokens stay in registers, lane by lane, and are added up in a fixed order:
 // first the warps of a CTA, then the CTAs.  No atomics on floating point: equal inputs give equal bits.
 #include "tkv_elem.cuh"
 
 namespace tkv {
 
-constexpr int kBalThreads = 512, kBalWarps = kBalThreads / 32, kBalCtas = 148;
+constexpr int kBalThreads = 1024, kBalWarps = kBalThreads / 32, kBalCtas = 148;
+#define bal_threads(per) ((per) <= 8 ? kBalThreads : kBalThreads / 2)   // many experts a lane: their registers
 
 struct Balance {
   const void* z; int64_t stride;                           // [tokens, experts]
@@ -25,57 +26,80 @@ struct Balance {
   void* dz; int64_t dz_stride;
 };
 
-// Softmax of a token's logits, expert lane + 32 i in p[i] (0 beyond the last).
-template <typename T, int kPer> __device__ __forceinline__ void balance_softmax(const T* z, int experts, int lane, float* p) {
-  float top = -INFINITY, sum = 0.f;
+// A token belongs to kLanes lanes, 32 / kLanes tokens to a warp.  kVec: lane l holds experts 4 (l + kLanes i) .. + 3 (four at a time from
+// memory; experts and strides are multiples of four), else l + kLanes i; kPer values a lane.
+template <typename T, int kLanes, int kPer, bool kVec> struct BalRow {
+  alignas(16) T raw[kPer];
+  __device__ __forceinline__ static int expert(int l, int i) { return kVec ? 4 * (l + kLanes * (i / 4)) + (i & 3) : l + kLanes * i; }
+  __device__ __forceinline__ void load(const T* z, int experts, int l) {
+    if constexpr (kVec) {
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    p[i] = lane + 32 * i < experts ? to_f32<T>(z[lane + 32 * i]) : -INFINITY;
-    top = fmaxf(top, p[i]);
+      for (int i = 0; i < kPer; i += 4) {
+        if (expert(l, i) >= experts) continue;
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(raw + i) = ld16_stream(z + expert(l, i));
+        else *reinterpret_cast<uint2*>(raw + i) = *reinterpret_cast<const uint2*>(z + expert(l, i));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (expert(l, i) < experts) raw[i] = z[expert(l, i)];
+    }
   }
+  __device__ __forceinline__ void softmax(int experts, int l, float* p) const {
+    float top = -INFINITY, sum = 0.f;
 #pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int i = 0; i < kPer; ++i) {
+      p[i] = expert(l, i) < experts ? to_f32<T>(raw[i]) : -INFINITY;
+      top = fmaxf(top, p[i]);
+    }
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    p[i] = lane + 32 * i < experts ? expf(p[i] - top) : 0.f;
-    sum += p[i];
+    for (int o = kLanes / 2; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      p[i] = expert(l, i) < experts ? expf(p[i] - top) : 0.f;
+      sum += p[i];
+    }
+#pragma unroll
+    for (int o = kLanes / 2; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const float inv = 1.0f / sum;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) p[i] *= inv;
   }
-  const float inv = 1.0f / warp_add(sum);
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) p[i] *= inv;
-}
+};
 
 // Adds up the CTAs' shares; one CTA.
-__device__ __forceinline__ void balance_finish(const Balance& p, int ctas, double* red /* [kBalWarps + 1] */) {
-  const int E = p.experts;
+__device__ __forceinline__ void balance_finish(const Balance& p, int ctas, double* red /* [kBalWarps] */) {
+  const int E = p.experts, warps = blockDim.x >> 5;
   int mine = 0;
-  for (int c = threadIdx.x; c < ctas; c += kBalThreads) mine += p.hits[(int64_t)c * (E + 1) + E];
+  for (int c = threadIdx.x; c < ctas; c += blockDim.x) mine += p.hits[(int64_t)c * (E + 1) + E];
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
   int* whole = reinterpret_cast<int*>(red);
   if ((threadIdx.x & 31) == 0) whole[threadIdx.x >> 5] = mine;
   __syncthreads();
   int64_t n = 0;
-  for (int w = 0; w < kBalWarps; ++w) n += whole[w];
+  for (int w = 0; w < warps; ++w) n += whole[w];
   __syncthreads();
   const double inv = n > 0 ? 1.0 / (double)n : 0.0;
   double part = 0.0;
   const int lane = threadIdx.x & 31;
-  for (int e0 = (threadIdx.x >> 5) * 8; e0 < E; e0 += kBalWarps * 8) {      // a warp takes 8 experts, 4 CTAs' shares at a time
-    const int e = e0 + (lane & 7);
+  for (int e0 = (threadIdx.x >> 5) * 4; e0 < E; e0 += warps * 4) {      // a warp takes 4 experts, 8 CTAs' shares at a time
+    const int e = e0 + (lane & 3);
     double s = 0.0;
     int64_t c = 0;
-    if (e < E)
-      for (int b = lane >> 3; b < ctas; b += 4) {
+    if (e < E) {
+#pragma unroll 5
+      for (int b = lane >> 2; b < ctas; b += 8) {
         s += (double)p.sums[(int64_t)b * E + e];
         c += p.hits[(int64_t)b * (E + 1) + e];
       }
+    }
 #pragma unroll
-    for (int o = 8; o <= 16; o <<= 1) {
+    for (int o = 4; o <= 16; o <<= 1) {
       s += __shfl_xor_sync(0xffffffffu, s, o);
       c += __shfl_xor_sync(0xffffffffu, c, o);
     }
-    if (e < E && lane < 8) {
+    if (e < E && lane < 4) {
       const double f = (double)c * inv / (double)(p.top > 0 ? p.top : 1);
       p.counts[e] = (int32_t)c;
       p.load[e] = (float)f;
@@ -88,48 +112,71 @@ __device__ __forceinline__ void balance_finish(const Balance& p, int ctas, doubl
   __syncthreads();
   if (threadIdx.x == 0) {
     double sum = 0.0;
-    for (int w = 0; w < kBalWarps; ++w) sum += red[w];
+    for (int w = 0; w < warps; ++w) sum += red[w];
     *p.loss = (float)(sum * (double)E);
     p.load[E] = (float)((double)E * inv);
   }
 }
 
-template <typename T, int kPer> __global__ void __launch_bounds__(kBalThreads) balance_sum_kernel(const __grid_constant__ Balance p) {
+template <typename T, int kLanes, int kPer, bool kVec> __global__ void __launch_bounds__(bal_threads(kPer), 1) balance_sum_kernel(const __grid_constant__ Balance p) {
   extern __shared__ float sm[];                            // [experts] sums, [experts + 1] hits
-  __shared__ double red[kBalWarps + 1];
+  __shared__ double red[kBalWarps];
+  constexpr int kRows = 32 / kLanes, kBatch = kPer <= 4 ? 4 : kPer <= 8 ? 2 : 1;   // tokens of a warp whose logits are requested together
+  using Row = BalRow<T, kLanes, kPer, kVec>;
   float* sums = sm;
   int32_t* hits = reinterpret_cast<int32_t*>(sm + p.experts);
-  const int E = p.experts, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int E = p.experts, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % kLanes, mine = lane / kLanes;
   grid_dependency_wait();
-  for (int e = threadIdx.x; e <= E; e += kBalThreads) { hits[e] = 0; if (e < E) sums[e] = 0.f; }
+  for (int e = threadIdx.x; e <= E; e += blockDim.x) { hits[e] = 0; if (e < E) sums[e] = 0.f; }
   __syncthreads();
   float acc[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
   int seen = 0;
-  for (int64_t t = (int64_t)blockIdx.x * kBalWarps + warp; t < p.tokens; t += (int64_t)gridDim.x * kBalWarps) {
-    if (p.valid != nullptr && p.valid[t * p.valid_stride] == 0) continue;
-    ++seen;
-    for (int c = lane; c < p.top; c += 32) {
-      const int64_t at = t * p.choice_stride + c;
-      const int64_t e = p.choice64 ? reinterpret_cast<const int64_t*>(p.choice)[at] : (int64_t) reinterpret_cast<const int32_t*>(p.choice)[at];
-      if (e >= 0 && e < E) atomicAdd(&hits[e], 1);
-    }
-    float s[kPer];
-    balance_softmax<T, kPer>(reinterpret_cast<const T*>(p.z) + t * p.stride, E, lane, s);
+  const int64_t step = (int64_t)gridDim.x * (bal_threads(kPer) / 32) * kRows;
+  for (int64_t t0 = ((int64_t)blockIdx.x * (bal_threads(kPer) / 32) + warp) * kRows + mine; t0 - mine < p.tokens; t0 += kBatch * step) {
+    Row row[kBatch];
+    bool live[kBatch];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) acc[i] += s[i];
+    for (int i = 0; i < kBatch; ++i) {
+      const int64_t t = t0 + i * step;
+      live[i] = t < p.tokens && (p.valid == nullptr || p.valid[t * p.valid_stride] != 0);
+      if (live[i]) row[i].load(reinterpret_cast<const T*>(p.z) + t * p.stride, E, l);
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (!live[i]) continue;
+      seen += l == 0;
+      for (int c = l; c < p.top; c += kLanes) {
+        const int64_t at = (t0 + i * step) * p.choice_stride + c;
+        const int64_t e = p.choice64 ? reinterpret_cast<const int64_t*>(p.choice)[at] : (int64_t)reinterpret_cast<const int32_t*>(p.choice)[at];
+        if (e >= 0 && e < E) atomicAdd(&hits[e], 1);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      float s[kPer];
+      row[i].softmax(E, l, s);                             // shuffles: every lane takes part
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) acc[k] += live[i] ? s[k] : 0.f;
+    }
   }
-  for (int w = 0; w < kBalWarps; ++w) {                    // the warps' sums, one warp after the other
-    if (warp == w) {
+#pragma unroll
+  for (int o = kLanes; o < 32; o <<= 1) {                  // the tokens of a warp
+    seen += __shfl_xor_sync(0xffffffffu, seen, o);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
+  }
+  for (int w = 0; w < bal_threads(kPer) / 32; ++w) {                    // the warps' sums, one warp after the other
+    if (warp == w && mine == 0) {
 #pragma unroll
       for (int i = 0; i < kPer; ++i)
-        if (lane + 32 * i < E) sums[lane + 32 * i] += acc[i];
-      if (lane == 0) hits[E] += seen;
+        if (Row::expert(l, i) < E) sums[Row::expert(l, i)] += acc[i];
+      if (l == 0) hits[E] += seen;
     }
     __syncthreads();
   }
-  for (int e = threadIdx.x; e <= E; e += kBalThreads) {
+  for (int e = threadIdx.x; e <= E; e += blockDim.x) {
     p.hits[(int64_t)blockIdx.x * (E + 1) + e] = hits[e];
     if (e < E) p.sums[(int64_t)blockIdx.x * E + e] = sums[e];
   }
@@ -141,63 +188,96 @@ template <typename T, int kPer> __global__ void __launch_bounds__(kBalThreads) b
 }
 
 __global__ void __launch_bounds__(kBalThreads) balance_finish_kernel(const __grid_constant__ Balance p, int ctas) {
-  __shared__ double red[kBalWarps + 1];
+  __shared__ double red[kBalWarps];
   grid_dependency_wait();
   grid_launch_dependents();
   balance_finish(p, ctas, red);
 }
 
-template <typename T, int kPer> __global__ void __launch_bounds__(kBalThreads) balance_grad_kernel(const __grid_constant__ Balance p) {
-  const int E = p.experts, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+template <typename T, int kLanes, int kPer, bool kVec> __global__ void __launch_bounds__(bal_threads(kPer), 1) balance_grad_kernel(const __grid_constant__ Balance p) {
+  constexpr int kRows = 32 / kLanes, kBatch = kPer <= 4 ? 2 : 1;
+  using Row = BalRow<T, kLanes, kPer, kVec>;
+  const int E = p.experts, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % kLanes, mine = lane / kLanes;
   grid_dependency_wait();
   grid_launch_dependents();
   const float g = p.grad[0] * p.load[E];
   float f[kPer];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) f[i] = lane + 32 * i < E ? p.load[lane + 32 * i] : 0.f;
-  for (int64_t t = (int64_t)blockIdx.x * kBalWarps + warp; t < p.tokens; t += (int64_t)gridDim.x * kBalWarps) {
-    T* out = reinterpret_cast<T*>(p.dz) + t * p.dz_stride;
-    if (p.valid != nullptr && p.valid[t * p.valid_stride] == 0) {
-      for (int e = lane; e < E; e += 32) out[e] = from_f32<T>(0.f);
-      continue;
+  for (int i = 0; i < kPer; ++i) f[i] = Row::expert(l, i) < E ? p.load[Row::expert(l, i)] : 0.f;
+  const int64_t step = (int64_t)gridDim.x * (bal_threads(kPer) / 32) * kRows;
+  for (int64_t t0 = ((int64_t)blockIdx.x * (bal_threads(kPer) / 32) + warp) * kRows + mine; t0 - mine < p.tokens; t0 += kBatch * step) {
+    Row row[kBatch];
+    bool live[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int64_t t = t0 + i * step;
+      live[i] = t < p.tokens && (p.valid == nullptr || p.valid[t * p.valid_stride] != 0);
+      if (live[i]) row[i].load(reinterpret_cast<const T*>(p.z) + t * p.stride, E, l);
     }
-    float s[kPer], dot = 0.f;
-    balance_softmax<T, kPer>(reinterpret_cast<const T*>(p.z) + t * p.stride, E, lane, s);
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) dot = fmaf(s[i], f[i], dot);
-    dot = warp_add(dot);
+    for (int i = 0; i < kBatch; ++i) {
+      float s[kPer], dot = 0.f;
+      row[i].softmax(E, l, s);
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (lane + 32 * i < E) out[lane + 32 * i] = from_f32<T>(g * s[i] * (f[i] - dot));
+      for (int k = 0; k < kPer; ++k) dot = fmaf(s[k], f[k], dot);
+#pragma unroll
+      for (int o = kLanes / 2; o >= 1; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+      const int64_t t = t0 + i * step;
+      if (t >= p.tokens) continue;
+      T* out = reinterpret_cast<T*>(p.dz) + t * p.dz_stride;
+      alignas(16) T d[kPer];
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) d[k] = from_f32<T>(live[i] ? g * s[k] * (f[k] - dot) : 0.f);
+      if constexpr (kVec) {
+#pragma unroll
+        for (int k = 0; k < kPer; k += 4) {
+          if (Row::expert(l, k) >= E) continue;
+          if constexpr (sizeof(T) == 4) st16(out + Row::expert(l, k), *reinterpret_cast<const uint4*>(d + k));
+          else *reinterpret_cast<uint2*>(out + Row::expert(l, k)) = *reinterpret_cast<const uint2*>(d + k);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < kPer; ++k)
+          if (Row::expert(l, k) < E) out[Row::expert(l, k)] = d[k];
+      }
+    }
   }
 }
 
-// Tokens of a CTA where there are fewer than one per warp of every SM; beyond, a CTA per SM (the sums of a CTA are read again).
+// One CTA where its warps take a token or a few each, so that nothing has to be joined by a second launch; else up to a CTA per SM.
 static int balance_ctas(int64_t tokens) {
-  const int64_t need = (tokens + 2 * kBalWarps - 1) / (2 * kBalWarps);
-  return need < 1 ? 1 : need < kBalCtas ? (int)need : kBalCtas;
+  if (tokens <= 4 * kBalWarps) return 1;
+  const int64_t need = (tokens + 4 * kBalWarps - 1) / (4 * kBalWarps);
+  return need < kBalCtas ? (int)need : kBalCtas;
 }
 
-template <typename T, int kPer> static int balance_forward(const Balance& p, cudaStream_t st) {
-  const int ctas = balance_ctas(p.tokens);
-  cudaError_t e = launch_pdl(balance_sum_kernel<T, kPer>, dim3(ctas), dim3(kBalThreads), (size_t)(2 * p.experts + 1) * 4, st, p);
-  if (e == cudaSuccess && ctas > 1) e = launch_pdl(balance_finish_kernel, dim3(1), dim3(kBalThreads), 0, st, p, ctas);
-  if (e != cudaSuccess) return fail(TKV_ERR_LAUNCH, "tkv_moe_balance: %s", cudaGetErrorString(e));
-  return check_launch("tkv_moe_balance");
-}
-template <typename T, int kPer> static int balance_backward(const Balance& p, cudaStream_t st) {
-  const int64_t need = (p.tokens + kBalWarps - 1) / kBalWarps;
-  cudaError_t e = launch_pdl(balance_grad_kernel<T, kPer>, dim3((unsigned)(need < 4 * kBalCtas ? need : 4 * kBalCtas)), dim3(kBalThreads), 0, st, p);
-  if (e != cudaSuccess) return fail(TKV_ERR_LAUNCH, "tkv_moe_balance_grad: %s", cudaGetErrorString(e));
-  return check_launch("tkv_moe_balance_grad");
+template <typename T, int kLanes, int kPer, bool kVec> static int balance_launch(const Balance& p, bool grad, cudaStream_t st) {
+  cudaError_t e;
+  if (grad) {
+    const int64_t need = (p.tokens * kLanes + bal_threads(kPer) - 1) / bal_threads(kPer);
+    e = launch_pdl(balance_grad_kernel<T, kLanes, kPer, kVec>, dim3((unsigned)(need < 2 * kBalCtas ? need : 2 * kBalCtas)), dim3(bal_threads(kPer)), 0, st, p);
+  } else {
+    const int ctas = balance_ctas(p.tokens);
+    e = launch_pdl(balance_sum_kernel<T, kLanes, kPer, kVec>, dim3(ctas), dim3(bal_threads(kPer)), (size_t)(2 * p.experts + 1) * 4, st, p);
+    if (e == cudaSuccess && ctas > 1) e = launch_pdl(balance_finish_kernel, dim3(1), dim3(kBalThreads), 0, st, p, ctas);
+  }
+  const char* what = grad ? "tkv_moe_balance_grad" : "tkv_moe_balance";
+  return e == cudaSuccess ? check_launch(what) : fail(TKV_ERR_LAUNCH, "%s: %s", what, cudaGetErrorString(e));
 }
 template <typename T> static int balance_run(const Balance& p, bool grad, cudaStream_t st) {
-  const int per = (p.experts + 31) / 32;
-  if (per <= 1) return grad ? balance_backward<T, 1>(p, st) : balance_forward<T, 1>(p, st);
-  if (per <= 2) return grad ? balance_backward<T, 2>(p, st) : balance_forward<T, 2>(p, st);
-  if (per <= 4) return grad ? balance_backward<T, 4>(p, st) : balance_forward<T, 4>(p, st);
-  if (per <= 8) return grad ? balance_backward<T, 8>(p, st) : balance_forward<T, 8>(p, st);
-  return grad ? balance_backward<T, 32>(p, st) : balance_forward<T, 32>(p, st);
+  const uintptr_t bytes = 4 * sizeof(T);
+  const bool vec = p.experts % 4 == 0 && p.stride % 4 == 0 && (uintptr_t)p.z % bytes == 0 && (!grad || (p.dz_stride % 4 == 0 && (uintptr_t)p.dz % bytes == 0));
+  const int E = p.experts;
+  if (vec) {
+    if (E <= 32) return balance_launch<T, 8, 4, true>(p, grad, st);
+    if (E <= 64) return balance_launch<T, 16, 4, true>(p, grad, st);
+    if (E <= 128) return balance_launch<T, 32, 4, true>(p, grad, st);
+    if (E <= 256) return balance_launch<T, 32, 8, true>(p, grad, st);
+    return balance_launch<T, 32, 32, true>(p, grad, st);
+  }
+  if (E <= 32) return balance_launch<T, 32, 1, false>(p, grad, st);
+  if (E <= 128) return balance_launch<T, 32, 4, false>(p, grad, st);
+  return balance_launch<T, 32, 32, false>(p, grad, st);
 }
 static int balance_any(const Balance& p, int dtype, bool grad, cudaStream_t st) {
   if (dtype == TKV_BF16) return balance_run<__nv_bfloat16>(p, grad, st);

@@ -8,6 +8,16 @@ import torch
 from . import ops
 
 
+def _once(backward):
+    """A backward pass without a gradient of its own: asking for one raises.  (torch's guard alone costs several microseconds a pass, so it
+    is put in front only where a graph of the backward pass is being made.)"""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
+    return staticmethod(run)
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, labels, ignore, reduction, status):
@@ -16,12 +26,11 @@ class _LinearCrossEntropy(torch.autograd.Function):
         ctx.how = reduction, status
         return reduced if reduction else loss
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, grad):
         x, w, plan = ctx.saved_tensors
         reduction, status = ctx.how
-        dx, dw = ops.vloss_backward(x, w, plan, grad.float(), reduction, ctx.needs_input_grad[0], ctx.needs_input_grad[1], status)
+        dx, dw = ops.vloss_backward(x, w, plan, ops.as_float(grad), reduction, ctx.needs_input_grad[0], ctx.needs_input_grad[1], status)
         return dx, dw, None, None, None, None
 
 
@@ -64,11 +73,10 @@ class _ExpertBalance(torch.autograd.Function):
         ctx.mark_non_differentiable(counts)
         return loss, counts
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, grad, _):
         logits, load, *valid = ctx.saved_tensors
-        return ops.moe_balance_grad(logits, valid[0] if valid else None, load, grad.float()), None, None
+        return ops.moe_balance_grad(logits, valid[0] if valid else None, load, ops.as_float(grad)), None, None
 
 
 def expert_balance(logits: torch.Tensor, choice: torch.Tensor, valid: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:

@@ -822,32 +822,40 @@ def on_device_of(t: torch.Tensor):
     return _here if t.get_device() == torch.cuda.current_device() else torch.cuda.device_of(t)
 
 
+def as_float(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dtype == torch.float32 else t.float()
+
+
+_ABSENT = (None, 0, 0, 0, None, 0)
+
+
+def _rotary_side(t, b: int, s: int, d: int):
+    sb, sh, ss, sd = t.stride()
+    if sd != 1:
+        t = t.contiguous()
+        sb, sh, ss, _ = t.stride()
+    h = t.shape[1]
+    y = t.new_empty_strided((b, h, s, d), (s * h * d, d, h * d, 1))
+    return y, (t.data_ptr(), sb, sh, ss, y.data_ptr(), h), t
+
+
 def rotary(q, k, positions, freq, layout: int, inverse: bool, scale: float):
     """``(q', k')`` of q and k ``[B, H, S, D]`` (one of them may be None), stored token by token; see ``positions.apply_rotary``, which
     checks the arguments."""
     x = q if q is not None else k
     b, _, s, d = x.shape
-    if q is not None and q.stride(3) != 1:
-        q = q.contiguous()
-    if k is not None and k.stride(3) != 1:
-        k = k.contiguous()
+    steps = positions.stride()
+    if len(steps) == 1 or positions.shape[0] == 1:
+        steps = (0, steps[-1])
     with on_device_of(x):
-        out, args = [], []
-        for t in (q, k):
-            if t is None:
-                out.append(None)
-                args += [None, 0, 0, 0, None, 0]
-                continue
-            h = t.shape[1]
-            y = torch.empty(b, s, h, d, dtype=t.dtype, device=t.device)
-            out.append(y.transpose(1, 2))
-            sb, sh, ss, _ = t.stride()
-            args += [t.data_ptr(), sb, sh, ss, y.data_ptr(), h]
-        check(lib().tkv_rotary(*args, positions.data_ptr(), _POS_BITS[positions.dtype], positions.stride(0), positions.stride(1),
-                               freq.data_ptr(), b, s, d, freq.shape[0], layout, int(inverse), float(scale), dtype_code(x.dtype), _stream(x)),
-              "tkv_rotary")
+        q2, q_args, _q = (None, _ABSENT, None) if q is None else _rotary_side(q, b, s, d)
+        k2, k_args, _k = (None, _ABSENT, None) if k is None else _rotary_side(k, b, s, d)
+        rc = lib().tkv_rotary(*q_args, *k_args, positions.data_ptr(), _POS_BITS[positions.dtype], *steps, freq.data_ptr(), b, s, d,
+                              freq.shape[0], layout, inverse, scale, _DTYPE[x.dtype], _raw_stream(x.get_device()))
+    if rc:
+        check(rc, "tkv_rotary")
     _count(1)
-    return out
+    return q2, k2
 
 
 VLOSS_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
@@ -886,25 +894,28 @@ def vloss_backward(x, w, plan, grad, reduction: int, want_dx: bool, want_dw: boo
 def moe_balance(logits, choice, valid):
     """``(loss, counts [E] int32, load)`` of router logits ``[T, E]``; ``load`` is what :func:`moe_balance_grad` takes."""
     T, E = logits.shape
+    L = lib()
     with on_device_of(logits):
-        dev = logits.device
-        loss, load = torch.empty((), dtype=torch.float32, device=dev), torch.empty(E + 1, dtype=torch.float32, device=dev)
-        counts = torch.empty(E, dtype=torch.int32, device=dev)
-        need = lib().tkv_moe_balance_workspace_bytes(T, E)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        check(lib().tkv_moe_balance(logits.data_ptr(), logits.stride(0), choice.data_ptr(), choice.stride(0), _POS_BITS[choice.dtype], _ptr(valid),
-                                    0 if valid is None else valid.stride(0), T, E, choice.shape[1], loss.data_ptr(), counts.data_ptr(),
-                                    load.data_ptr(), ws.data_ptr(), need, dtype_code(logits.dtype), _stream(logits)), "tkv_moe_balance")
-    _count(2 if T > 32 else 1)
+        need = L.tkv_moe_balance_workspace_bytes(T, E)
+        loss, counts = logits.new_empty((), dtype=torch.float32), logits.new_empty(E, dtype=torch.int32)
+        load = logits.new_empty(E + 1 + need // 4, dtype=torch.float32)       # and the workspace behind it
+        at = load.data_ptr()
+        rc = L.tkv_moe_balance(logits.data_ptr(), logits.stride(0), choice.data_ptr(), choice.stride(0), _POS_BITS[choice.dtype], _ptr(valid),
+                               0 if valid is None else valid.stride(0), T, E, choice.shape[1], loss.data_ptr(), counts.data_ptr(), at,
+                               at + 4 * (E + 1), need, _DTYPE[logits.dtype], _raw_stream(logits.get_device()))
+    if rc:
+        check(rc, "tkv_moe_balance")
+    _count(2 if T > 128 else 1)
     return loss, counts, load
 
 
 def moe_balance_grad(logits, valid, load, grad):
     T, E = logits.shape
     with on_device_of(logits):
-        out = torch.empty(T, E, dtype=logits.dtype, device=logits.device)
-        check(lib().tkv_moe_balance_grad(logits.data_ptr(), logits.stride(0), _ptr(valid), 0 if valid is None else valid.stride(0), load.data_ptr(),
-                                         grad.data_ptr(), T, E, out.data_ptr(), E, dtype_code(logits.dtype), _stream(logits)),
-              "tkv_moe_balance_grad")
+        out = logits.new_empty((T, E))
+        rc = lib().tkv_moe_balance_grad(logits.data_ptr(), logits.stride(0), _ptr(valid), 0 if valid is None else valid.stride(0), load.data_ptr(),
+                                        grad.data_ptr(), T, E, out.data_ptr(), E, _DTYPE[logits.dtype], _raw_stream(logits.get_device()))
+    if rc:
+        check(rc, "tkv_moe_balance_grad")
     _count(1)
     return out

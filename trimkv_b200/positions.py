@@ -16,25 +16,24 @@ LAYOUTS = {"half": 0, "pairs": 1}
 
 
 class _Rotary(torch.autograd.Function):
-    """The gradient of a turn is the turn back, with the same scale."""
+    """The gradient of a turn is the turn back, with the same scale; its gradient in turn is the turn itself."""
 
     @staticmethod
-    def forward(ctx, q, k, positions, freq, layout, scale):
+    def forward(ctx, q, k, positions, freq, layout, inverse, scale):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(positions, freq)
-        ctx.how = layout, scale
-        q2, k2 = ops.rotary(q, k, positions, freq, layout, False, scale)
-        return q2 if k2 is None else (q2, k2)
+        ctx.how = layout, inverse, scale
+        return ops.rotary(q, k, positions, freq, layout, inverse, scale)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dq, dk=None):
+    def backward(ctx, dq, dk):
         if dq is None and dk is None:
-            return (None,) * 6
+            return (None,) * 7
         positions, freq = ctx.saved_tensors
-        layout, scale = ctx.how
-        dq, dk = ops.rotary(dq, dk, positions, freq, layout, True, scale)
-        return dq, dk, None, None, None, None
+        layout, inverse, scale = ctx.how
+        turn = _Rotary.apply if torch.is_grad_enabled() else ops.rotary
+        dq, dk = turn(dq, dk, positions, freq, layout, not inverse, scale)
+        return dq, dk, None, None, None, None, None
 
 
 def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, freq: torch.Tensor, *, layout: str = "half",
@@ -46,29 +45,30 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     copied.  ``layout``: ``"half"`` turns element i with ``pairs + i``, ``"pairs"`` element 2i with 2i + 1.  Angles are exact to fp32 at
     any position, and a result is rounded once.  Any strides; the results are stored token by token (``[B, S, H, D]`` in memory).
     Differentiable in q and k."""
-    if layout not in LAYOUTS:
+    how = LAYOUTS.get(layout)
+    if how is None:
         raise ValueError(f"layout {layout!r}: one of {sorted(LAYOUTS)}")
-    if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[0] != q.shape[0] or k.shape[2:] != q.shape[2:])):
-        raise ValueError(f"queries {tuple(q.shape)} and keys {None if k is None else tuple(k.shape)}: want [B, H, S, D] of one batch, length and head size")
-    ops.dtype_code(q.dtype)
-    if k is not None and (k.dtype != q.dtype or k.device != q.device):
-        raise TypeError(f"queries {q.dtype} on {q.device}, keys {k.dtype} on {k.device}")
-    b, _, s, d = q.shape
-    if positions.dtype not in (torch.int32, torch.int64):
+    shape = q.shape
+    if len(shape) != 4 or (k is not None and (k.dim() != 4 or k.shape[0] != shape[0] or k.shape[2:] != shape[2:])):
+        raise ValueError(f"queries {tuple(shape)} and keys {None if k is None else tuple(k.shape)}: want [B, H, S, D] of one batch, length and head size")
+    b, _, s, d = shape
+    dtype, device = q.dtype, q.device
+    ops.dtype_code(dtype)
+    if k is not None and (k.dtype != dtype or k.device != device):
+        raise TypeError(f"queries {dtype} on {device}, keys {k.dtype} on {k.device}")
+    if positions.dtype != torch.int64 and positions.dtype != torch.int32:
         raise TypeError(f"positions of {positions.dtype}: want int32 or int64")
-    if positions.dim() == 1:
-        positions = positions[None]
-    if positions.dim() != 2 or positions.shape[1] != s or positions.shape[0] not in (1, b):
-        raise ValueError(f"positions {tuple(positions.shape)} for {b} x {s} tokens")
-    if freq.dim() != 2 or freq.shape[1] != 2 or freq.dtype != torch.float32 or not freq.is_contiguous() or 2 * freq.shape[0] > d:
-        raise ValueError(f"frequencies {freq.dtype} {tuple(freq.shape)}: want contiguous fp32 [pairs, 2] with at most {d // 2} pairs")
-    if positions.device != q.device or freq.device != q.device:
-        raise ValueError(f"queries on {q.device}, positions on {positions.device}, frequencies on {freq.device}")
-    positions = positions.expand(b, s)
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        out = _Rotary.apply(q, k, positions, freq, LAYOUTS[layout], float(scale))
-        return (out, None) if k is None else out
-    return tuple(ops.rotary(q, k, positions, freq, LAYOUTS[layout], False, scale))
+    at = positions.shape
+    if len(at) not in (1, 2) or at[-1] != s or (len(at) == 2 and at[0] != 1 and at[0] != b):
+        raise ValueError(f"positions {tuple(at)} for {b} x {s} tokens")
+    pairs = freq.shape
+    if len(pairs) != 2 or pairs[1] != 2 or freq.dtype != torch.float32 or not freq.is_contiguous() or 2 * pairs[0] > d:
+        raise ValueError(f"frequencies {freq.dtype} {tuple(pairs)}: want contiguous fp32 [pairs, 2] with at most {d // 2} pairs")
+    if positions.device != device or freq.device != device:
+        raise ValueError(f"queries on {device}, positions on {positions.device}, frequencies on {freq.device}")
+    if (q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled():
+        return _Rotary.apply(q, k, positions, freq, how, False, float(scale))
+    return ops.rotary(q, k, positions, freq, how, False, float(scale))
 
 
 __all__ = ["LAYOUTS", "apply_rotary"]
