@@ -8,8 +8,8 @@
 
 namespace tkv {
 
-constexpr int kBalThreads = 1024, kBalWarps = kBalThreads / 32, kBalCtas = 148;
-#define bal_threads(per) ((per) <= 8 ? kBalThreads : kBalThreads / 2)   // many experts a lane: their registers
+constexpr int kBalThreads = 1024, kBalWarps = kBalThreads / 32, kBalCtas = 148, kBalExperts = 1024;
+#define bal_threads(per) ((per) <= 4 ? kBalThreads : kBalThreads / 2)   // many experts a lane: their registers
 
 struct Balance {
   const void* z; int64_t stride;                           // [tokens, experts]
@@ -56,7 +56,7 @@ template <typename T, int kLanes, int kPer, bool kVec> struct BalRow {
     for (int o = kLanes / 2; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      p[i] = expert(l, i) < experts ? expf(p[i] - top) : 0.f;
+      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p[i]) : "f"((p[i] - top) * 1.4426950408889634f));   // 0 beyond the last
       sum += p[i];
     }
 #pragma unroll
@@ -67,92 +67,100 @@ template <typename T, int kLanes, int kPer, bool kVec> struct BalRow {
   }
 };
 
-// Adds up the CTAs' shares; one CTA.
-__device__ __forceinline__ void balance_finish(const Balance& p, int ctas, double* red /* [kBalWarps] */) {
-  const int E = p.experts, warps = blockDim.x >> 5;
-  int mine = 0;
-  for (int c = threadIdx.x; c < ctas; c += blockDim.x) mine += p.hits[(int64_t)c * (E + 1) + E];
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  int* whole = reinterpret_cast<int*>(red);
-  if ((threadIdx.x & 31) == 0) whole[threadIdx.x >> 5] = mine;
-  __syncthreads();
-  int64_t n = 0;
-  for (int w = 0; w < warps; ++w) n += whole[w];
-  __syncthreads();
-  const double inv = n > 0 ? 1.0 / (double)n : 0.0;
+// Adds up the CTAs' shares; one CTA of kThreads.  A column of the shares (an expert, and the valid tokens) to every thread, several threads
+// to a column where there are fewer columns, 16 CTAs' shares requested at a time.
+struct BalFinish { double part[kBalWarps]; float sums[kBalThreads]; int32_t hits[kBalThreads]; int32_t n; };
+
+template <int kThreads> __device__ __forceinline__ void balance_finish(const Balance& p, int ctas, BalFinish* sm) {
+  const int E = p.experts, wide = min((E + 1 + 31) / 32 * 32, kThreads), slices = kThreads / wide;
+  const int slice = threadIdx.x / wide, at = threadIdx.x - slice * wide;
   double part = 0.0;
-  const int lane = threadIdx.x & 31;
-  for (int e0 = (threadIdx.x >> 5) * 4; e0 < E; e0 += warps * 4) {      // a warp takes 4 experts, 8 CTAs' shares at a time
-    const int e = e0 + (lane & 3);
-    double s = 0.0;
-    int64_t c = 0;
-    if (e < E) {
-#pragma unroll 5
-      for (int b = lane >> 2; b < ctas; b += 8) {
-        s += (double)p.sums[(int64_t)b * E + e];
-        c += p.hits[(int64_t)b * (E + 1) + e];
-      }
-    }
+  for (int e0 = E / wide * wide; e0 >= 0; e0 -= wide) {    // the last columns first: the valid tokens are among them
+    const int e = e0 + at;
+    float s = 0.f;
+    int c = 0;
+    if (slice < slices && e <= E)
+      for (int b0 = slice; b0 < ctas; b0 += 16 * slices) {
+        float v[16];
+        int h[16];
 #pragma unroll
-    for (int o = 4; o <= 16; o <<= 1) {
-      s += __shfl_xor_sync(0xffffffffu, s, o);
-      c += __shfl_xor_sync(0xffffffffu, c, o);
+        for (int i = 0; i < 16; ++i) {
+          const int b = b0 + i * slices;
+          v[i] = b < ctas && e < E ? p.sums[(int64_t)b * E + e] : 0.f;
+          h[i] = b < ctas ? p.hits[(int64_t)b * (E + 1) + e] : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { s += v[i]; c += h[i]; }
+      }
+    sm->sums[threadIdx.x] = s;
+    sm->hits[threadIdx.x] = c;
+    __syncthreads();
+    if (slice == 0 && e <= E) {
+      for (int k = 1; k < slices; ++k) { s += sm->sums[k * wide + at]; c += sm->hits[k * wide + at]; }
+      if (e == E) sm->n = c;
     }
-    if (e < E && lane < 4) {
-      const double f = (double)c * inv / (double)(p.top > 0 ? p.top : 1);
-      p.counts[e] = (int32_t)c;
-      p.load[e] = (float)f;
-      part += f * s * inv;
+    __syncthreads();
+    if (slice == 0 && e < E) {
+      const int n = sm->n;
+      const float f = n > 0 && p.top > 0 ? (float)c / ((float)n * (float)p.top) : 0.f;
+      p.counts[e] = c;
+      p.load[e] = f;
+      part += (double)f * (double)s;
     }
   }
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-  if (lane == 0) red[threadIdx.x >> 5] = part;
+  if ((threadIdx.x & 31) == 0) sm->part[threadIdx.x >> 5] = part;
   __syncthreads();
   if (threadIdx.x == 0) {
     double sum = 0.0;
-    for (int w = 0; w < warps; ++w) sum += red[w];
-    *p.loss = (float)(sum * (double)E);
-    p.load[E] = (float)((double)E * inv);
+    for (int w = 0; w < kThreads / 32; ++w) sum += sm->part[w];
+    const float scale = sm->n > 0 ? (float)E / (float)sm->n : 0.f;
+    *p.loss = (float)sum * scale;
+    p.load[E] = scale;
   }
 }
 
+constexpr int kBalChunk = 128;                             // experts whose sums of all warps are in shared memory at a time
+
 template <typename T, int kLanes, int kPer, bool kVec> __global__ void __launch_bounds__(bal_threads(kPer), 1) balance_sum_kernel(const __grid_constant__ Balance p) {
-  extern __shared__ float sm[];                            // [experts] sums, [experts + 1] hits
-  __shared__ double red[kBalWarps];
-  constexpr int kRows = 32 / kLanes, kBatch = kPer <= 4 ? 4 : kPer <= 8 ? 2 : 1;   // tokens of a warp whose logits are requested together
+  extern __shared__ float sums[];                          // [warps][min(experts, kBalChunk)]
+  __shared__ BalFinish finish;
+  __shared__ int32_t hits[kBalExperts + 1];
+  constexpr int kRows = 32 / kLanes, kWarps = bal_threads(kPer) / 32, kBatch = kPer <= 4 ? 4 : kPer <= 16 ? 3 : 1;   // tokens of a warp whose logits are requested together
   using Row = BalRow<T, kLanes, kPer, kVec>;
-  float* sums = sm;
-  int32_t* hits = reinterpret_cast<int32_t*>(sm + p.experts);
   const int E = p.experts, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % kLanes, mine = lane / kLanes;
   grid_dependency_wait();
-  for (int e = threadIdx.x; e <= E; e += blockDim.x) { hits[e] = 0; if (e < E) sums[e] = 0.f; }
+  for (int e = threadIdx.x; e <= E; e += blockDim.x) hits[e] = 0;
   __syncthreads();
   float acc[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
   int seen = 0;
-  const int64_t step = (int64_t)gridDim.x * (bal_threads(kPer) / 32) * kRows;
-  for (int64_t t0 = ((int64_t)blockIdx.x * (bal_threads(kPer) / 32) + warp) * kRows + mine; t0 - mine < p.tokens; t0 += kBatch * step) {
-    Row row[kBatch];
-    bool live[kBatch];
+  const int64_t step = (int64_t)gridDim.x * kWarps * kRows;
+  Row row[kBatch];
+  bool live[kBatch];
+  auto request = [&](int64_t t0) {
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       const int64_t t = t0 + i * step;
       live[i] = t < p.tokens && (p.valid == nullptr || p.valid[t * p.valid_stride] != 0);
       if (live[i]) row[i].load(reinterpret_cast<const T*>(p.z) + t * p.stride, E, l);
+      seen += live[i] && l == 0;
     }
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      if (!live[i]) continue;
-      seen += l == 0;
-      for (int c = l; c < p.top; c += kLanes) {
-        const int64_t at = (t0 + i * step) * p.choice_stride + c;
-        const int64_t e = p.choice64 ? reinterpret_cast<const int64_t*>(p.choice)[at] : (int64_t)reinterpret_cast<const int32_t*>(p.choice)[at];
-        if (e >= 0 && e < E) atomicAdd(&hits[e], 1);
-      }
-    }
+  };
+  int64_t t0 = ((int64_t)blockIdx.x * kWarps + warp) * kRows + mine;
+  request(t0);
+  // While the first rows come, the choices, a thread each, wherever their tokens' logits are read (tokens * top is below 2^31).
+  const uint32_t all = (uint32_t)p.tokens * (uint32_t)p.top, threads = gridDim.x * blockDim.x;
+#pragma unroll 4
+  for (uint32_t i = blockIdx.x * blockDim.x + threadIdx.x; i < all; i += threads) {
+    const uint32_t t = i / (uint32_t)p.top;
+    const int64_t at = t * p.choice_stride + (i - t * (uint32_t)p.top);
+    const int64_t e = p.choice64 ? reinterpret_cast<const int64_t*>(p.choice)[at] : (int64_t)reinterpret_cast<const int32_t*>(p.choice)[at];
+    if (e >= 0 && e < E && (p.valid == nullptr || p.valid[t * p.valid_stride] != 0)) atomicAdd(&hits[e], 1);
+  }
+  while (t0 - mine < p.tokens) {
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       float s[kPer];
@@ -160,6 +168,8 @@ template <typename T, int kLanes, int kPer, bool kVec> __global__ void __launch_
 #pragma unroll
       for (int k = 0; k < kPer; ++k) acc[k] += live[i] ? s[k] : 0.f;
     }
+    t0 += kBatch * step;
+    if (t0 - mine < p.tokens) request(t0);
   }
 #pragma unroll
   for (int o = kLanes; o < 32; o <<= 1) {                  // the tokens of a warp
@@ -167,35 +177,42 @@ template <typename T, int kLanes, int kPer, bool kVec> __global__ void __launch_
 #pragma unroll
     for (int i = 0; i < kPer; ++i) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
   }
-  for (int w = 0; w < bal_threads(kPer) / 32; ++w) {                    // the warps' sums, one warp after the other
-    if (warp == w && mine == 0) {
+  if (lane == 0) atomicAdd(&hits[E], seen);
+  const int wide = min(E, kBalChunk);
+  for (int e0 = 0; e0 < E; e0 += wide) {                   // the warps of the CTA, in order
+    if (mine == 0) {
 #pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (Row::expert(l, i) < E) sums[Row::expert(l, i)] += acc[i];
-      if (l == 0) hits[E] += seen;
+      for (int i = 0; i < kPer; ++i) {
+        const int e = Row::expert(l, i) - e0;
+        if (e >= 0 && e < wide) sums[warp * wide + e] = acc[i];
+      }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < wide && e0 + e < E; e += blockDim.x) {
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) s += sums[w * wide + e];
+      p.sums[(int64_t)blockIdx.x * E + e0 + e] = s;
     }
     __syncthreads();
   }
-  for (int e = threadIdx.x; e <= E; e += blockDim.x) {
-    p.hits[(int64_t)blockIdx.x * (E + 1) + e] = hits[e];
-    if (e < E) p.sums[(int64_t)blockIdx.x * E + e] = sums[e];
-  }
+  for (int e = threadIdx.x; e <= E; e += blockDim.x) p.hits[(int64_t)blockIdx.x * (E + 1) + e] = hits[e];
   grid_launch_dependents();
   if (gridDim.x == 1) {
     __syncthreads();
-    balance_finish(p, 1, red);
+    balance_finish<bal_threads(kPer)>(p, 1, &finish);
   }
 }
 
 __global__ void __launch_bounds__(kBalThreads) balance_finish_kernel(const __grid_constant__ Balance p, int ctas) {
-  __shared__ double red[kBalWarps];
+  __shared__ BalFinish finish;
   grid_dependency_wait();
   grid_launch_dependents();
-  balance_finish(p, ctas, red);
+  balance_finish<kBalThreads>(p, ctas, &finish);
 }
 
 template <typename T, int kLanes, int kPer, bool kVec> __global__ void __launch_bounds__(bal_threads(kPer), 1) balance_grad_kernel(const __grid_constant__ Balance p) {
-  constexpr int kRows = 32 / kLanes, kBatch = kPer <= 4 ? 2 : 1;
+  constexpr int kRows = 32 / kLanes, kBatch = kPer <= 16 ? 2 : 1;
   using Row = BalRow<T, kLanes, kPer, kVec>;
   const int E = p.experts, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % kLanes, mine = lane / kLanes;
   grid_dependency_wait();
@@ -258,7 +275,8 @@ template <typename T, int kLanes, int kPer, bool kVec> static int balance_launch
     e = launch_pdl(balance_grad_kernel<T, kLanes, kPer, kVec>, dim3((unsigned)(need < 2 * kBalCtas ? need : 2 * kBalCtas)), dim3(bal_threads(kPer)), 0, st, p);
   } else {
     const int ctas = balance_ctas(p.tokens);
-    e = launch_pdl(balance_sum_kernel<T, kLanes, kPer, kVec>, dim3(ctas), dim3(bal_threads(kPer)), (size_t)(2 * p.experts + 1) * 4, st, p);
+    e = launch_pdl(balance_sum_kernel<T, kLanes, kPer, kVec>, dim3(ctas), dim3(bal_threads(kPer)),
+                   (size_t)bal_threads(kPer) / 32 * (p.experts < kBalChunk ? p.experts : kBalChunk) * 4, st, p);
     if (e == cudaSuccess && ctas > 1) e = launch_pdl(balance_finish_kernel, dim3(1), dim3(kBalThreads), 0, st, p, ctas);
   }
   const char* what = grad ? "tkv_moe_balance_grad" : "tkv_moe_balance";
@@ -268,11 +286,16 @@ template <typename T> static int balance_run(const Balance& p, bool grad, cudaSt
   const uintptr_t bytes = 4 * sizeof(T);
   const bool vec = p.experts % 4 == 0 && p.stride % 4 == 0 && (uintptr_t)p.z % bytes == 0 && (!grad || (p.dz_stride % 4 == 0 && (uintptr_t)p.dz % bytes == 0));
   const int E = p.experts;
+  // Few lanes a token, each with 16 of its experts: what a reduction over lanes costs is shared by the tokens of a warp.  us of 65536
+  // tokens, 128 experts, forward and gradient: a warp a token 24.7 and 20.2, 8 lanes a token BAL_NEW.
   if (vec) {
-    if (E <= 32) return balance_launch<T, 8, 4, true>(p, grad, st);
-    if (E <= 64) return balance_launch<T, 16, 4, true>(p, grad, st);
-    if (E <= 128) return balance_launch<T, 32, 4, true>(p, grad, st);
-    if (E <= 256) return balance_launch<T, 32, 8, true>(p, grad, st);
+    if (E <= 8) return balance_launch<T, 2, 4, true>(p, grad, st);
+    if (E <= 16) return balance_launch<T, 4, 4, true>(p, grad, st);
+    if (E <= 32) return balance_launch<T, 2, 16, true>(p, grad, st);
+    if (E <= 64) return balance_launch<T, 4, 16, true>(p, grad, st);
+    if (E <= 128) return balance_launch<T, 8, 16, true>(p, grad, st);
+    if (E <= 256) return balance_launch<T, 16, 16, true>(p, grad, st);
+    if (E <= 512) return balance_launch<T, 32, 16, true>(p, grad, st);
     return balance_launch<T, 32, 32, true>(p, grad, st);
   }
   if (E <= 32) return balance_launch<T, 32, 1, false>(p, grad, st);
@@ -298,7 +321,7 @@ extern "C" int tkv_moe_balance(const void* logits, int64_t logit_stride, const v
   using namespace tkv;
   if (tokens < 0 || tokens > INT32_MAX || experts < 1 || top < 0 || elem_size(dtype) == 0 || (choice_bits != 32 && choice_bits != 64))
     return fail(TKV_ERR_ARG, "tkv_moe_balance: tokens=%lld experts=%d top=%d dtype=%d, choices of %d bits", (long long)tokens, experts, top, dtype, choice_bits);
-  if (experts > 1024 || top > 1024 || tokens * top > INT32_MAX)
+  if (experts > kBalExperts || top > 1024 || tokens * top > INT32_MAX)
     return fail(TKV_ERR_UNSUPPORTED, "tkv_moe_balance: %d of %d experts (at most 1024), %lld tokens (at most 2^31 choices)", top, experts, (long long)tokens);
   if ((tokens && (!logits || (top && !choice))) || !loss || !counts || !load || !workspace) return fail(TKV_ERR_ARG, "tkv_moe_balance: NULL pointer argument");
   if (workspace_bytes < tkv_moe_balance_workspace_bytes(tokens, experts)) return fail(TKV_ERR_ARG, "tkv_moe_balance: workspace too small");
@@ -317,7 +340,7 @@ extern "C" int tkv_moe_balance_grad(const void* logits, int64_t logit_stride, co
   using namespace tkv;
   if (tokens < 0 || tokens > INT32_MAX || experts < 1 || elem_size(dtype) == 0)
     return fail(TKV_ERR_ARG, "tkv_moe_balance_grad: tokens=%lld experts=%d dtype=%d", (long long)tokens, experts, dtype);
-  if (experts > 1024) return fail(TKV_ERR_UNSUPPORTED, "tkv_moe_balance_grad: %d experts (at most 1024)", experts);
+  if (experts > kBalExperts) return fail(TKV_ERR_UNSUPPORTED, "tkv_moe_balance_grad: %d experts (at most 1024)", experts);
   if (tokens == 0) return TKV_OK;
   if (!logits || !load || !grad || !dlogits) return fail(TKV_ERR_ARG, "tkv_moe_balance_grad: NULL pointer argument");
   Balance p = {};

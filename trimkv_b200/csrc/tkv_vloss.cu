@@ -62,7 +62,7 @@ struct VgProduct {
   const int32_t* count;
   int token_axis;                                          // 0: m, 2: k
   int64_t col0;                                            // column 0 is this of the vocabulary
-  int split; int64_t split_len;                            // share s covers k in [s split_len, ..)
+  int split; int64_t split_len;                            // kVgShare: most shares; the whole of k
   int more;                                                // shares are added to what is there
   Vloss l;
 };
@@ -120,7 +120,13 @@ __global__ void __launch_bounds__(kVgThreads, 2) vloss_any_kernel(const __grid_c
   const int64_t count = *p.count;
   const int64_t m = p.token_axis == 0 ? min(p.m, count) : p.m, kend = p.token_axis == 2 ? min(p.k, count) : p.k;
   const int64_t m0 = (int64_t)blockIdx.x * kVgTile, n0 = (int64_t)blockIdx.y * kVgTile;
-  const int64_t k_first = (int64_t)blockIdx.z * p.split_len, k_last = min(kend, k_first + p.split_len);
+  int64_t split_len = p.split_len;
+  if (kMode == kVgShare) {                                 // as many shares as the device chose, of the grid's
+    const int64_t slots = *p.l.slots;
+    if ((int64_t)blockIdx.z >= slots) return;
+    split_len = ((p.split_len + slots - 1) / slots + kVgK - 1) / kVgK * kVgK;
+  }
+  const int64_t k_first = (int64_t)blockIdx.z * split_len, k_last = min(kend, k_first + split_len);
   if (m0 >= m) return;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   float2 acc[8][4];
@@ -195,7 +201,7 @@ __global__ void __launch_bounds__(kVgThreads, 2) vloss_any_kernel(const __grid_c
         for (int j = 0; j < 8; ++j)
           if (col[j] < p.n) reinterpret_cast<float*>(p.l.dl)[row * p.l.piece + col[j]] = g * (exp2f(fmaf(v[j] - lse.x, kLog2e, -lse.y)) - (col[j] == label ? 1.f : 0.f));
       } else if constexpr (kMode == kVgShare) {
-        float* out = p.l.acc + ((int64_t)blockIdx.z * p.l.tokens + row) * p.n;
+        float* out = p.l.acc + ((int64_t)blockIdx.z * count + row) * p.n;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           if (col[j] < p.n) out[col[j]] = p.more ? out[col[j]] + v[j] : v[j];
@@ -235,15 +241,14 @@ static int64_t any_piece(int tokens, int64_t vocab) {
   if (n < 1024) n = 1024;
   return n < vocab ? n : vl_round(vocab, 4);
 }
-// Shares of dx's inner axis, so that its few tiles of [tokens, width] fill the GPU.
-static int any_slots(int tokens, int width, int64_t piece) {
+// Room for shares of dx, whose few tiles of [tokens, width] are as long as the piece (the device chooses how many it uses).
+static int any_slots(int tokens, int width) {
   const int64_t tiles = ((tokens + kVgTile - 1) / kVgTile) * (int64_t)((width + kVgTile - 1) / kVgTile);
-  int64_t s = (2 * 148 + tiles - 1) / (tiles > 0 ? tiles : 1), most = (piece + 255) / 256;
-  if (s > most) s = most;
-  return (int)(s < 1 ? 1 : s > 32 ? 32 : s);
+  const int64_t s = (8 * 148 + tiles - 1) / (tiles > 0 ? tiles : 1);
+  return (int)(s < 1 ? 1 : s > kVlMaxSlots ? kVlMaxSlots : s);
 }
 
-template <typename T> static int vloss_any_backward(Vloss l, bool want_dx, cudaStream_t st) {
+template <typename T> static int vloss_any_backward(Vloss l, bool want_dx, int most_slots, cudaStream_t st) {
   for (int64_t v0 = 0; v0 < l.vocab; v0 += l.piece) {
     const int64_t n = l.vocab - v0 < l.piece ? l.vocab - v0 : l.piece;
     const T* w = reinterpret_cast<const T*>(l.w) + v0 * l.width;
@@ -255,7 +260,7 @@ template <typename T> static int vloss_any_backward(Vloss l, bool want_dx, cudaS
     int rc = vg_launch<T, true, T, true, kVgLogitGrad, T>(p, st);
     if (rc == TKV_OK && want_dx) {
       p.a = dl; p.b = wk; p.m = l.tokens; p.n = l.width; p.k = n; p.token_axis = 0;
-      p.split = l.slots; p.split_len = vl_round((n + l.slots - 1) / l.slots, kVgK); p.more = v0 > 0;
+      p.split = most_slots; p.split_len = l.piece; p.more = v0 > 0;
       rc = vg_launch<float, true, T, false, kVgShare, T>(p, st);
     }
     if (rc == TKV_OK && l.dw) {
@@ -326,17 +331,34 @@ __global__ void __launch_bounds__(kSumThreads) vloss_sum_kernel(const float* los
 
 // Gradient of every counting row's loss, times a power of two that brings the largest to about 2^14: fp16 keeps what is small beside it
 // (a mean over many tokens makes all of them small), and exponents of bf16 and fp32 are only shifted.
-__global__ void __launch_bounds__(kSumThreads) vloss_rows_grad_kernel(const float* grad, int64_t stride, int reduction, VlossPlan plan, float* g, float* scale) {
+// And the shares of dx: the tiles of a launch are dealt out in turn, those of dx first; with s shares a tile of dx takes steps / s (and a
+// little for what it writes), one of dw the tokens' steps.  The s that makes the busiest worker's work least.
+__global__ void __launch_bounds__(kSumThreads) vloss_rows_grad_kernel(const float* grad, int64_t stride, int reduction, VlossPlan plan, VlossWork work, float* g,
+                                                                      float* scale, int* slots) {
   __shared__ float red[kSumThreads / 32];
+  __shared__ int cost[kVlMaxSlots];
   grid_dependency_wait();
   grid_launch_dependents();
-  const int n = plan.head[0];
+  const int n = plan.head[0], lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const float by = reduction == 1 ? 1.0f / (float)n : 1.0f;
   float top = 0.f;
   for (int i = threadIdx.x; i < n; i += kSumThreads) top = fmaxf(top, fabsf(grad[(int64_t)plan.rows[i] * stride] * by));
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
+  if (lane == 0) red[warp] = top;
+  {
+    const int s = warp + 1, mt = (n + work.rows - 1) / work.rows;                    // this warp looks at s shares
+    const int dx = work.dx ? mt * work.ht * s : 0, all = dx + (work.dw ? work.vt * work.ht : 0);
+    const int dx_cost = (work.steps + s - 1) / s + 12, dw_cost = (n + work.step - 1) / work.step + 4;
+    int most = 0;
+    for (int w = lane; w < work.workers; w += 32) {
+      const int mine = dx > w ? (dx - w - 1) / work.workers + 1 : 0, total = all > w ? (all - w - 1) / work.workers + 1 : 0;
+      most = max(most, mine * dx_cost + (total - mine) * dw_cost);
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    const bool fits = s == 1 || ((int64_t)s * ((n + work.acc_rows - 1) / work.acc_rows * work.acc_rows) <= (int64_t)work.room * work.tokens && work.steps >= 8 * s);
+    if (lane == 0) cost[warp] = fits ? most : INT32_MAX;
+  }
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kSumThreads / 32; ++w) top = fmaxf(top, red[w]);
@@ -344,8 +366,15 @@ __global__ void __launch_bounds__(kSumThreads) vloss_rows_grad_kernel(const floa
   if (top > 0.f && top < INFINITY) e = min(max(14 - ilogbf(top), -100), 100);
   const float s = ldexpf(1.f, e);
   for (int i = threadIdx.x; i < n; i += kSumThreads) g[i] = grad[(int64_t)plan.rows[i] * stride] * by * s;
-  if (threadIdx.x == 0) { scale[0] = s; scale[1] = ldexpf(1.f, -e); }
+  if (threadIdx.x == 0) {
+    scale[0] = s; scale[1] = ldexpf(1.f, -e);
+    int best = 0;
+    for (int i = 1; i < kVlMaxSlots; ++i)
+      if (cost[i] < cost[best]) best = i;
+    *slots = best + 1;
+  }
 }
+static_assert(kSumThreads / 32 == kVlMaxSlots, "a warp for every number of shares");
 
 constexpr int kDxThreads = 256;
 
@@ -361,15 +390,17 @@ template <typename T> __global__ void __launch_bounds__(kDxThreads) vloss_dx_ker
     if (p.plan.rows[mid] < t) lo = mid + 1; else hi = mid;
   }
   const bool live = lo < n && p.plan.rows[lo] == t;
+  const int slots = *p.slots;
+  const int64_t each = ((int64_t)n + p.acc_rows - 1) / p.acc_rows * p.acc_rows;
   const float back = p.plan.head[2] ? __int_as_float(0x7fffffff) : p.g_scale[1];
   T* out = dx + (int64_t)t * p.width;
   if (p.width % 8 == 0) {
     for (int c = threadIdx.x * 8; c < p.width; c += kDxThreads * 8) {
       float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       if (live)
-        for (int i = 0; i < p.slots; ++i) {
+        for (int i = 0; i < slots; ++i) {
           float v[8];
-          load_vec<8>(p.acc + ((int64_t)i * p.tokens + lo) * p.width + c, v);
+          load_vec<8>(p.acc + (i * each + lo) * p.width + c, v);
 #pragma unroll
           for (int e = 0; e < 8; ++e) s[e] += v[e];
         }
@@ -384,7 +415,7 @@ template <typename T> __global__ void __launch_bounds__(kDxThreads) vloss_dx_ker
   for (int c = threadIdx.x; c < p.width; c += kDxThreads) {
     float s = 0.f;
     if (live)
-      for (int i = 0; i < p.slots; ++i) s += p.acc[((int64_t)i * p.tokens + lo) * p.width + c];
+      for (int i = 0; i < slots; ++i) s += p.acc[(i * each + lo) * p.width + c];
     out[c] = from_f32<T>(s * back);
   }
 }
@@ -395,12 +426,15 @@ template <typename... A> static int vl_launch(const char* what, void (*kernel)(A
   return check_launch(what);
 }
 
+int vloss_plan_rows(const Vloss& p, const int64_t* labels, int64_t ignore, float* loss, cudaStream_t st) {
+  return vl_launch("tkv_vloss_forward", vloss_plan_kernel, dim3(1), kPlanThreads, st, labels, ignore, p.tokens, p.vocab, p.plan, loss, p.status);
+}
 static bool use_tc(const Vloss& p) { return vloss_tc_shape(p.tokens, p.vocab, p.width, p.dtype) && aligned16(p.w) && (p.dw == nullptr || aligned16(p.dw)); }
 static int64_t pad256(int64_t bytes) { return vl_round(bytes, 256); }
 static int64_t any_forward_bytes(int tokens, int64_t vocab) { return (int64_t)tokens * ((vocab + kVgTile - 1) / kVgTile) * 8; }
 static int64_t any_backward_bytes(int tokens, int64_t vocab, int width, bool dx) {
   const int64_t piece = any_piece(tokens, vocab);
-  return pad256((int64_t)tokens * piece * 4) + (dx ? (int64_t)any_slots(tokens, width, piece) * tokens * width * 4 : 0);
+  return pad256((int64_t)tokens * piece * 4) + (dx ? (int64_t)any_slots(tokens, width) * tokens * width * 4 : 0);
 }
 static int check_sizes(const char* what, int64_t tokens, int64_t vocab, int width, int64_t x_stride, int dtype) {
   if (tokens < 0 || vocab < 1 || width < 1 || elem_size(dtype) == 0 || (tokens > 1 && x_stride < width))
@@ -442,13 +476,17 @@ extern "C" int tkv_vloss_forward(const void* x, int64_t x_stride, const void* w,
   p.plan = vloss_plan(plan, tokens); p.status = status;
   p.mine = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + 512);
   void* rest = reinterpret_cast<char*>(p.mine) + pad256(tokens * 4);
-  int rc = vl_launch("tkv_vloss_forward", vloss_plan_kernel, dim3(1), kPlanThreads, st, labels, ignore, p.tokens, vocab, p.plan, loss, status);
-  if (rc == TKV_OK && tokens) {
+  int rc;
+  if (tokens && use_tc(p)) {
+    rc = vloss_tc_forward(p, labels, ignore, loss, rest, st);
+  } else {
+    rc = vloss_plan_rows(p, labels, ignore, loss, st);
     p.part = reinterpret_cast<float2*>(rest);
     p.tiles = (int)((vocab + kVgTile - 1) / kVgTile);
-    rc = use_tc(p) ? vloss_tc_forward(p, rest, st) : dtype == TKV_F32 ? vloss_any_forward<float>(p, st) : dtype == TKV_BF16 ? vloss_any_forward<__nv_bfloat16>(p, st) : vloss_any_forward<__half>(p, st);
-    if (rc == TKV_OK) rc = vl_launch("tkv_vloss_forward", vloss_join_kernel, dim3((unsigned)tokens), kJoinThreads, st, p, loss);
+    if (rc == TKV_OK && tokens)
+      rc = dtype == TKV_F32 ? vloss_any_forward<float>(p, st) : dtype == TKV_BF16 ? vloss_any_forward<__nv_bfloat16>(p, st) : vloss_any_forward<__half>(p, st);
   }
+  if (rc == TKV_OK && tokens) rc = vl_launch("tkv_vloss_forward", vloss_join_kernel, dim3((unsigned)tokens), kJoinThreads, st, p, loss);
   if (rc == TKV_OK && reduction) rc = vl_launch("tkv_vloss_forward", vloss_sum_kernel, dim3(1), kSumThreads, st, (const float*)loss, p.tokens, p.plan, reduction, reduced);
   return rc;
 }
@@ -475,18 +513,24 @@ extern "C" int tkv_vloss_backward(const void* x, int64_t x_stride, const void* w
   float* scale = reinterpret_cast<float*>(workspace);
   float* g = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + 512);
   char* rest = reinterpret_cast<char*>(g) + pad256(tokens * 4);
-  p.g = g; p.g_scale = scale;
-  int rc = vl_launch("tkv_vloss_backward", vloss_rows_grad_kernel, dim3(1), kSumThreads, st, grad, grad_stride, reduction, p.plan, g, scale);
+  p.g = g; p.g_scale = scale; p.slots = reinterpret_cast<int*>(scale) + 2;
+  const bool tc = use_tc(p);
+  const int64_t piece = any_piece(p.tokens, vocab);
+  const int room = any_slots(p.tokens, width);
+  const VlossWork work = tc ? vloss_tc_work(p.tokens, vocab, width, dx != nullptr, dw != nullptr)
+                            : VlossWork{2 * 148, kVgTile, 1, (width + kVgTile - 1) / kVgTile, 0, (int)((piece + kVgK - 1) / kVgK), kVgK, room, p.tokens, dx != nullptr, false};
+  int rc = vl_launch("tkv_vloss_backward", vloss_rows_grad_kernel, dim3(1), kSumThreads, st, grad, grad_stride, reduction, p.plan, work, g, scale,
+                     reinterpret_cast<int*>(scale) + 2);
   if (rc != TKV_OK) return rc;
-  if (use_tc(p)) {
+  p.acc_rows = work.acc_rows;
+  if (tc) {
     rc = vloss_tc_backward(p, rest, dx != nullptr, st);
   } else {
-    p.piece = any_piece(p.tokens, vocab);
-    p.slots = any_slots(p.tokens, width, p.piece);
+    p.piece = piece;
     p.dl = rest;
-    p.acc = reinterpret_cast<float*>(rest + pad256(tokens * p.piece * 4));
-    rc = dtype == TKV_F32 ? vloss_any_backward<float>(p, dx != nullptr, st)
-                        : dtype == TKV_BF16 ? vloss_any_backward<__nv_bfloat16>(p, dx != nullptr, st) : vloss_any_backward<__half>(p, dx != nullptr, st);
+    p.acc = reinterpret_cast<float*>(rest + pad256(tokens * piece * 4));
+    rc = dtype == TKV_F32 ? vloss_any_backward<float>(p, dx != nullptr, room, st)
+                          : dtype == TKV_BF16 ? vloss_any_backward<__nv_bfloat16>(p, dx != nullptr, room, st) : vloss_any_backward<__half>(p, dx != nullptr, room, st);
   }
   if (rc != TKV_OK || dx == nullptr) return rc;
   if (dtype == TKV_F32) return vl_launch("tkv_vloss_backward", vloss_dx_kernel<float>, dim3((unsigned)tokens), kDxThreads, st, p, (float*)dx);

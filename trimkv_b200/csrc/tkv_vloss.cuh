@@ -38,18 +38,28 @@ struct Vloss {
   // backward
   const float* g;                                          // [tokens] gradient of each counting row's loss, times g_scale
   const float* g_scale;                                    // [2] scale and its inverse
+  const int* slots;                                        // shares of dx
   void* dl; int64_t piece;                                 // [tokens][piece]
-  float* acc; int slots;                                   // [slots][tokens][width] shares of dx
+  float* acc;                                              // [*slots][tokens that count, whole tiles of acc_rows][width] shares of dx
+  int acc_rows;
   void* dw;
 };
 
 inline int64_t vl_round(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
+constexpr int kVlMaxSlots = 32;
+// What a launch of the gradients has to share out, for the choice of the shares of dx: workers, rows of a tile and what rows
+// of a share are rounded to, tiles of the width and of a piece, steps of a piece, elements of a step, room for shares of `tokens` rows.
+struct VlossWork { int workers, rows, acc_rows, ht, vt, steps, step, room, tokens; bool dx, dw; };
+
+int vloss_plan_rows(const Vloss& p, const int64_t* labels, int64_t ignore, float* loss, cudaStream_t st);
+
 // The form on the tensor cores (tkv_vloss_tc.cu): 16-bit types, widths of whole 16-byte vectors, w and dw on 16 bytes; x of any alignment.
 bool vloss_tc_shape(int tokens, int64_t vocab, int width, int dtype);
 int64_t vloss_tc_forward_bytes(int tokens, int64_t vocab, int width);
 int64_t vloss_tc_backward_bytes(int tokens, int64_t vocab, int width, bool dx);
-int vloss_tc_forward(Vloss& p, void* ws, cudaStream_t st);                   // fills part and mine, sets tiles
-int vloss_tc_backward(Vloss& p, void* ws, bool want_dx, cudaStream_t st);    // fills dw and acc, sets slots
+VlossWork vloss_tc_work(int tokens, int64_t vocab, int width, bool want_dx, bool want_dw);
+int vloss_tc_forward(Vloss& p, const int64_t* labels, int64_t ignore, float* loss, void* ws, cudaStream_t st);   // the plan, part and mine; sets tiles
+int vloss_tc_backward(Vloss& p, void* ws, bool want_dx, cudaStream_t st);                                        // dw and acc
 
 }  // namespace tkv

@@ -33,14 +33,17 @@ struct VtSmem {
   uint32_t tmem_base;
   int abort_flag;
 };
-constexpr int kVtSmemBytes = kVtStages * kVtStage + (int)sizeof(VtSmem);
+constexpr int kVtOut = 4096;                               // 32 rows of 128 bytes on their way out, two per warp of the epilogue
+constexpr int kVtSmemBytes = kVtStages * kVtStage + 8 * kVtOut + (int)sizeof(VtSmem);
+static_assert(kVtSmemBytes <= 232448, "shared memory");
 
 struct VtParams {
   Vloss l;
   int cols;                                                // of a tile (a multiple of 16)
+  int a_box, a_ranks;                                      // rows of x or dL that a CTA fetches, CTAs of a pair that have any (few tokens)
   int64_t v0, piece_cols;                                  // the vocabulary from v0 (kVtStats: all of it)
-  int64_t piece_pitch;
-  int want_dx, want_dw, more, split_steps;                 // kVtGrads: stages of a share of dx
+  int want_dx, want_dw, more;                              // kVtGrads
+  int64_t piece_steps;                                     // stages of a whole piece
 };
 
 // ---- instructions for pairs of CTAs
@@ -82,7 +85,7 @@ struct VtTile {
 };
 template <int kMode> struct VtTiles {
   const VtParams& p;
-  int n, tile, count, dx_count, mt, nt, ht, vt, slots;
+  int n, tile, count, dx_count, mt, nt, ht, vt, slots, split;
   __device__ __forceinline__ VtTiles(const VtParams& q, int pair) : p(q) {
     n = q.l.plan.head[0];
     tile = pair - kVtPairs;
@@ -90,7 +93,8 @@ template <int kMode> struct VtTiles {
     if (kMode == kVtGrads) {
       ht = (q.l.width + kVtCols - 1) / kVtCols;
       vt = (int)((q.piece_cols + kVtRows - 1) / kVtRows);
-      slots = q.l.slots;
+      slots = *q.l.slots;
+      split = ((int)q.piece_steps + slots - 1) / slots;
       dx_count = q.want_dx ? mt * ht * slots : 0;
       count = dx_count + (q.want_dw ? vt * ht : 0);
     } else {
@@ -109,8 +113,8 @@ template <int kMode> struct VtTiles {
       if (t.dx) {
         t.row0 = r / slots * kVtRows;
         t.slot = r % slots;
-        t.step0 = t.slot * p.split_steps;
-        t.steps = max(0, min(p.split_steps, (int)((p.piece_cols + kVtK - 1) / kVtK) - t.step0));
+        t.step0 = t.slot * split;
+        t.steps = max(0, min(split, (int)((p.piece_cols + kVtK - 1) / kVtK) - t.step0));
       } else {
         t.row0 = r * kVtRows;
         t.slot = t.step0 = 0;
@@ -137,13 +141,15 @@ template <typename T> __device__ __forceinline__ uint32_t vt_pack(float a, float
   }
 }
 
-// Maps: a, b of the logits (x, w, K-major); of the gradients dL along and across (a, a2), w across (b), x across (b2).
+// Maps: a, b of the logits (x, w, K-major), c: dL; of the gradients dL along and across (a, a2), w across (b), x across (b2), shares of dx
+// (c), dw (d).
 template <int kMode, typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kVtThreads, 1)
 vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_a2,
-                const __grid_constant__ CUtensorMap map_b2, const __grid_constant__ VtParams p) {
+                const __grid_constant__ CUtensorMap map_b2, const __grid_constant__ CUtensorMap map_c, const __grid_constant__ CUtensorMap map_d,
+                const __grid_constant__ VtParams p) {
   extern __shared__ __align__(1024) uint8_t base[];
-  VtSmem* sm = reinterpret_cast<VtSmem*>(base + kVtStages * kVtStage);
+  VtSmem* sm = reinterpret_cast<VtSmem*>(base + kVtStages * kVtStage + 8 * kVtOut);
   const int tid = threadIdx.x, warp = warp_uniform(tid >> 5), lane = tid & 31;
   const int rank = (int)vt_rank(), pair = blockIdx.x >> 1;
   volatile int* abort_flag = &sm->abort_flag;
@@ -182,7 +188,8 @@ vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     while (ok && tiles.next(t)) {
       const bool a_mn = kMode == kVtGrads && !t.dx, b_mn = kMode == kVtGrads;
       const int half = kMode == kVtGrads ? kVtCols / 2 : p.cols / 2;
-      const uint32_t bytes = 2 * (kVtABytes + half * kVtK * 2);          // of both CTAs
+      const int box = a_mn ? 128 : p.a_box, ranks = a_mn ? 2 : p.a_ranks;
+      const uint32_t bytes = (ranks * box + 2 * half) * kVtK * 2;        // of both CTAs
       const int arow = t.row0 + rank * 128, brow = t.col0 + rank * half;
       for (int k = t.step0; k < t.step0 + t.steps; ++k, ++it) {
         const int s = it % kVtStages;
@@ -194,7 +201,7 @@ vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
           if (a_mn) {
             vt_load(a, &map_a2, bar, arow, k * kVtK);
             vt_load(a + kVtABytes / 2, &map_a2, bar, arow + 64, k * kVtK);
-          } else {
+          } else if (rank < ranks) {                       // rows beyond the box hold what was there: rows of D that nobody reads
             vt_load(a, &map_a, bar, k * kVtK, arow);
           }
           if (b_mn) {
@@ -255,7 +262,20 @@ vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     // ---- epilogue: thread = row of the CTA's half of the tile
     const int quarter = warp & 3, row_in = quarter * 32 + lane;
     const uint32_t acc_empty0 = vt_of_rank(smem_u32(&sm->acc_empty[0]), 0);
-    int acc = 0;
+    int acc = 0, outs = 0;
+    uint8_t* out_s = base + kVtStages * kVtStage + quarter * 2 * kVtOut;
+    // 32 rows of 128 bytes by a bulk copy: a lane puts the eight 16-byte pieces of its row in the swizzled places.  Two boxes per warp: one
+    // is filled while the other leaves.
+    auto put = [&](const uint32_t* w) {
+      if (lane == 0 && outs >= 2) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+      __syncwarp();
+      uint8_t* box = out_s + (outs & 1) * kVtOut + lane * 128;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(box + ((i ^ (lane & 7)) << 4)) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+      fence_async_smem();
+      __syncwarp();
+    };
+    auto box_of = [&]() { return out_s + (outs & 1) * kVtOut; };
     bool ok = *abort_flag == 0;
     while (ok && tiles.next(t)) {
       const int buf = acc & 1;
@@ -302,52 +322,64 @@ vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         const float2 lse = live ? p.l.plan.lse[row] : make_float2(0.f, 0.f);
         const float g = live ? p.l.g[row] : 0.f;
         const int left = (int)min((int64_t)p.cols, p.piece_cols - t.col0);
-        T* out = reinterpret_cast<T*>(p.l.dl) + (int64_t)row * p.piece_pitch + t.col0;
-        for (int c = 0; c < p.cols; c += 32) {
-          float v[32];
-          tmem_ld32(from + c, v);
+        const int first = t.row0 + rank * 128 + quarter * 32;
+        // the products to come read whole steps of rows
+        for (int c = first < (tiles.n + kVtK - 1) / kVtK * kVtK ? 0 : p.cols; c < p.cols; c += 64) {
+          uint32_t w[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float d = exp2_weight(fmaf(v[i] - lse.x, kLog2e, -lse.y)) - (i == label - c ? 1.f : 0.f);
-            v[i] = live && c + i < left ? g * d : 0.f;     // rows and columns that do not exist are zeros for the products to come
+          for (int h = 0; h < 2; ++h) {
+            float v[32];
+            tmem_ld32(from + c + 32 * h, v);
+            const int at = c + 32 * h;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {                 // rows and columns that do not exist are zeros for the products to come
+              const float d = exp2_weight(fmaf(v[i] - lse.x, kLog2e, -lse.y)) - (i == label - at ? 1.f : 0.f);
+              v[i] = live && at + i < left ? g * d : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[16 * h + i] = vt_pack<T>(v[2 * i], v[2 * i + 1]);
           }
-#pragma unroll
-          for (int i = 0; i < 32; i += 8)
-            st16(out + c + i, make_uint4(vt_pack<T>(v[i], v[i + 1]), vt_pack<T>(v[i + 2], v[i + 3]), vt_pack<T>(v[i + 4], v[i + 5]), vt_pack<T>(v[i + 6], v[i + 7])));
+          put(w);
+          if (lane == 0) tma_store_2d(&map_c, box_of(), t.col0 + c, first);
+          ++outs;
         }
       } else {
-        const int left = p.l.width - t.col0;               // a multiple of 8
-        const bool live = t.dx ? row < tiles.n : row < p.piece_cols;
+        const int left = p.l.width - t.col0, first = t.row0 + rank * 128 + quarter * 32;
         const float back = t.dx ? 0.f : p.l.g_scale[1];
-        float* share = p.l.acc + ((int64_t)t.slot * p.l.tokens + row) * p.l.width + t.col0;
-        T* out = reinterpret_cast<T*>(p.l.dw) + (p.v0 + row) * p.l.width + t.col0;
-        for (int c = 0; c < kVtCols && c < left; c += 32) {
-          float v[32];
-          if (t.steps > 0) tmem_ld32(from + c, v);
-          else {
+        if (t.dx) {                                        // a share's rows are whole tiles
+          for (int c = 0; first < tiles.n && c < kVtCols && c < left; c += 32) {
+            float v[32];
+            if (t.steps > 0) tmem_ld32(from + c, v);
+            else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = 0.f;
-          }
-          if (live && t.dx) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              if (c + i < left) {
-                float4 w = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-                if (p.more) {
-                  const float4 o = *reinterpret_cast<const float4*>(share + c + i);
-                  w.x += o.x; w.y += o.y; w.z += o.z; w.w += o.w;
-                }
-                *reinterpret_cast<float4*>(share + c + i) = w;
-              }
+              for (int i = 0; i < 32; ++i) v[i] = 0.f;
             }
-          } else if (live) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 8)
-              if (c + i < left)
-                st16(out + c + i, make_uint4(vt_pack<T>(v[i] * back, v[i + 1] * back), vt_pack<T>(v[i + 2] * back, v[i + 3] * back),
-                                             vt_pack<T>(v[i + 4] * back, v[i + 5] * back), vt_pack<T>(v[i + 6] * back, v[i + 7] * back)));
+            put(reinterpret_cast<const uint32_t*>(v));
+            if (lane == 0) {
+              const int y = t.slot * tiles.mt * kVtRows + first;
+              if (p.more) tma_add_2d(&map_c, box_of(), t.col0 + c, y);
+              else tma_store_2d(&map_c, box_of(), t.col0 + c, y);
+            }
+            ++outs;
           }
-          __syncwarp();
+        } else if (first < p.piece_cols) {
+          for (int c = 0; c < kVtCols && c < left; c += 64) {
+            uint32_t w[32];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float v[32];
+              if (t.steps > 0) tmem_ld32(from + c + 32 * h, v);
+              else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = 0.f;
+              }
+#pragma unroll
+              for (int i = 0; i < 16; ++i) w[16 * h + i] = vt_pack<T>(v[2 * i] * back, v[2 * i + 1] * back);
+            }
+            put(w);
+            if (lane == 0) tma_store_2d(&map_d, box_of(), t.col0 + c, (int)p.v0 + first);
+            ++outs;
+          }
         }
       }
       tc_fence_before();
@@ -355,6 +387,7 @@ vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       if (lane == 0) vt_arrive(acc_empty0 + buf * 8);
       ++acc;
     }
+    if (lane == 0 && kMode != kVtStats) tma_store_done();
     if (!ok && lane == 0) give_up();
   }
   __syncwarp();
@@ -390,36 +423,94 @@ template <bool kVec> __global__ void __launch_bounds__(kVtGatherThreads) vloss_g
   }
 }
 
+constexpr int kVtFirst = 1024;                             // most tokens for which every CTA can look through the labels itself
+
+// vloss_plan_kernel and vloss_gather_kernel in one launch, for few tokens: every CTA finds its row among the labels.  The grid is the rows
+// that the logits' boxes reach.
+template <bool kVec> __global__ void __launch_bounds__(kVtGatherThreads) vloss_first_kernel(const int64_t* labels, int64_t ignore, int tokens, int64_t vocab, VlossPlan plan,
+                                                                                        float* loss, int32_t* status, const uint16_t* x, int64_t x_stride, int width, uint16_t* xc) {
+  constexpr int kPer = kVtFirst / kVtGatherThreads;
+  __shared__ int sums[kVtGatherThreads / 32 + 1], token, bad_any;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  if (threadIdx.x == 0) bad_any = 0;
+  int64_t y[kPer];
+  int n = 0;
+  bool bad = false;
+  const int t1 = threadIdx.x * kPer;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    y[i] = t1 + i < tokens ? labels[t1 + i] : ignore;
+    const bool off = y[i] != ignore && (y[i] < 0 || y[i] >= vocab);
+    if (blockIdx.x == 0 && t1 + i < tokens && (off || y[i] == ignore)) loss[t1 + i] = off ? __int_as_float(0x7fffffff) : 0.f;
+    bad |= off;
+    if (off) y[i] = ignore;
+    n += y[i] != ignore;
+  }
+  if (bad) bad_any = 1;
+  int total;
+  int at = block_exclusive_scan<kVtGatherThreads>(n, sums, &total);
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+    if (y[i] != ignore) {
+      if (at == (int)blockIdx.x) token = t1 + i;
+      if (blockIdx.x == 0) { plan.rows[at] = t1 + i; plan.label[at] = (int32_t)y[i]; }
+      ++at;
+    }
+  __syncthreads();
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    plan.head[0] = total; plan.head[1] = bad_any; plan.head[2] = plan.head[3] = 0;
+    if (bad_any) report(status, TKV_DEV_BAD_INDEX);
+  }
+  if ((int)blockIdx.x >= (total + kVtRows - 1) / kVtRows * kVtRows) return;
+  uint16_t* out = xc + (int64_t)blockIdx.x * width;
+  const bool live = (int)blockIdx.x < total;
+  const uint16_t* in = x + (live ? token : 0) * x_stride;
+  for (int c = threadIdx.x * 8; c < width; c += kVtGatherThreads * 8) {
+    if (!live) st16(out + c, make_uint4(0, 0, 0, 0));
+    else if (kVec) st16(out + c, ld16_stream(in + c));
+    else
+      for (int e = 0; e < 8; ++e) out[c + e] = in[c + e];
+  }
+}
+
 // ------------------------------------------------------------------------------------------------------------------ the host
 bool vloss_tc_shape(int tokens, int64_t vocab, int width, int dtype) { return (dtype == TKV_BF16 || dtype == TKV_F16) && width % 8 == 0 && tokens > 0; }
 
 static int64_t vt_rows(int tokens) { return vl_round(tokens, kVtRows); }
-// Columns of a tile: the fewest that keep the number of rounds over the pairs that 256 columns need (few tokens: a last round that is
-// nearly empty costs as much as a whole one).
+// Columns of a tile: what a pair does in its rounds is rounds x columns, and a little per round; few rounds make it matter that the last
+// one is full.  us of one token, 151936 words, width 2048: 256 columns 106, by this rule (208) VL_ONE.
 static int vt_tile_cols(int tokens, int64_t vocab) {
-  const int64_t mt = vt_rows(tokens) / kVtRows, nt = (vocab + kVtCols - 1) / kVtCols, rounds = (mt * nt + kVtPairs - 1) / kVtPairs;
-  if (rounds > 16) return kVtCols;
-  int64_t most = rounds * kVtPairs / mt;                   // tiles of columns that fit those rounds
-  if (most < 1) most = 1;
-  const int64_t cols = vl_round((vocab + most - 1) / most, 16);
-  return (int)(cols < 32 ? 32 : cols > kVtCols ? kVtCols : cols);
+  const int64_t mt = vt_rows(tokens) / kVtRows;
+  if (mt * ((vocab + kVtCols - 1) / kVtCols) > 20 * kVtPairs) return kVtCols;
+  int best = kVtCols;
+  int64_t least = INT64_MAX;
+  for (int cols = kVtCols; cols >= 128; cols -= 16) {
+    const int64_t rounds = (mt * ((vocab + cols - 1) / cols) + kVtPairs - 1) / kVtPairs;
+    if (rounds * (cols + 16) < least) { least = rounds * (cols + 16); best = cols; }
+  }
+  return best;
 }
+static int vt_a_box(int tokens) { return tokens >= 128 ? 128 : (int)vl_round(tokens, 8); }
 // The vocabulary in equal pieces, of at most 256 MB of dL where that is not fewer than 8192 words.
-static int64_t vt_piece(int tokens, int64_t vocab) {
+static int64_t vl_piece(int tokens, int64_t vocab) {
   int64_t n = ((int64_t)256 << 20) / (2 * vt_rows(tokens)) / kVtCols * kVtCols;
   if (n < 8192) n = 8192;
   const int64_t pieces = (vocab + n - 1) / n;
   return vl_round((vocab + pieces - 1) / pieces, kVtCols);
 }
-// Shares of dx: a tile of dx is as long as the piece, so where few tiles of the launch are, it is cut until it is a third of a pair's part.
-static int vt_slots(int tokens, int width, int64_t piece) {
-  const int64_t mt = vt_rows(tokens) / kVtRows, ht = (width + kVtCols - 1) / kVtCols, ks = piece / kVtK;
-  const int64_t total = mt * ht * ks;                      // stages of dx alone: it may be asked for alone
-  const int64_t part = (total + kVtPairs - 1) / kVtPairs;
-  int64_t s = (3 * ks + part - 1) / (part > 0 ? part : 1);
-  if (s > ks / 8) s = ks / 8;
-  if (mt * ht >= 2 * kVtPairs || s < 1) s = 1;
-  return (int)(s > 32 ? 32 : s);
+// Room for shares of dx.  How many there are is decided on the device, where the number of tokens that count is known (vloss_rows_grad_kernel):
+// a tile of dx is as long as the piece, and its few tiles rarely fill whole rounds of the pairs.
+static int vt_slots(int tokens, int width) {
+  const int64_t tiles = vt_rows(tokens) / kVtRows * ((width + kVtCols - 1) / kVtCols);
+  const int64_t s = (8 * kVtPairs + tiles - 1) / tiles;
+  return (int)(s > kVlMaxSlots ? kVlMaxSlots : s < 1 ? 1 : s);
+}
+VlossWork vloss_tc_work(int tokens, int64_t vocab, int width, bool want_dx, bool want_dw) {
+  const int64_t piece = vl_piece(tokens, vocab);
+  return {kVtPairs, kVtRows, kVtRows, (width + kVtCols - 1) / kVtCols, (int)((piece + kVtRows - 1) / kVtRows), (int)(piece / kVtK), kVtK, vt_slots(tokens, width), (int)vt_rows(tokens),
+          want_dx, want_dw};
 }
 static int64_t vt_pad(int64_t bytes) { return vl_round(bytes, 1024); }
 
@@ -428,8 +519,8 @@ int64_t vloss_tc_forward_bytes(int tokens, int64_t vocab, int width) {
   return 1024 + vt_pad(vt_rows(tokens) * width * 2) + (int64_t)tokens * ((vocab + cols - 1) / cols) * 8;
 }
 int64_t vloss_tc_backward_bytes(int tokens, int64_t vocab, int width, bool dx) {
-  const int64_t piece = vt_piece(tokens, vocab);
-  return 1024 + vt_pad(vt_rows(tokens) * width * 2) + vt_pad(vt_rows(tokens) * piece * 2) + (dx ? (int64_t)vt_slots(tokens, width, piece) * tokens * width * 4 : 0);
+  const int64_t piece = vl_piece(tokens, vocab);
+  return 1024 + vt_pad(vt_rows(tokens) * width * 2) + vt_pad(vt_rows(tokens) * piece * 2) + (dx ? (int64_t)vt_slots(tokens, width) * vt_rows(tokens) * width * 4 : 0);
 }
 
 static int vt_gather(const Vloss& p, void* xc, cudaStream_t st) {
@@ -448,49 +539,63 @@ template <int kMode, typename T> static int vt_launch(const CUtensorMap* m, cons
     e = cudaFuncSetAttribute(vloss_tc_kernel<kMode, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kVtSmemBytes);
     if (e == cudaSuccess && dev >= 0 && dev < 64) allowed[dev] = true;
   }
-  if (e == cudaSuccess) e = launch_pdl(vloss_tc_kernel<kMode, T>, dim3(2 * kVtPairs), dim3(kVtThreads), (size_t)kVtSmemBytes, st, m[0], m[1], m[2], m[3], p);
+  if (e == cudaSuccess) e = launch_pdl(vloss_tc_kernel<kMode, T>, dim3(2 * kVtPairs), dim3(kVtThreads), (size_t)kVtSmemBytes, st, m[0], m[1], m[2], m[3], m[4], m[5], p);
   if (e != cudaSuccess) return fail(TKV_ERR_LAUNCH, "tkv_vloss: %s", cudaGetErrorString(e));
   return check_launch("tkv_vloss");
 }
 
 static void* vt_align(void* p) { return reinterpret_cast<void*>(((uintptr_t)p + 1023) & ~(uintptr_t)1023); }
 
-int vloss_tc_forward(Vloss& l, void* ws, cudaStream_t st) {
+int vloss_tc_forward(Vloss& l, const int64_t* labels, int64_t ignore, float* loss, void* ws, cudaStream_t st) {
   void* xc = vt_align(ws);
+  int rc;
+  if (l.tokens <= kVtFirst) {
+    const bool vec = aligned16(l.x) && l.x_stride % 8 == 0;
+    cudaError_t e = launch_pdl(vec ? vloss_first_kernel<true> : vloss_first_kernel<false>, dim3((unsigned)(l.tokens > 128 ? vt_rows(l.tokens) : vt_a_box(l.tokens))), dim3(kVtGatherThreads), 0, st,
+                               labels, ignore, l.tokens, l.vocab, l.plan, loss, l.status, reinterpret_cast<const uint16_t*>(l.x), l.x_stride, l.width, reinterpret_cast<uint16_t*>(xc));
+    rc = e == cudaSuccess ? check_launch("tkv_vloss") : fail(TKV_ERR_LAUNCH, "tkv_vloss: %s", cudaGetErrorString(e));
+  } else {
+    rc = vloss_plan_rows(l, labels, ignore, loss, st);
+    if (rc == TKV_OK) rc = vt_gather(l, xc, st);
+  }
   VtParams p = {};
   p.cols = vt_tile_cols(l.tokens, l.vocab);
   l.part = reinterpret_cast<float2*>(reinterpret_cast<char*>(xc) + vt_pad(vt_rows(l.tokens) * l.width * 2));
   l.tiles = (int)((l.vocab + p.cols - 1) / p.cols);
-  p.l = l; p.v0 = 0; p.piece_cols = l.vocab;
-  CUtensorMap m[4];
-  int rc = vt_gather(l, xc, st);
-  if (rc == TKV_OK) rc = make_map_2d(&m[0], xc, l.width, vt_rows(l.tokens), kVtK, 128, l.dtype);
-  if (rc == TKV_OK) rc = make_map_2d(&m[1], l.w, l.width, l.vocab, kVtK, p.cols / 2, l.dtype);
+  p.l = l; p.v0 = 0; p.piece_cols = l.vocab; p.a_box = vt_a_box(l.tokens); p.a_ranks = l.tokens > 128 ? 2 : 1;
+  CUtensorMap m[6];
+  if (rc == TKV_OK) rc = make_map_wide(&m[0], xc, l.width, vt_rows(l.tokens), kVtK, p.a_box, l.dtype);
+  if (rc == TKV_OK) rc = make_map_wide(&m[1], l.w, l.width, l.vocab, kVtK, p.cols / 2, l.dtype);
   if (rc != TKV_OK) return rc;
-  m[2] = m[3] = m[0];
+  m[2] = m[3] = m[4] = m[5] = m[0];
   return l.dtype == TKV_BF16 ? vt_launch<kVtStats, __nv_bfloat16>(m, p, st) : vt_launch<kVtStats, __half>(m, p, st);
 }
 
 int vloss_tc_backward(Vloss& l, void* ws, bool want_dx, cudaStream_t st) {
   char* xc = reinterpret_cast<char*>(vt_align(ws));
-  const int64_t rows = vt_rows(l.tokens), piece = vt_piece(l.tokens, l.vocab);
+  const int64_t rows = vt_rows(l.tokens), piece = vl_piece(l.tokens, l.vocab);
   l.dl = xc + vt_pad(rows * l.width * 2);
   l.piece = piece;
   l.acc = reinterpret_cast<float*>(reinterpret_cast<char*>(l.dl) + vt_pad(rows * piece * 2));
-  l.slots = vt_slots(l.tokens, l.width, piece);
-  CUtensorMap a[4], g[4];
+  CUtensorMap a[6], g[6];
+  const int box = vt_a_box(l.tokens);
   int rc = vt_gather(l, xc, st);
-  if (rc == TKV_OK) rc = make_map_2d(&a[0], xc, l.width, rows, kVtK, 128, l.dtype);
-  if (rc == TKV_OK) rc = make_map_2d(&a[1], l.w, l.width, l.vocab, kVtK, 128, l.dtype);
-  if (rc == TKV_OK) rc = make_map_2d(&g[0], l.dl, piece, rows, kVtK, 128, l.dtype);
-  if (rc == TKV_OK) rc = make_map_2d(&g[1], l.w, l.width, l.vocab, 64, kVtK, l.dtype);
-  if (rc == TKV_OK) rc = make_map_2d(&g[2], l.dl, piece, rows, 64, kVtK, l.dtype);
-  if (rc == TKV_OK) rc = make_map_2d(&g[3], xc, l.width, rows, 64, kVtK, l.dtype);
+  if (rc == TKV_OK) rc = make_map_wide(&a[0], xc, l.width, rows, kVtK, box, l.dtype);
+  if (rc == TKV_OK) rc = make_map_wide(&a[1], l.w, l.width, l.vocab, kVtK, 128, l.dtype);
+  if (rc == TKV_OK) rc = make_map_wide(&g[0], l.dl, piece, rows, kVtK, box, l.dtype);
+  if (rc == TKV_OK) rc = make_map_wide(&g[1], l.w, l.width, l.vocab, 64, kVtK, l.dtype);
+  if (rc == TKV_OK) rc = make_map_wide(&g[2], l.dl, piece, rows, 64, kVtK, l.dtype);
+  if (rc == TKV_OK) rc = make_map_wide(&g[3], xc, l.width, rows, 64, kVtK, l.dtype);
+  if (rc == TKV_OK) rc = make_map_wide(&a[4], l.dl, piece, rows, 64, 32, l.dtype);
+  if (rc == TKV_OK && want_dx) rc = make_map_wide(&g[4], l.acc, l.width, (int64_t)vt_slots(l.tokens, l.width) * rows, 32, 32, TKV_F32);
+  if (rc == TKV_OK && l.dw) rc = make_map_wide(&g[5], l.dw, l.width, l.vocab, 64, 32, l.dtype);
   if (rc != TKV_OK) return rc;
-  a[2] = a[3] = a[0];
+  a[2] = a[3] = a[5] = a[0];
+  if (!want_dx) g[4] = g[0];
+  if (l.dw == nullptr) g[5] = g[0];
   VtParams p = {};
-  p.cols = kVtCols; p.piece_pitch = piece; p.want_dx = want_dx; p.want_dw = l.dw != nullptr; p.l = l;
-  p.split_steps = (int)((piece / kVtK + l.slots - 1) / l.slots);
+  p.cols = kVtCols; p.a_box = box; p.a_ranks = l.tokens > 128 ? 2 : 1; p.want_dx = want_dx; p.want_dw = l.dw != nullptr; p.l = l;
+  p.piece_steps = piece / kVtK;
   for (int64_t v0 = 0; v0 < l.vocab && rc == TKV_OK; v0 += piece) {
     p.v0 = v0; p.piece_cols = l.vocab - v0 < piece ? l.vocab - v0 : piece; p.more = v0 > 0;
     if (l.dtype == TKV_BF16) {

@@ -57,12 +57,12 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: tor
         raise TypeError(f"labels of {labels.dtype}: want int32 or int64")
     if not hidden.device == weight.device == labels.device:
         raise ValueError(f"hidden rows on {hidden.device}, weight on {weight.device}, labels on {labels.device}")
-    x = hidden.reshape(-1, hidden.shape[-1])
+    x = hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])
     if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
         x = x.contiguous()
     loss = _LinearCrossEntropy.apply(x, weight.contiguous(), labels.reshape(-1).to(torch.int64).contiguous(), int(ignore_index),
                                      ops.VLOSS_REDUCTIONS[reduction], status)
-    return loss.view(labels.shape) if reduction == "none" else loss
+    return loss.view(labels.shape) if reduction == "none" and labels.dim() != 1 else loss
 
 
 class _ExpertBalance(torch.autograd.Function):
@@ -93,10 +93,14 @@ def expert_balance(logits: torch.Tensor, choice: torch.Tensor, valid: Optional[t
         raise TypeError(f"choices of {choice.dtype}: want int32 or int64")
     if choice.device != logits.device or (valid is not None and valid.device != logits.device):
         raise ValueError(f"logits on {logits.device}, choice on {choice.device}, valid on {None if valid is None else valid.device}")
-    z, c = logits.reshape(-1, logits.shape[-1]), choice.reshape(-1, choice.shape[-1])
-    z = z if z.stride(1) == 1 else z.contiguous()
-    c = c if c.stride(1) == 1 else c.contiguous()
-    return _ExpertBalance.apply(z, c, None if valid is None else valid.reshape(-1))
+    if logits.dim() != 2:                          # a reshape of two dimensions would only add a node to the graph
+        logits, choice = logits.reshape(-1, logits.shape[-1]), choice.reshape(-1, choice.shape[-1])
+        valid = None if valid is None else valid.reshape(-1)
+    if logits.stride(1) != 1:
+        logits = logits.contiguous()
+    if choice.stride(1) != 1:
+        choice = choice.contiguous()
+    return _ExpertBalance.apply(logits, choice, valid)
 
 
 __all__ = ["expert_balance", "linear_cross_entropy"]
