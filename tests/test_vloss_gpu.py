@@ -77,6 +77,11 @@ def _check(x, w, y, reduction="none", grad=None):
         lost = 2.0 ** -38 * float(each.abs().max())
         tol_x = tol_x + lost * w.detach().double().abs().sum(0)
         tol_w = tol_w + lost * x.detach().double()[y >= 0].abs().sum(0)
+    # A weight exp(s - lse) below 2^-126, the smallest normal fp32 number, may be taken as 0 (and the smaller parts that an fp32 number of
+    # that size is made of): dL is then off by at most 2 * 2^-126 of the row's gradient, a gradient by that times the sum of |w| or |x|.
+    under = 2.0 ** -125 * each.double().abs() * (y >= 0)
+    tol_x = tol_x + under[:, None] * w.detach().double().abs().sum(0)
+    tol_w = tol_w + (under[:, None] * x.detach().double().abs()).sum(0)
     assert dx.dtype == x.dtype and dw.dtype == w.dtype
     assert _within(dx, ex, tol_x) and _within(dw, ew, tol_w)
     assert not bool(dx[y < 0].any())

@@ -454,7 +454,7 @@ extern "C" int64_t tkv_vloss_workspace_bytes(int64_t tokens, int64_t vocab, int 
   const int t = (int)tokens;
   int64_t n = backward ? any_backward_bytes(t, vocab, width, want_dx != 0) : any_forward_bytes(t, vocab);
   if (vloss_tc_shape(t, vocab, width, dtype)) {            // which form runs is known with the addresses: room for either
-    const int64_t tc = backward ? vloss_tc_backward_bytes(t, vocab, width, want_dx != 0) : vloss_tc_forward_bytes(t, vocab, width);
+    const int64_t tc = vloss_tc_bytes(t, vocab, width, dtype, backward != 0, want_dx != 0);
     n = n > tc ? n : tc;
   }
   return 512 + pad256((int64_t)t * 4) + n;
@@ -517,7 +517,7 @@ extern "C" int tkv_vloss_backward(const void* x, int64_t x_stride, const void* w
   const bool tc = use_tc(p);
   const int64_t piece = any_piece(p.tokens, vocab);
   const int room = any_slots(p.tokens, width);
-  const VlossWork work = tc ? vloss_tc_work(p.tokens, vocab, width, dx != nullptr, dw != nullptr)
+  const VlossWork work = tc ? vloss_tc_work(p.tokens, vocab, width, dtype, dx != nullptr, dw != nullptr)
                             : VlossWork{2 * 148, kVgTile, 1, (width + kVgTile - 1) / kVgTile, 0, (int)((piece + kVgK - 1) / kVgK), kVgK, room, p.tokens, dx != nullptr, false};
   int rc = vl_launch("tkv_vloss_backward", vloss_rows_grad_kernel, dim3(1), kSumThreads, st, grad, grad_stride, reduction, p.plan, work, g, scale,
                      reinterpret_cast<int*>(scale) + 2);

@@ -54,11 +54,10 @@ struct VlossWork { int workers, rows, acc_rows, ht, vt, steps, step, room, token
 
 int vloss_plan_rows(const Vloss& p, const int64_t* labels, int64_t ignore, float* loss, cudaStream_t st);
 
-// The form on the tensor cores (tkv_vloss_tc.cu): 16-bit types, widths of whole 16-byte vectors, w and dw on 16 bytes; x of any alignment.
+// The form on the tensor cores (tkv_vloss_tc.cu): widths of multiples of 8, w and dw on 16 bytes; x of any alignment.
 bool vloss_tc_shape(int tokens, int64_t vocab, int width, int dtype);
-int64_t vloss_tc_forward_bytes(int tokens, int64_t vocab, int width);
-int64_t vloss_tc_backward_bytes(int tokens, int64_t vocab, int width, bool dx);
-VlossWork vloss_tc_work(int tokens, int64_t vocab, int width, bool want_dx, bool want_dw);
+int64_t vloss_tc_bytes(int tokens, int64_t vocab, int width, int dtype, bool backward, bool dx);
+VlossWork vloss_tc_work(int tokens, int64_t vocab, int width, int dtype, bool want_dx, bool want_dw);
 int vloss_tc_forward(Vloss& p, const int64_t* labels, int64_t ignore, float* loss, void* ws, cudaStream_t st);   // the plan, part and mine; sets tiles
 int vloss_tc_backward(Vloss& p, void* ws, bool want_dx, cudaStream_t st);                                        // dw and acc
 

@@ -1,4 +1,4 @@
-// Cross entropy against a vocabulary (tkv_vloss.cuh) on tcgen05 + TMEM, for 16-bit types:
+// Cross entropy against a vocabulary (tkv_vloss.cuh) on tcgen05 + TMEM:
 //   kVtStats  : logits of 256 tokens x up to 256 words -> largest logit and sum of weights of every token, logit of its label;
 //   kVtLogits : the same logits again -> a tile of dL in the type of the operands;
 //   kVtGrads  : dx shares (dL w, both read along the vocabulary) and dw (dL^T x, both read along the tokens) of a piece, one launch.
@@ -10,6 +10,9 @@
 // tile of w comes from HBM once per group.
 // What is stored along the inner axis (x, w in the logits; dL for dx) is read K-major, what is stored across it MN-major: nothing is
 // transposed in memory.
+// fp32 operands are three bf16 numbers each (x = a + b + c, each the rounding of what the ones before leave: 24 bits together), stored as
+// three matrices one below the other, and a product is the six products of parts down to 2^-16 of the first, the smallest ones first; what
+// is left out is below 2^-24 of a product.  w is taken apart a piece of the vocabulary at a time, so that its parts stay in L2.
 //
 // Copies of both CTAs complete on the even CTA's barriers; it issues the products; their completion is told to both.  Every wait is
 // bounded; a CTA whose wait runs out records TKV_DEV_TIMEOUT, in the plan too (losses and dx become NaN), and tells its neighbour; both
@@ -41,10 +44,17 @@ struct VtParams {
   Vloss l;
   int cols;                                                // of a tile (a multiple of 16)
   int a_box, a_ranks;                                      // rows of x or dL that a CTA fetches, CTAs of a pair that have any (few tokens)
-  int64_t v0, piece_cols;                                  // the vocabulary from v0 (kVtStats: all of it)
+  int64_t v0, piece_cols;                                  // the vocabulary from v0
+  int tile0;                                               // kVtStats: tiles of the pieces before
+  int parts, rows, w_rows, w0;                             // of an operand (1 or 3), rows of a part of x and dL, and of w; the piece's first row there
   int want_dx, want_dw, more;                              // kVtGrads
   int64_t piece_steps;                                     // stages of a whole piece
 };
+
+// The parts that product c takes of A and of B; with one part there is product 5 alone.
+constexpr int kVtProducts = 6;
+__device__ __forceinline__ int vt_part_a(int c) { return (0x052 >> (2 * c)) & 3; }   // 2 0 1 1 0 0
+__device__ __forceinline__ int vt_part_b(int c) { return (0x118 >> (2 * c)) & 3; }   // 0 2 1 0 1 0
 
 // ---- instructions for pairs of CTAs
 __device__ __forceinline__ uint32_t vt_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
@@ -164,6 +174,12 @@ vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm->tmem_base)), "r"(512));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
   }
+  if (kMode != kVtGrads || p.want_dx) {                    // rows of A that no copy fills: zeros cost the products least power (1 token: 139 us, and VL_ZERO)
+    const int kept = rank < p.a_ranks ? p.a_box * 128 : 0;
+    for (int i = kept + tid * 16; i < kVtABytes; i += kVtThreads * 16)
+      for (int st = 0; st < kVtStages; ++st) st16(base + st * kVtStage + i, make_uint4(0, 0, 0, 0));
+    fence_async_smem();
+  }
   grid_dependency_wait();
   grid_launch_dependents();
   tc_fence_before();
@@ -191,26 +207,28 @@ vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       const int box = a_mn ? 128 : p.a_box, ranks = a_mn ? 2 : p.a_ranks;
       const uint32_t bytes = (ranks * box + 2 * half) * kVtK * 2;        // of both CTAs
       const int arow = t.row0 + rank * 128, brow = t.col0 + rank * half;
+      for (int c = p.parts == 1 ? kVtProducts - 1 : 0; ok && c < kVtProducts; ++c)
       for (int k = t.step0; k < t.step0 + t.steps; ++k, ++it) {
         const int s = it % kVtStages;
+        const int a_at = vt_part_a(c) * p.rows, x_at = vt_part_b(c) * p.rows, w_at = p.w0 + vt_part_b(c) * p.w_rows;
         ok = warp_wait(&sm->empty[s], ((it / kVtStages) & 1) ^ 1, abort_flag);
         if (!ok) break;
         if (elect_one()) {
           const uint32_t bar = vt_of_rank(smem_u32(&sm->full[s]), 0), a = smem_u32(base + s * kVtStage), b = a + kVtABytes;
           if (rank == 0) mbar_expect_tx(&sm->full[s], bytes);
           if (a_mn) {
-            vt_load(a, &map_a2, bar, arow, k * kVtK);
-            vt_load(a + kVtABytes / 2, &map_a2, bar, arow + 64, k * kVtK);
+            vt_load(a, &map_a2, bar, arow, a_at + k * kVtK);
+            vt_load(a + kVtABytes / 2, &map_a2, bar, arow + 64, a_at + k * kVtK);
           } else if (rank < ranks) {                       // rows beyond the box hold what was there: rows of D that nobody reads
-            vt_load(a, &map_a, bar, k * kVtK, arow);
+            vt_load(a, &map_a, bar, k * kVtK, a_at + arow);
           }
           if (b_mn) {
             const CUtensorMap* mb = t.dx ? &map_b : &map_b2;
-            const int y = k * kVtK + (t.dx ? (int)p.v0 : 0);
+            const int y = k * kVtK + (t.dx ? w_at : x_at);
             vt_load(b, mb, bar, brow, y);
             vt_load(b + kVtBBytes / 2, mb, bar, brow + 64, y);
           } else {
-            vt_load(b, &map_b, bar, k * kVtK, (int)p.v0 + brow);
+            vt_load(b, &map_b, bar, k * kVtK, w_at + brow);
           }
         }
         __syncwarp();
@@ -233,7 +251,8 @@ vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         const int buf = acc & 1;
         ok = warp_wait(&sm->acc_empty[buf], ((acc >> 1) & 1) ^ 1, abort_flag);
         tc_fence_after();
-        for (int k = 0; k < t.steps && ok; ++k, ++it) {
+        const int steps = t.steps * (p.parts == 1 ? 1 : kVtProducts);
+        for (int k = 0; k < steps && ok; ++k, ++it) {
           const int s = it % kVtStages;
           ok = warp_wait(&sm->full[s], (it / kVtStages) & 1, abort_flag);
           if (!ok) break;
@@ -245,7 +264,7 @@ vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 #pragma unroll
             for (int q = 0; q < 4; ++q) vt_mma(tm + buf * kVtCols, a + q * da, b + q * db, idesc, (k > 0 || q > 0));
             vt_commit(&sm->empty[s]);
-            if (k == t.steps - 1) vt_commit(&sm->acc_full[buf]);
+            if (k == steps - 1) vt_commit(&sm->acc_full[buf]);
           }
           __syncwarp();
         }
@@ -288,7 +307,7 @@ vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         const bool live = row < tiles.n;
         const int left = (int)min((int64_t)p.cols, p.piece_cols - t.col0);        // columns that exist
         if (t.row0 + rank * 128 + quarter * 32 < tiles.n) {
-          const int label = live ? p.l.plan.label[row] - t.col0 : -1;
+          const int label = live ? (int)(p.l.plan.label[row] - p.v0 - t.col0) : -1;
           float top = -INFINITY, sum = 0.f;
           for (int c = 0; c < left; c += 32) {
             float v[32];
@@ -314,7 +333,7 @@ vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             sum = fmaf(sum, exp2_weight((top - from0) * kLog2e), part);
             top = next;
           }
-          if (live) p.l.part[(int64_t)row * p.l.tiles + t.col0 / p.cols] = make_float2(top, sum);
+          if (live) p.l.part[(int64_t)row * p.l.tiles + p.tile0 + t.col0 / p.cols] = make_float2(top, sum);
         }
       } else if constexpr (kMode == kVtLogits) {
         const bool live = row < tiles.n;
@@ -325,39 +344,50 @@ vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         const int first = t.row0 + rank * 128 + quarter * 32;
         // the products to come read whole steps of rows
         for (int c = first < (tiles.n + kVtK - 1) / kVtK * kVtK ? 0 : p.cols; c < p.cols; c += 64) {
-          uint32_t w[32];
+          float v[64];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            float v[32];
-            tmem_ld32(from + c + 32 * h, v);
             const int at = c + 32 * h;
+            tmem_ld32(from + at, v + 32 * h);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {                 // rows and columns that do not exist are zeros for the products to come
-              const float d = exp2_weight(fmaf(v[i] - lse.x, kLog2e, -lse.y)) - (i == label - at ? 1.f : 0.f);
-              v[i] = live && at + i < left ? g * d : 0.f;
+            for (int i = 32 * h; i < 32 * h + 32; ++i) {   // rows and columns that do not exist are zeros for the products to come
+              const float d = exp2_weight(fmaf(v[i] - lse.x, kLog2e, -lse.y)) - (i == label - c ? 1.f : 0.f);
+              v[i] = live && c + i < left ? g * d : 0.f;
             }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) w[16 * h + i] = vt_pack<T>(v[2 * i], v[2 * i + 1]);
           }
-          put(w);
-          if (lane == 0) tma_store_2d(&map_c, box_of(), t.col0 + c, first);
-          ++outs;
+          for (int part = 0; part < (sizeof(T) == 4 ? 3 : 1); ++part) {
+            uint32_t w[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              w[i] = vt_pack<T>(v[2 * i], v[2 * i + 1]);
+              if (sizeof(T) == 4) { v[2 * i] -= __uint_as_float(w[i] << 16); v[2 * i + 1] -= __uint_as_float(w[i] & 0xffff0000u); }
+            }
+            put(w);
+            if (lane == 0) tma_store_2d(&map_c, box_of(), t.col0 + c, part * p.rows + first);
+            ++outs;
+          }
         }
       } else {
         const int left = p.l.width - t.col0, first = t.row0 + rank * 128 + quarter * 32;
         const float back = t.dx ? 0.f : p.l.g_scale[1];
-        if (t.dx) {                                        // a share's rows are whole tiles
-          for (int c = 0; first < tiles.n && c < kVtCols && c < left; c += 32) {
+        if (t.dx || sizeof(T) == 4) {                      // a share's rows are whole tiles
+          const bool any = t.dx ? first < tiles.n : first < p.piece_cols;
+          for (int c = 0; any && c < kVtCols && c < left; c += 32) {
             float v[32];
             if (t.steps > 0) tmem_ld32(from + c, v);
             else {
 #pragma unroll
               for (int i = 0; i < 32; ++i) v[i] = 0.f;
             }
+            if (sizeof(T) == 4 && !t.dx) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] *= back;
+            }
             put(reinterpret_cast<const uint32_t*>(v));
             if (lane == 0) {
               const int y = t.slot * tiles.mt * kVtRows + first;
-              if (p.more) tma_add_2d(&map_c, box_of(), t.col0 + c, y);
+              if (sizeof(T) == 4 && !t.dx) tma_store_2d(&map_d, box_of(), t.col0 + c, (int)p.v0 + first);
+              else if (p.more) tma_add_2d(&map_c, box_of(), t.col0 + c, y);
               else tma_store_2d(&map_c, box_of(), t.col0 + c, y);
             }
             ++outs;
@@ -403,23 +433,56 @@ vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 // -------------------------------------------------------------------------------------------------- rows that count, together
 constexpr int kVtGatherThreads = 256;
 
-// Row i of xc is the row of the i-th token that counts; zeros up to the end of the last tile of rows.
-template <bool kVec> __global__ void __launch_bounds__(kVtGatherThreads) vloss_gather_kernel(const uint16_t* x, int64_t x_stride, VlossPlan plan, int width, uint16_t* xc) {
+// Eight elements as they are stored for the products: themselves, or (fp32) their three parts.
+template <typename T, bool kVec> __device__ __forceinline__ void vt_take(const T* in, uint16_t* out, int64_t part) {
+  if constexpr (sizeof(T) == 2) {
+    if (kVec) st16(out, ld16_stream(in));
+    else
+      for (int e = 0; e < 8; ++e) out[e] = in[e];
+  } else {
+    float v[8];
+    if (kVec) load_vec<8>(in, v);
+    else
+      for (int e = 0; e < 8; ++e) v[e] = in[e];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[i] = vt_pack<float>(v[2 * i], v[2 * i + 1]);
+        v[2 * i] -= __uint_as_float(w[i] << 16);
+        v[2 * i + 1] -= __uint_as_float(w[i] & 0xffff0000u);
+      }
+      st16(out + k * part, make_uint4(w[0], w[1], w[2], w[3]));
+    }
+  }
+}
+template <typename T> __device__ __forceinline__ void vt_zero(uint16_t* out, int64_t part) {
+  for (int k = 0; k < (sizeof(T) == 4 ? 3 : 1); ++k) st16(out + k * part, make_uint4(0, 0, 0, 0));
+}
+
+// Row i of xc is the row of the i-th token that counts; zeros up to the end of the last tile of rows.  T: uint16_t or float.
+template <typename T, bool kVec> __global__ void __launch_bounds__(kVtGatherThreads) vloss_gather_kernel(const T* x, int64_t x_stride, VlossPlan plan, int width, uint16_t* xc, int64_t part) {
   grid_dependency_wait();
   grid_launch_dependents();
   const int n = plan.head[0];
   const int64_t i = blockIdx.x;
   if (i >= ((int64_t)n + kVtRows - 1) / kVtRows * kVtRows) return;
   uint16_t* out = xc + i * width;
-  if (i >= n) {
-    for (int c = threadIdx.x * 8; c < width; c += kVtGatherThreads * 8) st16(out + c, make_uint4(0, 0, 0, 0));
-    return;
+  const T* in = x + (i < n ? (int64_t)plan.rows[i] : 0) * x_stride;
+  for (int c = threadIdx.x * 8; c < width; c += kVtGatherThreads * 8) {
+    if (i < n) vt_take<T, kVec>(in + c, out + c, part);
+    else vt_zero<T>(out + c, part);
   }
-  const uint16_t* in = x + (int64_t)plan.rows[i] * x_stride;
-  if (kVec) {
-    for (int c = threadIdx.x * 8; c < width; c += kVtGatherThreads * 8) st16(out + c, ld16_stream(in + c));
-  } else {
-    for (int c = threadIdx.x; c < width; c += kVtGatherThreads) out[c] = in[c];
+}
+
+// The three parts of a piece of w (fp32), zeros behind its last row up to a whole step.
+__global__ void __launch_bounds__(kVtGatherThreads) vloss_parts_kernel(const float* w, int64_t n, int64_t whole, uint16_t* out, int64_t part) {
+  grid_dependency_wait();
+  grid_launch_dependents();
+  for (int64_t i = ((int64_t)blockIdx.x * kVtGatherThreads + threadIdx.x) * 8; i < whole; i += (int64_t)gridDim.x * kVtGatherThreads * 8) {
+    if (i < n) vt_take<float, true>(w + i, out + i, part);
+    else vt_zero<float>(out + i, part);
   }
 }
 
@@ -427,8 +490,9 @@ constexpr int kVtFirst = 1024;                             // most tokens for wh
 
 // vloss_plan_kernel and vloss_gather_kernel in one launch, for few tokens: every CTA finds its row among the labels.  The grid is the rows
 // that the logits' boxes reach.
-template <bool kVec> __global__ void __launch_bounds__(kVtGatherThreads) vloss_first_kernel(const int64_t* labels, int64_t ignore, int tokens, int64_t vocab, VlossPlan plan,
-                                                                                        float* loss, int32_t* status, const uint16_t* x, int64_t x_stride, int width, uint16_t* xc) {
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(kVtGatherThreads) vloss_first_kernel(const int64_t* labels, int64_t ignore, int tokens, int64_t vocab, VlossPlan plan, float* loss,
+                                                                     int32_t* status, const T* x, int64_t x_stride, int width, uint16_t* xc, int64_t part) {
   constexpr int kPer = kVtFirst / kVtGatherThreads;
   __shared__ int sums[kVtGatherThreads / 32 + 1], token, bad_any;
   grid_dependency_wait();
@@ -466,17 +530,16 @@ template <bool kVec> __global__ void __launch_bounds__(kVtGatherThreads) vloss_f
   if ((int)blockIdx.x >= (total + kVtRows - 1) / kVtRows * kVtRows) return;
   uint16_t* out = xc + (int64_t)blockIdx.x * width;
   const bool live = (int)blockIdx.x < total;
-  const uint16_t* in = x + (live ? token : 0) * x_stride;
+  const T* in = x + (live ? token : 0) * x_stride;
   for (int c = threadIdx.x * 8; c < width; c += kVtGatherThreads * 8) {
-    if (!live) st16(out + c, make_uint4(0, 0, 0, 0));
-    else if (kVec) st16(out + c, ld16_stream(in + c));
-    else
-      for (int e = 0; e < 8; ++e) out[c + e] = in[c + e];
+    if (live) vt_take<T, kVec>(in + c, out + c, part);
+    else vt_zero<T>(out + c, part);
   }
 }
 
 // ------------------------------------------------------------------------------------------------------------------ the host
-bool vloss_tc_shape(int tokens, int64_t vocab, int width, int dtype) { return (dtype == TKV_BF16 || dtype == TKV_F16) && width % 8 == 0 && tokens > 0; }
+bool vloss_tc_shape(int tokens, int64_t vocab, int width, int dtype) { return elem_size(dtype) != 0 && width % 8 == 0 && tokens > 0; }
+static int vt_parts(int dtype) { return dtype == TKV_F32 ? 3 : 1; }
 
 static int64_t vt_rows(int tokens) { return vl_round(tokens, kVtRows); }
 // Columns of a tile: what a pair does in its rounds is rounds x columns, and a little per round; few rounds make it matter that the last
@@ -493,10 +556,18 @@ static int vt_tile_cols(int tokens, int64_t vocab) {
   return best;
 }
 static int vt_a_box(int tokens) { return tokens >= 128 ? 128 : (int)vl_round(tokens, 8); }
-// The vocabulary in equal pieces, of at most 256 MB of dL where that is not fewer than 8192 words.
-static int64_t vl_piece(int tokens, int64_t vocab) {
-  int64_t n = ((int64_t)256 << 20) / (2 * vt_rows(tokens)) / kVtCols * kVtCols;
-  if (n < 8192) n = 8192;
+// The vocabulary in equal pieces: of at most 256 MB of dL where that is not fewer than 8192 words; fp32: of at most 96 MB of parts of w too,
+// and not fewer than 2048 words.
+static int64_t vt_piece(int tokens, int64_t vocab, int width, int dtype) {
+  int64_t n = ((int64_t)256 << 20) / (2 * vt_parts(dtype) * vt_rows(tokens));
+  int64_t least = 8192;
+  if (dtype == TKV_F32) {
+    const int64_t w = ((int64_t)96 << 20) / (6 * (int64_t)width);
+    if (n > w) n = w;
+    least = 2048;
+  }
+  n = n / kVtCols * kVtCols;
+  if (n < least) n = least;
   const int64_t pieces = (vocab + n - 1) / n;
   return vl_round((vocab + pieces - 1) / pieces, kVtCols);
 }
@@ -507,28 +578,54 @@ static int vt_slots(int tokens, int width) {
   const int64_t s = (8 * kVtPairs + tiles - 1) / tiles;
   return (int)(s > kVlMaxSlots ? kVlMaxSlots : s < 1 ? 1 : s);
 }
-VlossWork vloss_tc_work(int tokens, int64_t vocab, int width, bool want_dx, bool want_dw) {
-  const int64_t piece = vl_piece(tokens, vocab);
+VlossWork vloss_tc_work(int tokens, int64_t vocab, int width, int dtype, bool want_dx, bool want_dw) {
+  const int64_t piece = vt_piece(tokens, vocab, width, dtype);
   return {kVtPairs, kVtRows, kVtRows, (width + kVtCols - 1) / kVtCols, (int)((piece + kVtRows - 1) / kVtRows), (int)(piece / kVtK), kVtK, vt_slots(tokens, width), (int)vt_rows(tokens),
           want_dx, want_dw};
 }
-static int64_t vt_pad(int64_t bytes) { return vl_round(bytes, 1024); }
 
-int64_t vloss_tc_forward_bytes(int tokens, int64_t vocab, int width) {
-  const int cols = vt_tile_cols(tokens, vocab);
-  return 1024 + vt_pad(vt_rows(tokens) * width * 2) + (int64_t)tokens * ((vocab + cols - 1) / cols) * 8;
-}
-int64_t vloss_tc_backward_bytes(int tokens, int64_t vocab, int width, bool dx) {
-  const int64_t piece = vl_piece(tokens, vocab);
-  return 1024 + vt_pad(vt_rows(tokens) * width * 2) + vt_pad(vt_rows(tokens) * piece * 2) + (dx ? (int64_t)vt_slots(tokens, width) * vt_rows(tokens) * width * 4 : 0);
-}
+// What lies where in a workspace.
+struct VtRoom {
+  int64_t rows, piece, xc, w, dl, acc, part, bytes;        // bytes from the start
+  int cols, tiles;
+  VtRoom(int tokens, int64_t vocab, int width, int dtype, bool backward, bool dx) {
+    const int64_t parts = vt_parts(dtype);
+    auto pad = [](int64_t n) { return vl_round(n, 1024); };
+    rows = vt_rows(tokens);
+    piece = backward || parts == 3 ? vt_piece(tokens, vocab, width, dtype) : vocab;
+    cols = backward ? kVtCols : vt_tile_cols(tokens, piece);
+    const int64_t before = (vocab - 1) / piece;              // whole pieces before the last
+    tiles = (int)(before * ((piece + cols - 1) / cols) + (vocab - before * piece + cols - 1) / cols);
+    xc = 0;
+    w = xc + pad(parts * rows * width * 2);
+    dl = w + (parts == 3 ? pad(3 * piece * width * 2) : 0);
+    acc = dl + (backward ? pad(parts * rows * piece * 2) : 0);
+    part = acc + (backward && dx ? pad((int64_t)vt_slots(tokens, width) * rows * width * 4) : 0);
+    bytes = part + (backward ? 0 : pad((int64_t)tokens * tiles * 8));
+  }
+};
+int64_t vloss_tc_bytes(int tokens, int64_t vocab, int width, int dtype, bool backward, bool dx) { return 1024 + VtRoom(tokens, vocab, width, dtype, backward, dx).bytes; }
 
-static int vt_gather(const Vloss& p, void* xc, cudaStream_t st) {
-  const bool vec = aligned16(p.x) && p.x_stride % 8 == 0;
-  cudaError_t e = launch_pdl(vec ? vloss_gather_kernel<true> : vloss_gather_kernel<false>, dim3((unsigned)vt_rows(p.tokens)), dim3(kVtGatherThreads), 0, st,
-                             reinterpret_cast<const uint16_t*>(p.x), p.x_stride, p.plan, p.width, reinterpret_cast<uint16_t*>(xc));
-  if (e != cudaSuccess) return fail(TKV_ERR_LAUNCH, "tkv_vloss: %s", cudaGetErrorString(e));
-  return check_launch("tkv_vloss");
+static int vt_check(cudaError_t e) { return e == cudaSuccess ? check_launch("tkv_vloss") : fail(TKV_ERR_LAUNCH, "tkv_vloss: %s", cudaGetErrorString(e)); }
+
+template <typename T> static int vt_gather(const Vloss& p, void* xc, cudaStream_t st) {
+  const bool vec = aligned16(p.x) && p.x_stride % (16 / (int64_t)sizeof(T)) == 0;
+  return vt_check(launch_pdl(vec ? vloss_gather_kernel<T, true> : vloss_gather_kernel<T, false>, dim3((unsigned)vt_rows(p.tokens)), dim3(kVtGatherThreads), 0, st,
+                             reinterpret_cast<const T*>(p.x), p.x_stride, p.plan, p.width, reinterpret_cast<uint16_t*>(xc), vt_rows(p.tokens) * p.width));
+}
+template <typename T> static int vt_first(const Vloss& p, const int64_t* labels, int64_t ignore, float* loss, void* xc, cudaStream_t st) {
+  const bool vec = aligned16(p.x) && p.x_stride % (16 / (int64_t)sizeof(T)) == 0;
+  return vt_check(launch_pdl(vec ? vloss_first_kernel<T, true> : vloss_first_kernel<T, false>, dim3((unsigned)(p.tokens > 128 ? vt_rows(p.tokens) : vt_a_box(p.tokens))),
+                             dim3(kVtGatherThreads), 0, st, labels, ignore, p.tokens, p.vocab, p.plan, loss, p.status, reinterpret_cast<const T*>(p.x), p.x_stride, p.width,
+                             reinterpret_cast<uint16_t*>(xc), vt_rows(p.tokens) * p.width));
+}
+// fp32: the parts of the piece of w at v0.
+static int vt_parts_of(const VtParams& p, const VtRoom& room, void* w, cudaStream_t st) {
+  if (p.parts == 1) return TKV_OK;
+  const int64_t whole = vl_round(p.piece_cols, kVtK) * p.l.width;
+  const int64_t blocks = (whole + kVtGatherThreads * 8 - 1) / (kVtGatherThreads * 8);
+  return vt_check(launch_pdl(vloss_parts_kernel, dim3((unsigned)(blocks < 148 * 16 ? blocks : 148 * 16)), dim3(kVtGatherThreads), 0, st,
+                             reinterpret_cast<const float*>(p.l.w) + p.v0 * p.l.width, p.piece_cols * p.l.width, whole, reinterpret_cast<uint16_t*>(w), room.piece * p.l.width));
 }
 
 template <int kMode, typename T> static int vt_launch(const CUtensorMap* m, const VtParams& p, cudaStream_t st) {
@@ -540,71 +637,95 @@ template <int kMode, typename T> static int vt_launch(const CUtensorMap* m, cons
     if (e == cudaSuccess && dev >= 0 && dev < 64) allowed[dev] = true;
   }
   if (e == cudaSuccess) e = launch_pdl(vloss_tc_kernel<kMode, T>, dim3(2 * kVtPairs), dim3(kVtThreads), (size_t)kVtSmemBytes, st, m[0], m[1], m[2], m[3], m[4], m[5], p);
-  if (e != cudaSuccess) return fail(TKV_ERR_LAUNCH, "tkv_vloss: %s", cudaGetErrorString(e));
-  return check_launch("tkv_vloss");
+  return vt_check(e);
+}
+template <int kMode> static int vt_launch(const CUtensorMap* m, const VtParams& p, cudaStream_t st) {
+  return p.l.dtype == TKV_BF16 ? vt_launch<kMode, __nv_bfloat16>(m, p, st) : p.l.dtype == TKV_F16 ? vt_launch<kMode, __half>(m, p, st) : vt_launch<kMode, float>(m, p, st);
 }
 
-static void* vt_align(void* p) { return reinterpret_cast<void*>(((uintptr_t)p + 1023) & ~(uintptr_t)1023); }
+static char* vt_align(void* p) { return reinterpret_cast<char*>(((uintptr_t)p + 1023) & ~(uintptr_t)1023); }
+
+static VtParams vt_params(const Vloss& l, const VtRoom& room) {
+  VtParams p = {};
+  p.l = l;
+  p.cols = room.cols;
+  p.a_box = vt_a_box(l.tokens);
+  p.a_ranks = l.tokens > 128 ? 2 : 1;
+  p.parts = vt_parts(l.dtype);
+  p.rows = (int)room.rows;
+  p.w_rows = (int)room.piece;
+  return p;
+}
+static void vt_piece_at(VtParams* p, const VtRoom& room, int64_t v0) {
+  p->v0 = v0;
+  p->piece_cols = p->l.vocab - v0 < room.piece ? p->l.vocab - v0 : room.piece;
+  p->w0 = p->parts == 1 ? (int)v0 : 0;
+  p->tile0 = (int)(v0 / room.piece * ((room.piece + room.cols - 1) / room.cols));
+  p->more = v0 > 0;
+}
 
 int vloss_tc_forward(Vloss& l, const int64_t* labels, int64_t ignore, float* loss, void* ws, cudaStream_t st) {
-  void* xc = vt_align(ws);
+  const VtRoom room(l.tokens, l.vocab, l.width, l.dtype, false, false);
+  char* base = vt_align(ws);
+  const bool f32 = l.dtype == TKV_F32;
   int rc;
   if (l.tokens <= kVtFirst) {
-    const bool vec = aligned16(l.x) && l.x_stride % 8 == 0;
-    cudaError_t e = launch_pdl(vec ? vloss_first_kernel<true> : vloss_first_kernel<false>, dim3((unsigned)(l.tokens > 128 ? vt_rows(l.tokens) : vt_a_box(l.tokens))), dim3(kVtGatherThreads), 0, st,
-                               labels, ignore, l.tokens, l.vocab, l.plan, loss, l.status, reinterpret_cast<const uint16_t*>(l.x), l.x_stride, l.width, reinterpret_cast<uint16_t*>(xc));
-    rc = e == cudaSuccess ? check_launch("tkv_vloss") : fail(TKV_ERR_LAUNCH, "tkv_vloss: %s", cudaGetErrorString(e));
+    rc = f32 ? vt_first<float>(l, labels, ignore, loss, base, st) : vt_first<uint16_t>(l, labels, ignore, loss, base, st);
   } else {
     rc = vloss_plan_rows(l, labels, ignore, loss, st);
-    if (rc == TKV_OK) rc = vt_gather(l, xc, st);
+    if (rc == TKV_OK) rc = f32 ? vt_gather<float>(l, base, st) : vt_gather<uint16_t>(l, base, st);
   }
-  VtParams p = {};
-  p.cols = vt_tile_cols(l.tokens, l.vocab);
-  l.part = reinterpret_cast<float2*>(reinterpret_cast<char*>(xc) + vt_pad(vt_rows(l.tokens) * l.width * 2));
-  l.tiles = (int)((l.vocab + p.cols - 1) / p.cols);
-  p.l = l; p.v0 = 0; p.piece_cols = l.vocab; p.a_box = vt_a_box(l.tokens); p.a_ranks = l.tokens > 128 ? 2 : 1;
+  l.part = reinterpret_cast<float2*>(base + room.part);
+  l.tiles = room.tiles;
+  VtParams p = vt_params(l, room);
+  const int type = f32 ? TKV_BF16 : l.dtype;
+  const void* w = f32 ? (const void*)(base + room.w) : l.w;
   CUtensorMap m[6];
-  if (rc == TKV_OK) rc = make_map_wide(&m[0], xc, l.width, vt_rows(l.tokens), kVtK, p.a_box, l.dtype);
-  if (rc == TKV_OK) rc = make_map_wide(&m[1], l.w, l.width, l.vocab, kVtK, p.cols / 2, l.dtype);
+  if (rc == TKV_OK) rc = make_map_wide(&m[0], base, l.width, p.parts * room.rows, kVtK, p.a_box, type);
+  if (rc == TKV_OK) rc = make_map_wide(&m[1], w, l.width, f32 ? 3 * room.piece : l.vocab, kVtK, p.cols / 2, type);
   if (rc != TKV_OK) return rc;
   m[2] = m[3] = m[4] = m[5] = m[0];
-  return l.dtype == TKV_BF16 ? vt_launch<kVtStats, __nv_bfloat16>(m, p, st) : vt_launch<kVtStats, __half>(m, p, st);
+  for (int64_t v0 = 0; v0 < l.vocab && rc == TKV_OK; v0 += room.piece) {
+    vt_piece_at(&p, room, v0);
+    rc = vt_parts_of(p, room, base + room.w, st);
+    if (rc == TKV_OK) rc = vt_launch<kVtStats>(m, p, st);
+  }
+  return rc;
 }
 
 int vloss_tc_backward(Vloss& l, void* ws, bool want_dx, cudaStream_t st) {
-  char* xc = reinterpret_cast<char*>(vt_align(ws));
-  const int64_t rows = vt_rows(l.tokens), piece = vl_piece(l.tokens, l.vocab);
-  l.dl = xc + vt_pad(rows * l.width * 2);
-  l.piece = piece;
-  l.acc = reinterpret_cast<float*>(reinterpret_cast<char*>(l.dl) + vt_pad(rows * piece * 2));
+  const VtRoom room(l.tokens, l.vocab, l.width, l.dtype, true, want_dx);
+  char* base = vt_align(ws);
+  const bool f32 = l.dtype == TKV_F32;
+  l.dl = base + room.dl;
+  l.acc = reinterpret_cast<float*>(base + room.acc);
+  VtParams p = vt_params(l, room);
+  p.want_dx = want_dx;
+  p.want_dw = l.dw != nullptr;
+  p.piece_steps = room.piece / kVtK;
+  const int type = f32 ? TKV_BF16 : l.dtype;
+  const void* w = f32 ? (const void*)(base + room.w) : l.w;
+  const int64_t rows = p.parts * room.rows, w_rows = f32 ? 3 * room.piece : l.vocab;
   CUtensorMap a[6], g[6];
-  const int box = vt_a_box(l.tokens);
-  int rc = vt_gather(l, xc, st);
-  if (rc == TKV_OK) rc = make_map_wide(&a[0], xc, l.width, rows, kVtK, box, l.dtype);
-  if (rc == TKV_OK) rc = make_map_wide(&a[1], l.w, l.width, l.vocab, kVtK, 128, l.dtype);
-  if (rc == TKV_OK) rc = make_map_wide(&g[0], l.dl, piece, rows, kVtK, box, l.dtype);
-  if (rc == TKV_OK) rc = make_map_wide(&g[1], l.w, l.width, l.vocab, 64, kVtK, l.dtype);
-  if (rc == TKV_OK) rc = make_map_wide(&g[2], l.dl, piece, rows, 64, kVtK, l.dtype);
-  if (rc == TKV_OK) rc = make_map_wide(&g[3], xc, l.width, rows, 64, kVtK, l.dtype);
-  if (rc == TKV_OK) rc = make_map_wide(&a[4], l.dl, piece, rows, 64, 32, l.dtype);
-  if (rc == TKV_OK && want_dx) rc = make_map_wide(&g[4], l.acc, l.width, (int64_t)vt_slots(l.tokens, l.width) * rows, 32, 32, TKV_F32);
-  if (rc == TKV_OK && l.dw) rc = make_map_wide(&g[5], l.dw, l.width, l.vocab, 64, 32, l.dtype);
+  int rc = f32 ? vt_gather<float>(l, base, st) : vt_gather<uint16_t>(l, base, st);
+  if (rc == TKV_OK) rc = make_map_wide(&a[0], base, l.width, rows, kVtK, p.a_box, type);
+  if (rc == TKV_OK) rc = make_map_wide(&a[1], w, l.width, w_rows, kVtK, kVtCols / 2, type);
+  if (rc == TKV_OK) rc = make_map_wide(&a[4], l.dl, room.piece, rows, 64, 32, type);
+  if (rc == TKV_OK) rc = make_map_wide(&g[0], l.dl, room.piece, rows, kVtK, p.a_box, type);
+  if (rc == TKV_OK) rc = make_map_wide(&g[1], w, l.width, w_rows, 64, kVtK, type);
+  if (rc == TKV_OK) rc = make_map_wide(&g[2], l.dl, room.piece, rows, 64, kVtK, type);
+  if (rc == TKV_OK) rc = make_map_wide(&g[3], base, l.width, rows, 64, kVtK, type);
+  if (rc == TKV_OK && want_dx) rc = make_map_wide(&g[4], l.acc, l.width, (int64_t)vt_slots(l.tokens, l.width) * room.rows, 32, 32, TKV_F32);
+  if (rc == TKV_OK && l.dw) rc = make_map_wide(&g[5], l.dw, l.width, l.vocab, f32 ? 32 : 64, 32, l.dtype);
   if (rc != TKV_OK) return rc;
   a[2] = a[3] = a[5] = a[0];
   if (!want_dx) g[4] = g[0];
   if (l.dw == nullptr) g[5] = g[0];
-  VtParams p = {};
-  p.cols = kVtCols; p.a_box = box; p.a_ranks = l.tokens > 128 ? 2 : 1; p.want_dx = want_dx; p.want_dw = l.dw != nullptr; p.l = l;
-  p.piece_steps = piece / kVtK;
-  for (int64_t v0 = 0; v0 < l.vocab && rc == TKV_OK; v0 += piece) {
-    p.v0 = v0; p.piece_cols = l.vocab - v0 < piece ? l.vocab - v0 : piece; p.more = v0 > 0;
-    if (l.dtype == TKV_BF16) {
-      rc = vt_launch<kVtLogits, __nv_bfloat16>(a, p, st);
-      if (rc == TKV_OK) rc = vt_launch<kVtGrads, __nv_bfloat16>(g, p, st);
-    } else {
-      rc = vt_launch<kVtLogits, __half>(a, p, st);
-      if (rc == TKV_OK) rc = vt_launch<kVtGrads, __half>(g, p, st);
-    }
+  for (int64_t v0 = 0; v0 < l.vocab && rc == TKV_OK; v0 += room.piece) {
+    vt_piece_at(&p, room, v0);
+    rc = vt_parts_of(p, room, base + room.w, st);
+    if (rc == TKV_OK) rc = vt_launch<kVtLogits>(a, p, st);
+    if (rc == TKV_OK) rc = vt_launch<kVtGrads>(g, p, st);
   }
   return rc;
 }
