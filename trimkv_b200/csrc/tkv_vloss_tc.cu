@@ -23,11 +23,16 @@
 
 namespace tkv {
 
-constexpr int kVtThreads = 192;                            // warp 0: copies, warp 1: products, warps 2-5: epilogue
+constexpr int kVtThreads = 320;                            // warp 0: copies, warp 1: products, warps 2-9: epilogue
 constexpr int kVtK = 64, kVtRows = 256, kVtCols = 256, kVtStages = 6;
 constexpr int kVtABytes = 128 * kVtK * 2, kVtBBytes = 128 * kVtK * 2, kVtStage = kVtABytes + kVtBBytes;
 constexpr int kVtGroup = 32;                               // row tiles that share a pass over w
 constexpr int kVtPairs = 74;
+constexpr int kVtHalf = kVtCols / 2;                       // columns of a warp of the epilogue
+// Stages that are added up in TMEM (1024 of the inner axis): the tensor cores cut what they add to an accumulator.  Relative error of a
+// logit of 40 whose products are all positive, width 4096, bf16: one sum -5.4e-6; sums of 16 stages -1.3e-6, of 8 -5.6e-7, of 4 -2.8e-7.
+// ms of 8192 x 151936 x 2048 with both gradients: 14.6, 14.7, 15.2, 16.4; us of 1500 tokens scored: 600, 620, 655, 710.
+constexpr int kVtSum = 16;
 
 enum { kVtStats, kVtLogits, kVtGrads };
 
@@ -36,7 +41,7 @@ struct VtSmem {
   uint32_t tmem_base;
   int abort_flag;
 };
-constexpr int kVtOut = 4096;                               // 32 rows of 128 bytes on their way out, two per warp of the epilogue
+constexpr int kVtOut = 4096;                               // 32 rows of 128 bytes on their way out, for every warp of the epilogue
 constexpr int kVtSmemBytes = kVtStages * kVtStage + 8 * kVtOut + (int)sizeof(VtSmem);
 static_assert(kVtSmemBytes <= 232448, "shared memory");
 
@@ -49,6 +54,7 @@ struct VtParams {
   int parts, rows, w_rows, w0;                             // of an operand (1 or 3), rows of a part of x and dL, and of w; the piece's first row there
   int want_dx, want_dw, more;                              // kVtGrads
   int64_t piece_steps;                                     // stages of a whole piece
+  int sum_steps;                                           // stages that are added up in TMEM
 };
 
 // The parts that product c takes of A and of B; with one part there is product 5 alone.
@@ -166,7 +172,7 @@ vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
   const uint32_t peer_abort = vt_of_rank(smem_u32(&sm->abort_flag), rank ^ 1);
   if (tid == 0) {
     for (int s = 0; s < kVtStages; ++s) { mbar_init(&sm->full[s], 1); mbar_init(&sm->empty[s], 1); }
-    for (int s = 0; s < 2; ++s) { mbar_init(&sm->acc_full[s], 1); mbar_init(&sm->acc_empty[s], 8); }
+    for (int s = 0; s < 2; ++s) { mbar_init(&sm->acc_full[s], 1); mbar_init(&sm->acc_empty[s], 16); }
     sm->abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -248,174 +254,167 @@ vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       while (ok && tiles.next(t)) {
         const bool a_mn = kMode == kVtGrads && !t.dx, b_mn = kMode == kVtGrads;
         const uint32_t idesc = vt_idesc(bf16, a_mn, b_mn, kMode == kVtGrads ? kVtCols : p.cols);
-        const int buf = acc & 1;
-        ok = warp_wait(&sm->acc_empty[buf], ((acc >> 1) & 1) ^ 1, abort_flag);
-        tc_fence_after();
         const int steps = t.steps * (p.parts == 1 ? 1 : kVtProducts);
-        for (int k = 0; k < steps && ok; ++k, ++it) {
+        for (int k = 0, in_sum = 0; ok && k < max(steps, 1); ++k) {      // (a share without stages: its epilogue writes zeros)
+          const int buf = acc & 1;
+          if (in_sum == 0) {
+            ok = warp_wait(&sm->acc_empty[buf], ((acc >> 1) & 1) ^ 1, abort_flag);
+            tc_fence_after();
+          }
           const int s = it % kVtStages;
-          ok = warp_wait(&sm->full[s], (it / kVtStages) & 1, abort_flag);
+          if (ok && steps > 0) ok = warp_wait(&sm->full[s], (it / kVtStages) & 1, abort_flag);
           if (!ok) break;
           tc_fence_after();
+          const bool last = in_sum == p.sum_steps - 1 || k >= steps - 1;
           if (elect_one()) {
-            const uint64_t at = (uint32_t)s * (kVtStage >> 4);
-            const uint64_t a = (a_mn ? mn_desc : k_desc) + at, b = (b_mn ? mn_desc : k_desc) + at + (kVtABytes >> 4);
-            const uint32_t da = a_mn ? 128 : 2, db = b_mn ? 128 : 2;
+            if (steps > 0) {
+              const uint64_t at = (uint32_t)s * (kVtStage >> 4);
+              const uint64_t a = (a_mn ? mn_desc : k_desc) + at, b = (b_mn ? mn_desc : k_desc) + at + (kVtABytes >> 4);
+              const uint32_t da = a_mn ? 128 : 2, db = b_mn ? 128 : 2;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) vt_mma(tm + buf * kVtCols, a + q * da, b + q * db, idesc, (k > 0 || q > 0));
-            vt_commit(&sm->empty[s]);
-            if (k == steps - 1) vt_commit(&sm->acc_full[buf]);
+              for (int q = 0; q < 4; ++q) vt_mma(tm + buf * kVtCols, a + q * da, b + q * db, idesc, (in_sum > 0 || q > 0));
+              vt_commit(&sm->empty[s]);
+            }
+            if (last) vt_commit(&sm->acc_full[buf]);
           }
           __syncwarp();
+          if (steps > 0) ++it;
+          ++in_sum;
+          if (last) { in_sum = 0; ++acc; }
         }
-        if (ok && t.steps == 0) {                          // a share without stages: its epilogue writes zeros
-          if (elect_one()) vt_commit(&sm->acc_full[buf]);
-          __syncwarp();
-        }
-        ++acc;
       }
       if (!ok && lane == 0) give_up();
     }
     __syncwarp();
   } else {
-    // ---- epilogue: thread = row of the CTA's half of the tile
-    const int quarter = warp & 3, row_in = quarter * 32 + lane;
+    // ---- epilogue: thread = row of the CTA's half of the tile, and half of its columns; the sums of kVtSum stages are added up here, where
+    // additions round.
+    const int quarter = warp & 3, row_in = quarter * 32 + lane, c0 = warp >= 6 ? kVtHalf : 0;
     const uint32_t acc_empty0 = vt_of_rank(smem_u32(&sm->acc_empty[0]), 0);
-    int acc = 0, outs = 0;
-    uint8_t* out_s = base + kVtStages * kVtStage + quarter * 2 * kVtOut;
-    // 32 rows of 128 bytes by a bulk copy: a lane puts the eight 16-byte pieces of its row in the swizzled places.  Two boxes per warp: one
-    // is filled while the other leaves.
+    int acc = 0;
+    uint8_t* box = base + kVtStages * kVtStage + (warp - 2) * kVtOut;
+    // 32 rows of 128 bytes by a bulk copy: a lane puts the eight 16-byte pieces of its row in the swizzled places.
     auto put = [&](const uint32_t* w) {
-      if (lane == 0 && outs >= 2) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+      if (lane == 0) tma_store_read();
       __syncwarp();
-      uint8_t* box = out_s + (outs & 1) * kVtOut + lane * 128;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(box + ((i ^ (lane & 7)) << 4)) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+      for (int i = 0; i < 8; ++i)
+        *reinterpret_cast<uint4*>(box + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
       fence_async_smem();
       __syncwarp();
     };
-    auto box_of = [&]() { return out_s + (outs & 1) * kVtOut; };
     bool ok = *abort_flag == 0;
     while (ok && tiles.next(t)) {
-      const int buf = acc & 1;
-      ok = (bool)__all_sync(0xffffffffu, mbar_wait_or_abort(&sm->acc_full[buf], (acc >> 1) & 1, abort_flag));
+      const int row = t.row0 + rank * 128 + row_in, first = t.row0 + rank * 128 + quarter * 32;
+      // columns of this warp that exist, and whether any of its rows is wanted (dL: the products to come read whole steps of rows)
+      const int left = (int)min((int64_t)(kMode == kVtGrads ? kVtCols : p.cols), kMode == kVtGrads ? (int64_t)p.l.width - t.col0 : p.piece_cols - t.col0) - c0;
+      const bool wanted = left > 0 && first < (kMode == kVtStats || t.dx ? tiles.n : kMode == kVtLogits ? (tiles.n + kVtK - 1) / kVtK * kVtK : (int)p.piece_cols);
+      const int steps = t.steps * (p.parts == 1 ? 1 : kVtProducts);
+      float v[kVtHalf];
+#pragma unroll
+      for (int i = 0; i < kVtHalf; ++i) v[i] = 0.f;
+      for (int k = 0; k < max(steps, 1); k += p.sum_steps) {
+        const int buf = acc & 1;
+        ok = (bool)__all_sync(0xffffffffu, mbar_wait_or_abort(&sm->acc_full[buf], (acc >> 1) & 1, abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + buf * kVtCols + c0;
+        if (wanted && steps > 0) {                         // (columns beyond the last hold what was there: nobody reads them)
+#pragma unroll
+          for (int c = 0; c < kVtHalf; c += 16) {
+            float u[16];
+            tmem_ld16(from + c, u);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[c + i] += u[i];
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) vt_arrive(acc_empty0 + buf * 8);
+        ++acc;
+      }
       if (!ok) break;
-      tc_fence_after();
-      const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + buf * kVtCols;
-      const int row = t.row0 + rank * 128 + row_in;
+      if (!wanted) {
+        // a half without columns has nothing to say of its rows
+        if (kMode == kVtStats && row < tiles.n) p.l.part[(int64_t)row * p.l.tiles + 2 * (p.tile0 + t.col0 / p.cols) + (c0 > 0)] = make_float2(-INFINITY, 0.f);
+        continue;
+      }
       if constexpr (kMode == kVtStats) {
         const bool live = row < tiles.n;
-        const int left = (int)min((int64_t)p.cols, p.piece_cols - t.col0);        // columns that exist
-        if (t.row0 + rank * 128 + quarter * 32 < tiles.n) {
-          const int label = live ? (int)(p.l.plan.label[row] - p.v0 - t.col0) : -1;
-          float top = -INFINITY, sum = 0.f;
-          for (int c = 0; c < left; c += 32) {
-            float v[32];
-            tmem_ld32(from + c, v);
-            if ((unsigned)(label - c) < 32u && label < left) {
-              float mine = 0.f;
+        const int label = live ? (int)(p.l.plan.label[row] - p.v0 - t.col0) - c0 : -1;
+        if ((unsigned)label < (unsigned)min(left, kVtHalf)) {
+          float mine = 0.f;
 #pragma unroll
-              for (int i = 0; i < 32; ++i) mine = i == label - c ? v[i] : mine;
-              p.l.mine[row] = mine;
-            }
-            __syncwarp();
-            if (c + 32 > left) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = c + i < left ? v[i] : -INFINITY;
-            }
-            float next = top;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) next = fmaxf(next, v[i]);
-            const float from0 = next == -INFINITY ? 0.f : next;
-            float part = 0.f;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) part += exp2_weight((v[i] - from0) * kLog2e);
-            sum = fmaf(sum, exp2_weight((top - from0) * kLog2e), part);
-            top = next;
-          }
-          if (live) p.l.part[(int64_t)row * p.l.tiles + p.tile0 + t.col0 / p.cols] = make_float2(top, sum);
+          for (int i = 0; i < kVtHalf; ++i) mine = i == label ? v[i] : mine;
+          p.l.mine[row] = mine;
         }
+        __syncwarp();
+        if (left < kVtHalf) {
+#pragma unroll
+          for (int i = 0; i < kVtHalf; ++i) v[i] = i < left ? v[i] : -INFINITY;
+        }
+        float top[4] = {v[0], v[1], v[2], v[3]}, sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 4; i < kVtHalf; ++i) top[i & 3] = fmaxf(top[i & 3], v[i]);
+        top[0] = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        const float at = top[0] == -INFINITY ? 0.f : top[0];
+#pragma unroll
+        for (int i = 0; i < kVtHalf; ++i) sum[i & 3] += exp2_weight((v[i] - at) * kLog2e);
+        if (live) p.l.part[(int64_t)row * p.l.tiles + 2 * (p.tile0 + t.col0 / p.cols) + (c0 > 0)] = make_float2(top[0], (sum[0] + sum[1]) + (sum[2] + sum[3]));
       } else if constexpr (kMode == kVtLogits) {
         const bool live = row < tiles.n;
-        const int label = live ? (int)(p.l.plan.label[row] - p.v0 - t.col0) : -1;
+        const int label = live ? (int)(p.l.plan.label[row] - p.v0 - t.col0) - c0 : -1;
         const float2 lse = live ? p.l.plan.lse[row] : make_float2(0.f, 0.f);
         const float g = live ? p.l.g[row] : 0.f;
-        const int left = (int)min((int64_t)p.cols, p.piece_cols - t.col0);
-        const int first = t.row0 + rank * 128 + quarter * 32;
-        // the products to come read whole steps of rows
-        for (int c = first < (tiles.n + kVtK - 1) / kVtK * kVtK ? 0 : p.cols; c < p.cols; c += 64) {
-          float v[64];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int at = c + 32 * h;
-            tmem_ld32(from + at, v + 32 * h);
+        for (int i = 0; i < kVtHalf; ++i) {                // rows and columns that do not exist are zeros for the products to come
+          const float d = exp2_weight(fmaf(v[i] - lse.x, kLog2e, -lse.y)) - (i == label ? 1.f : 0.f);
+          v[i] = live && i < left ? g * d : 0.f;
+        }
 #pragma unroll
-            for (int i = 32 * h; i < 32 * h + 32; ++i) {   // rows and columns that do not exist are zeros for the products to come
-              const float d = exp2_weight(fmaf(v[i] - lse.x, kLog2e, -lse.y)) - (i == label - c ? 1.f : 0.f);
-              v[i] = live && c + i < left ? g * d : 0.f;
-            }
-          }
+        for (int c = 0; c < kVtHalf; c += 64) {
+#pragma unroll
           for (int part = 0; part < (sizeof(T) == 4 ? 3 : 1); ++part) {
             uint32_t w[32];
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-              w[i] = vt_pack<T>(v[2 * i], v[2 * i + 1]);
-              if (sizeof(T) == 4) { v[2 * i] -= __uint_as_float(w[i] << 16); v[2 * i + 1] -= __uint_as_float(w[i] & 0xffff0000u); }
+              w[i] = vt_pack<T>(v[c + 2 * i], v[c + 2 * i + 1]);
+              if (sizeof(T) == 4) { v[c + 2 * i] -= __uint_as_float(w[i] << 16); v[c + 2 * i + 1] -= __uint_as_float(w[i] & 0xffff0000u); }
             }
             put(w);
-            if (lane == 0) tma_store_2d(&map_c, box_of(), t.col0 + c, part * p.rows + first);
-            ++outs;
+            if (lane == 0) tma_store_2d(&map_c, box, t.col0 + c0 + c, part * p.rows + first);
           }
         }
       } else {
-        const int left = p.l.width - t.col0, first = t.row0 + rank * 128 + quarter * 32;
-        const float back = t.dx ? 0.f : p.l.g_scale[1];
+        const float back = t.dx ? 1.f : p.l.g_scale[1];
         if (t.dx || sizeof(T) == 4) {                      // a share's rows are whole tiles
-          const bool any = t.dx ? first < tiles.n : first < p.piece_cols;
-          for (int c = 0; any && c < kVtCols && c < left; c += 32) {
-            float v[32];
-            if (t.steps > 0) tmem_ld32(from + c, v);
-            else {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = 0.f;
-            }
-            if (sizeof(T) == 4 && !t.dx) {
+          for (int c = 0; c < kVtHalf; c += 32) {
+            if (c >= left) break;
+            if (!t.dx) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] *= back;
+              for (int i = 0; i < 32; ++i) v[c + i] *= back;
             }
-            put(reinterpret_cast<const uint32_t*>(v));
+            put(reinterpret_cast<const uint32_t*>(v + c));
             if (lane == 0) {
               const int y = t.slot * tiles.mt * kVtRows + first;
-              if (sizeof(T) == 4 && !t.dx) tma_store_2d(&map_d, box_of(), t.col0 + c, (int)p.v0 + first);
-              else if (p.more) tma_add_2d(&map_c, box_of(), t.col0 + c, y);
-              else tma_store_2d(&map_c, box_of(), t.col0 + c, y);
+              if (!t.dx) tma_store_2d(&map_d, box, t.col0 + c0 + c, (int)p.v0 + first);
+              else if (p.more) tma_add_2d(&map_c, box, t.col0 + c0 + c, y);
+              else tma_store_2d(&map_c, box, t.col0 + c0 + c, y);
             }
-            ++outs;
           }
-        } else if (first < p.piece_cols) {
-          for (int c = 0; c < kVtCols && c < left; c += 64) {
+        } else {
+#pragma unroll
+          for (int c = 0; c < kVtHalf; c += 64) {
+            if (c >= left) break;
             uint32_t w[32];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float v[32];
-              if (t.steps > 0) tmem_ld32(from + c + 32 * h, v);
-              else {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = 0.f;
-              }
-#pragma unroll
-              for (int i = 0; i < 16; ++i) w[16 * h + i] = vt_pack<T>(v[2 * i] * back, v[2 * i + 1] * back);
-            }
+            for (int i = 0; i < 32; ++i) w[i] = vt_pack<T>(v[c + 2 * i] * back, v[c + 2 * i + 1] * back);
             put(w);
-            if (lane == 0) tma_store_2d(&map_d, box_of(), t.col0 + c, (int)p.v0 + first);
-            ++outs;
+            if (lane == 0) tma_store_2d(&map_d, box, t.col0 + c0 + c, (int)p.v0 + first);
           }
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) vt_arrive(acc_empty0 + buf * 8);
-      ++acc;
     }
     if (lane == 0 && kMode != kVtStats) tma_store_done();
     if (!ok && lane == 0) give_up();
@@ -587,7 +586,7 @@ VlossWork vloss_tc_work(int tokens, int64_t vocab, int width, int dtype, bool wa
 // What lies where in a workspace.
 struct VtRoom {
   int64_t rows, piece, xc, w, dl, acc, part, bytes;        // bytes from the start
-  int cols, tiles;
+  int cols, tiles;                                         // columns of a tile; halves of tiles
   VtRoom(int tokens, int64_t vocab, int width, int dtype, bool backward, bool dx) {
     const int64_t parts = vt_parts(dtype);
     auto pad = [](int64_t n) { return vl_round(n, 1024); };
@@ -595,7 +594,7 @@ struct VtRoom {
     piece = backward || parts == 3 ? vt_piece(tokens, vocab, width, dtype) : vocab;
     cols = backward ? kVtCols : vt_tile_cols(tokens, piece);
     const int64_t before = (vocab - 1) / piece;              // whole pieces before the last
-    tiles = (int)(before * ((piece + cols - 1) / cols) + (vocab - before * piece + cols - 1) / cols);
+    tiles = (int)(before * ((piece + cols - 1) / cols) + (vocab - before * piece + cols - 1) / cols) * 2;
     xc = 0;
     w = xc + pad(parts * rows * width * 2);
     dl = w + (parts == 3 ? pad(3 * piece * width * 2) : 0);
@@ -654,6 +653,7 @@ static VtParams vt_params(const Vloss& l, const VtRoom& room) {
   p.parts = vt_parts(l.dtype);
   p.rows = (int)room.rows;
   p.w_rows = (int)room.piece;
+  p.sum_steps = kVtSum;
   return p;
 }
 static void vt_piece_at(VtParams* p, const VtRoom& room, int64_t v0) {
@@ -724,7 +724,9 @@ int vloss_tc_backward(Vloss& l, void* ws, bool want_dx, cudaStream_t st) {
   for (int64_t v0 = 0; v0 < l.vocab && rc == TKV_OK; v0 += room.piece) {
     vt_piece_at(&p, room, v0);
     rc = vt_parts_of(p, room, base + room.w, st);
+    p.sum_steps = kVtSum;
     if (rc == TKV_OK) rc = vt_launch<kVtLogits>(a, p, st);
+    if (!f32) p.sum_steps = INT32_MAX;                     // gradients that are rounded to 8 or 11 bits in the end
     if (rc == TKV_OK) rc = vt_launch<kVtGrads>(g, p, st);
   }
   return rc;
