@@ -216,6 +216,245 @@ __global__ void __launch_bounds__(kVgThreads, 2) vloss_any_kernel(const __grid_c
   }
 }
 
+// ------------------------------------------------------------------------------------------------ few tokens, fp32, CUDA cores
+// Bound by the weight's bytes: tiles of 64 words x 64 of the inner axis come by cp.async, kFewStages of them ahead, and are multiplied with
+// up to 32 tokens.  us of 8 tokens, 162637 words, width 3488, loss and both gradients: as three parts on the tensor cores 9875, so VL_FEW.
+constexpr int kFewThreads = 256, kFewCols = 64, kFewK = 64, kFewPitch = kFewK + 4, kFewStages = 4;
+
+// 64 words a CTA: a lane has a word and, with three other warps, a quarter of every 64 of the inner axis.
+template <int kR, int kMode> __global__ void __launch_bounds__(kFewThreads) vloss_few_kernel(const __grid_constant__ Vloss p, const float* w, int64_t col0, int64_t cols) {
+  extern __shared__ __align__(16) float few_s[];
+  constexpr int kStage = (kFewCols + kR) * kFewPitch;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int n = p.plan.head[0], r0 = blockIdx.y * kR, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quarter = warp & 3;
+  if (r0 >= n) return;
+  const int word = (warp >> 2) * 32 + lane, steps = (p.width + kFewK - 1) / kFewK;
+  float* join = few_s;                                     // [quarter][token][word], when the stages are done with
+  // A thread fetches the same four columns of the same rows of every stage: words i0 + 16 i, then tokens.
+  const int i0 = threadIdx.x >> 4, k0 = 4 * (threadIdx.x & 15);
+  constexpr int kMine = kFewCols / 16 + (kR + 15) / 16;
+  const float* from[kMine];
+  bool there[kMine];
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int r = i0 + 16 * i, x_row = r - kFewCols;
+    const int64_t v = (int64_t)blockIdx.x * kFewCols + r;
+    there[i] = x_row < 0 ? v < cols : x_row < kR && r0 + x_row < n;
+    from[i] = (!there[i] ? w : x_row < 0 ? w + v * p.width : reinterpret_cast<const float*>(p.x) + (int64_t)p.plan.rows[r0 + x_row] * p.x_stride) + k0;
+  }
+  const uint32_t to0 = (uint32_t)__cvta_generic_to_shared(few_s + i0 * kFewPitch + k0);
+  int step_in = 0, slot_in = 0;
+  auto fetch = [&]() {                                     // words and tokens that do not exist, and columns beyond the last: zeros
+    if (step_in < steps) {
+      const bool in = step_in * kFewK + k0 < p.width;
+      const uint32_t to = to0 + (uint32_t)(slot_in * kStage) * 4;
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        if (i < kFewCols / 16 || i0 + 16 * i < kFewCols + kR)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + i * 16 * kFewPitch * 4), "l"(in ? from[i] : w), "r"(in && there[i] ? 16 : 0) : "memory");
+        from[i] += kFewK;
+      }
+      ++step_in;
+      slot_in = slot_in + 1 == kFewStages ? 0 : slot_in + 1;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  for (int i = 0; i < kFewStages - 1; ++i) fetch();
+  int slot = 0;
+  {
+    float2 acc[kR][2];
+#pragma unroll
+    for (int r = 0; r < kR; ++r) acc[r][0] = acc[r][1] = make_float2(0.f, 0.f);
+    for (int step = 0; step < steps; ++step) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kFewStages - 2) : "memory");
+      __syncthreads();                                     // this stage is there, and everyone is done with the one that is fetched into
+      fetch();
+      const float* stage = few_s + slot * kStage + quarter * (kFewK / 4);
+      slot = slot + 1 == kFewStages ? 0 : slot + 1;
+#pragma unroll
+      for (int k = 0; k < kFewK / 4; k += 4) {
+        const float4 f = *reinterpret_cast<const float4*>(stage + word * kFewPitch + k);
+#pragma unroll
+        for (int r = 0; r < kR; ++r) {
+          const float4 y = *reinterpret_cast<const float4*>(stage + (kFewCols + r) * kFewPitch + k);
+          acc[r][0] = fma2(make_float2(y.x, y.y), make_float2(f.x, f.y), acc[r][0]);
+          acc[r][1] = fma2(make_float2(y.z, y.w), make_float2(f.z, f.w), acc[r][1]);
+        }
+      }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kR; ++r) join[(quarter * kR + r) * kFewCols + word] = (acc[r][0].x + acc[r][0].y) + (acc[r][1].x + acc[r][1].y);
+    __syncthreads();
+    for (int r = warp; r < kR && r0 + r < n; r += kFewThreads / 32) {
+      const int t = r0 + r;
+      float s[2];
+      int64_t c[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int at = lane + 32 * h;
+        c[h] = (int64_t)blockIdx.x * kFewCols + at;
+        s[h] = (join[r * kFewCols + at] + join[(kR + r) * kFewCols + at]) + (join[(2 * kR + r) * kFewCols + at] + join[(3 * kR + r) * kFewCols + at]);
+      }
+      const int64_t label = p.plan.label[t] - col0;
+      if constexpr (kMode == kVgStats) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (c[h] == label) p.mine[t] = s[h];
+          if (c[h] < cols) top = fmaxf(top, s[h]);
+        }
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float sum = warp_add((c[0] < cols ? vl_weight(s[0], top) : 0.f) + (c[1] < cols ? vl_weight(s[1], top) : 0.f));
+        if (lane == 0) p.part[(int64_t)t * p.tiles + blockIdx.x] = make_float2(top, sum);
+      } else {
+        const float2 lse = p.plan.lse[t];
+        const float g = p.g[t];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (c[h] < cols) reinterpret_cast<float*>(p.dl)[t * p.piece + c[h]] = g * (exp2f(fmaf(s[h] - lse.x, kLog2e, -lse.y)) - (c[h] == label ? 1.f : 0.f));
+      }
+    }
+  }
+}
+
+// Shares of dx of kR tokens and 512 columns: 4 columns a thread, every fourth run of 64 words of the share to each quarter of the CTA.
+constexpr int kFewShareThreads = 512, kFewShareCols = 512, kFewWords = 64;
+
+template <int kR> __global__ void __launch_bounds__(kFewShareThreads) vloss_few_share_kernel(const __grid_constant__ Vloss p, const float* w, int64_t words, int more) {
+  __shared__ __align__(16) float ds[4][kFewWords][kR];
+  __shared__ __align__(16) float join[kR][kFewShareCols / 4];          // a quarter of the columns at a time
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int n = p.plan.head[0], slots = *p.slots, r0 = blockIdx.y * kR, quarter = threadIdx.x >> 7, t = threadIdx.x & 127;
+  if (r0 >= n || (int)blockIdx.z >= slots) return;
+  const int64_t each = ((words + slots - 1) / slots + 3) / 4 * 4, first = blockIdx.z * each, last = min(words, first + each);
+  const int c = blockIdx.x * kFewShareCols + 4 * t;
+  const bool mine = c < p.width;
+  float2 acc[kR][2];
+#pragma unroll
+  for (int r = 0; r < kR; ++r) acc[r][0] = acc[r][1] = make_float2(0.f, 0.f);
+  for (int64_t v0 = first; v0 < last; v0 += 4 * kFewWords) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < 4 * kFewWords * kR; i += kFewShareThreads) {
+      const int r = i / (4 * kFewWords), k = i - r * (4 * kFewWords);
+      ds[k / kFewWords][k % kFewWords][r] = r0 + r < n && v0 + k < last ? reinterpret_cast<const float*>(p.dl)[(int64_t)(r0 + r) * p.piece + v0 + k] : 0.f;
+    }
+    __syncthreads();
+    const int64_t v1 = v0 + quarter * kFewWords;
+    const int left = mine ? (int)min((int64_t)kFewWords, last - v1) : 0;
+    const float* at = w + v1 * p.width + c;
+    for (int k = 0; k < left; k += 8) {
+      float4 f[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = k + i < left ? *reinterpret_cast<const float4*>(at + (int64_t)(k + i) * p.width) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int r = 0; r < kR; ++r) {
+          const float d = ds[quarter][k + i][r];
+          acc[r][0] = fma2(make_float2(f[i].x, f[i].y), make_float2(d, d), acc[r][0]);
+          acc[r][1] = fma2(make_float2(f[i].z, f[i].w), make_float2(d, d), acc[r][1]);
+        }
+    }
+  }
+  for (int part = 0; part < 4; ++part) {                   // threads 32 part .. + 31 of every quarter, the quarters in order
+    const bool in = (t >> 5) == part;
+    for (int q = 0; q < 4; ++q) {
+      __syncthreads();
+      if (in && quarter == q)
+#pragma unroll
+        for (int r = 0; r < kR; ++r) {
+          float4* to = reinterpret_cast<float4*>(&join[r][4 * (t & 31)]);
+          float4 s = make_float4(acc[r][0].x, acc[r][0].y, acc[r][1].x, acc[r][1].y);
+          if (q > 0) { s.x += to->x; s.y += to->y; s.z += to->z; s.w += to->w; }
+          if (q < 3) { *to = s; continue; }
+          if (!mine || r0 + r >= n) continue;
+          float4* out = reinterpret_cast<float4*>(p.acc + ((int64_t)blockIdx.z * n + r0 + r) * p.width + c);
+          if (more) { const float4 o = *out; s.x += o.x; s.y += o.y; s.z += o.z; s.w += o.w; }
+          *out = s;
+        }
+    }
+  }
+}
+
+// dw of up to kR tokens: a thread has four columns of all of them in registers and writes those of 64 words.
+constexpr int kFewOutThreads = 128;
+
+template <int kR> __global__ void __launch_bounds__(kFewOutThreads) vloss_few_out_kernel(const __grid_constant__ Vloss p, int64_t v0, int64_t words) {
+  __shared__ __align__(16) float ds[kFewWords][kR];
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int n = p.plan.head[0];
+  const int64_t first = (int64_t)blockIdx.x * kFewWords;
+  const int c = (blockIdx.y * kFewOutThreads + threadIdx.x) * 4, left = (int)min((int64_t)kFewWords, words - first);
+  for (int i = threadIdx.x; i < kR * kFewWords; i += kFewOutThreads) {
+    const int r = i / kFewWords, k = i - r * kFewWords;
+    ds[k][r] = r < n && k < left ? reinterpret_cast<const float*>(p.dl)[r * p.piece + first + k] : 0.f;
+  }
+  float4 x[kR];
+#pragma unroll
+  for (int r = 0; r < kR; ++r)
+    x[r] = r < n && c < p.width ? *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.x) + (int64_t)p.plan.rows[r] * p.x_stride + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+  __syncthreads();
+  if (c >= p.width) return;
+  const float back = p.g_scale[1];
+  float* out = reinterpret_cast<float*>(p.dw) + (v0 + first) * p.width + c;
+  for (int k = 0; k < left; ++k) {
+    float2 a = make_float2(0.f, 0.f), b = a;
+#pragma unroll
+    for (int r = 0; r < kR; ++r) {
+      const float d = ds[k][r];
+      a = fma2(make_float2(x[r].x, x[r].y), make_float2(d, d), a);
+      b = fma2(make_float2(x[r].z, x[r].w), make_float2(d, d), b);
+    }
+    *reinterpret_cast<float4*>(out + (int64_t)k * p.width) = make_float4(a.x * back, a.y * back, b.x * back, b.y * back);
+  }
+}
+
+// Where they are used: fp32, rows of x and w in vectors of 16 bytes, few enough tokens that a pass over w for each 32 of them costs less
+// than what taking w apart does.
+static bool few_shape(int tokens, int width, int dtype) { return dtype == TKV_F32 && width % 8 == 0 && tokens > 0 && tokens <= 32; }
+static int few_rows(int tokens) { return tokens <= 8 ? 8 : tokens <= 16 ? 16 : 32; }
+template <int kR, int kMode> static int few_launch(const Vloss& p, const float* w, int64_t col0, int64_t cols, cudaStream_t st) {
+  constexpr int kBytes = kFewStages * (kFewCols + kR) * kFewPitch * 4;
+  static_assert(4 * kR * kFewCols * 4 <= kBytes, "the quarters are joined where the stages were");
+  const int64_t tiles = (cols + kFewCols - 1) / kFewCols;
+  static bool allowed[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev < 0 || dev >= 64 || !allowed[dev])) {
+    e = cudaFuncSetAttribute(vloss_few_kernel<kR, kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+    if (e == cudaSuccess && dev >= 0 && dev < 64) allowed[dev] = true;
+  }
+  if (e == cudaSuccess)
+    e = launch_pdl(vloss_few_kernel<kR, kMode>, dim3((unsigned)tiles, (p.tokens + kR - 1) / kR), dim3(kFewThreads), (size_t)kBytes, st, p, w, col0, cols);
+  return e == cudaSuccess ? check_launch("tkv_vloss") : fail(TKV_ERR_LAUNCH, "tkv_vloss: %s", cudaGetErrorString(e));
+}
+template <int kMode> static int few_launch(const Vloss& p, const float* w, int64_t col0, int64_t cols, cudaStream_t st) {
+  switch (few_rows(p.tokens)) {
+    case 8: return few_launch<8, kMode>(p, w, col0, cols, st);
+    case 16: return few_launch<16, kMode>(p, w, col0, cols, st);
+    default: return few_launch<32, kMode>(p, w, col0, cols, st);
+  }
+}
+static int few_out_launch(const Vloss& p, int64_t v0, int64_t words, cudaStream_t st) {
+  const int r = few_rows(p.tokens);
+  const int64_t blocks = (words + kFewWords - 1) / kFewWords;
+  cudaError_t e = launch_pdl(r == 8 ? vloss_few_out_kernel<8> : r == 16 ? vloss_few_out_kernel<16> : vloss_few_out_kernel<32>,
+                             dim3((unsigned)blocks, (p.width + 4 * kFewOutThreads - 1) / (4 * kFewOutThreads)), dim3(kFewOutThreads), 0, st, p, v0, words);
+  return e == cudaSuccess ? check_launch("tkv_vloss") : fail(TKV_ERR_LAUNCH, "tkv_vloss: %s", cudaGetErrorString(e));
+}
+static int few_share_launch(const Vloss& p, const float* w, int64_t words, int room, int more, cudaStream_t st) {
+  const int r = p.tokens <= 8 ? 8 : 16;
+  cudaError_t e = launch_pdl(r == 8 ? vloss_few_share_kernel<8> : vloss_few_share_kernel<16>, dim3((p.width + kFewShareCols - 1) / kFewShareCols, (p.tokens + r - 1) / r, room),
+                             dim3(kFewShareThreads), 0, st, p, w, words, more);
+  return e == cudaSuccess ? check_launch("tkv_vloss") : fail(TKV_ERR_LAUNCH, "tkv_vloss: %s", cudaGetErrorString(e));
+}
+
 template <typename TA, bool kAK, typename TB, bool kBK, int kMode, typename TOut> static int vg_launch(const VgProduct& p, cudaStream_t st) {
   const int64_t mt = (p.m + kVgTile - 1) / kVgTile, nt = (p.n + kVgTile - 1) / kVgTile;
   if (nt > 65535 || mt > INT32_MAX) return fail(TKV_ERR_UNSUPPORTED, "tkv_vloss: %lld x %lld tiles", (long long)mt, (long long)nt);
@@ -248,7 +487,7 @@ static int any_slots(int tokens, int width) {
   return (int)(s < 1 ? 1 : s > kVlMaxSlots ? kVlMaxSlots : s);
 }
 
-template <typename T> static int vloss_any_backward(Vloss l, bool want_dx, int most_slots, cudaStream_t st) {
+template <typename T> static int vloss_any_backward(Vloss l, bool want_dx, int most_slots, bool few, cudaStream_t st) {
   for (int64_t v0 = 0; v0 < l.vocab; v0 += l.piece) {
     const int64_t n = l.vocab - v0 < l.piece ? l.vocab - v0 : l.piece;
     const T* w = reinterpret_cast<const T*>(l.w) + v0 * l.width;
@@ -257,13 +496,17 @@ template <typename T> static int vloss_any_backward(Vloss l, bool want_dx, int m
     const VgOperand x = {l.x, l.x_stride, l.plan.rows, vec4(l.x, l.x_stride, sizeof(T))}, wk = {w, l.width, nullptr, vec4(w, l.width, sizeof(T))},
                     dl = {l.dl, l.piece, nullptr, vec4(l.dl, l.piece, 4)};
     p.a = x; p.b = wk; p.m = l.tokens; p.n = n; p.k = p.split_len = l.width; p.token_axis = 0;
-    int rc = vg_launch<T, true, T, true, kVgLogitGrad, T>(p, st);
-    if (rc == TKV_OK && want_dx) {
+    int rc = few ? few_launch<kVgLogitGrad>(l, reinterpret_cast<const float*>(w), v0, n, st) : vg_launch<T, true, T, true, kVgLogitGrad, T>(p, st);
+    if (rc == TKV_OK && want_dx && few) {
+      rc = few_share_launch(l, reinterpret_cast<const float*>(w), n, most_slots, v0 > 0, st);
+    } else if (rc == TKV_OK && want_dx) {
       p.a = dl; p.b = wk; p.m = l.tokens; p.n = l.width; p.k = n; p.token_axis = 0;
       p.split = most_slots; p.split_len = l.piece; p.more = v0 > 0;
       rc = vg_launch<float, true, T, false, kVgShare, T>(p, st);
     }
-    if (rc == TKV_OK && l.dw) {
+    if (rc == TKV_OK && l.dw && few) {
+      rc = few_out_launch(l, v0, n, st);
+    } else if (rc == TKV_OK && l.dw) {
       p.a = dl; p.b = x; p.m = n; p.n = l.width; p.k = p.split_len = l.tokens; p.token_axis = 2; p.split = 1;
       rc = vg_launch<float, false, T, false, kVgOut, T>(p, st);
     }
@@ -429,9 +672,10 @@ template <typename... A> static int vl_launch(const char* what, void (*kernel)(A
 int vloss_plan_rows(const Vloss& p, const int64_t* labels, int64_t ignore, float* loss, cudaStream_t st) {
   return vl_launch("tkv_vloss_forward", vloss_plan_kernel, dim3(1), kPlanThreads, st, labels, ignore, p.tokens, p.vocab, p.plan, loss, p.status);
 }
-static bool use_tc(const Vloss& p) { return vloss_tc_shape(p.tokens, p.vocab, p.width, p.dtype) && aligned16(p.w) && (p.dw == nullptr || aligned16(p.dw)); }
+static bool use_few(const Vloss& p) { return few_shape(p.tokens, p.width, p.dtype) && aligned16(p.w) && aligned16(p.x) && p.x_stride % 4 == 0; }
+static bool use_tc(const Vloss& p) { return !use_few(p) && vloss_tc_shape(p.tokens, p.vocab, p.width, p.dtype) && aligned16(p.w) && (p.dw == nullptr || aligned16(p.dw)); }
 static int64_t pad256(int64_t bytes) { return vl_round(bytes, 256); }
-static int64_t any_forward_bytes(int tokens, int64_t vocab) { return (int64_t)tokens * ((vocab + kVgTile - 1) / kVgTile) * 8; }
+static int64_t any_forward_bytes(int tokens, int64_t vocab) { return (int64_t)tokens * ((vocab + kFewCols - 1) / kFewCols) * 8; }
 static int64_t any_backward_bytes(int tokens, int64_t vocab, int width, bool dx) {
   const int64_t piece = any_piece(tokens, vocab);
   return pad256((int64_t)tokens * piece * 4) + (dx ? (int64_t)any_slots(tokens, width) * tokens * width * 4 : 0);
@@ -482,9 +726,11 @@ extern "C" int tkv_vloss_forward(const void* x, int64_t x_stride, const void* w,
   } else {
     rc = vloss_plan_rows(p, labels, ignore, loss, st);
     p.part = reinterpret_cast<float2*>(rest);
-    p.tiles = (int)((vocab + kVgTile - 1) / kVgTile);
+    const bool few = use_few(p);
+    const int tile = few ? kFewCols : kVgTile;
+    p.tiles = (int)((vocab + tile - 1) / tile);
     if (rc == TKV_OK && tokens)
-      rc = dtype == TKV_F32 ? vloss_any_forward<float>(p, st) : dtype == TKV_BF16 ? vloss_any_forward<__nv_bfloat16>(p, st) : vloss_any_forward<__half>(p, st);
+      rc = few ? few_launch<kVgStats>(p, reinterpret_cast<const float*>(w), 0, vocab, st) : dtype == TKV_F32 ? vloss_any_forward<float>(p, st) : dtype == TKV_BF16 ? vloss_any_forward<__nv_bfloat16>(p, st) : vloss_any_forward<__half>(p, st);
   }
   if (rc == TKV_OK && tokens) rc = vl_launch("tkv_vloss_forward", vloss_join_kernel, dim3((unsigned)tokens), kJoinThreads, st, p, loss);
   if (rc == TKV_OK && reduction) rc = vl_launch("tkv_vloss_forward", vloss_sum_kernel, dim3(1), kSumThreads, st, (const float*)loss, p.tokens, p.plan, reduction, reduced);
@@ -517,7 +763,9 @@ extern "C" int tkv_vloss_backward(const void* x, int64_t x_stride, const void* w
   const bool tc = use_tc(p);
   const int64_t piece = any_piece(p.tokens, vocab);
   const int room = any_slots(p.tokens, width);
-  const VlossWork work = tc ? vloss_tc_work(p.tokens, vocab, width, dtype, dx != nullptr, dw != nullptr)
+  const bool few = use_few(p);
+  const VlossWork work = few ? VlossWork{148, p.tokens <= 8 ? 8 : 16, 1, (width + kFewShareCols - 1) / kFewShareCols, 0, (int)((piece + kFewWords - 1) / kFewWords), kFewWords, room, p.tokens, dx != nullptr, false}
+                       : tc ? vloss_tc_work(p.tokens, vocab, width, dtype, dx != nullptr, dw != nullptr)
                             : VlossWork{2 * 148, kVgTile, 1, (width + kVgTile - 1) / kVgTile, 0, (int)((piece + kVgK - 1) / kVgK), kVgK, room, p.tokens, dx != nullptr, false};
   int rc = vl_launch("tkv_vloss_backward", vloss_rows_grad_kernel, dim3(1), kSumThreads, st, grad, grad_stride, reduction, p.plan, work, g, scale,
                      reinterpret_cast<int*>(scale) + 2);
@@ -529,8 +777,8 @@ extern "C" int tkv_vloss_backward(const void* x, int64_t x_stride, const void* w
     p.piece = piece;
     p.dl = rest;
     p.acc = reinterpret_cast<float*>(rest + pad256(tokens * piece * 4));
-    rc = dtype == TKV_F32 ? vloss_any_backward<float>(p, dx != nullptr, room, st)
-                          : dtype == TKV_BF16 ? vloss_any_backward<__nv_bfloat16>(p, dx != nullptr, room, st) : vloss_any_backward<__half>(p, dx != nullptr, room, st);
+    rc = dtype == TKV_F32 ? vloss_any_backward<float>(p, dx != nullptr, room, few, st)
+                          : dtype == TKV_BF16 ? vloss_any_backward<__nv_bfloat16>(p, dx != nullptr, room, false, st) : vloss_any_backward<__half>(p, dx != nullptr, room, false, st);
   }
   if (rc != TKV_OK || dx == nullptr) return rc;
   if (dtype == TKV_F32) return vl_launch("tkv_vloss_backward", vloss_dx_kernel<float>, dim3((unsigned)tokens), kDxThreads, st, p, (float*)dx);

@@ -373,6 +373,7 @@ vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         }
 #pragma unroll
         for (int c = 0; c < kVtHalf; c += 64) {
+          if (c0 + c >= p.cols) break;
 #pragma unroll
           for (int part = 0; part < (sizeof(T) == 4 ? 3 : 1); ++part) {
             uint32_t w[32];
@@ -543,12 +544,12 @@ static int vt_parts(int dtype) { return dtype == TKV_F32 ? 3 : 1; }
 static int64_t vt_rows(int tokens) { return vl_round(tokens, kVtRows); }
 // Columns of a tile: what a pair does in its rounds is rounds x columns, and a little per round; few rounds make it matter that the last
 // one is full.  us of one token, 151936 words, width 2048: 256 columns 106, by this rule (208) VL_ONE.
-static int vt_tile_cols(int tokens, int64_t vocab) {
+static int vt_tile_cols(int tokens, int64_t vocab, int step) {
   const int64_t mt = vt_rows(tokens) / kVtRows;
   if (mt * ((vocab + kVtCols - 1) / kVtCols) > 20 * kVtPairs) return kVtCols;
   int best = kVtCols;
   int64_t least = INT64_MAX;
-  for (int cols = kVtCols; cols >= 128; cols -= 16) {
+  for (int cols = kVtCols; cols >= 64; cols -= step) {
     const int64_t rounds = (mt * ((vocab + cols - 1) / cols) + kVtPairs - 1) / kVtPairs;
     if (rounds * (cols + 16) < least) { least = rounds * (cols + 16); best = cols; }
   }
@@ -592,7 +593,7 @@ struct VtRoom {
     auto pad = [](int64_t n) { return vl_round(n, 1024); };
     rows = vt_rows(tokens);
     piece = backward || parts == 3 ? vt_piece(tokens, vocab, width, dtype) : vocab;
-    cols = backward ? kVtCols : vt_tile_cols(tokens, piece);
+    cols = vt_tile_cols(tokens, piece, backward ? 64 : 16);   // dL leaves in boxes of 64 columns
     const int64_t before = (vocab - 1) / piece;              // whole pieces before the last
     tiles = (int)(before * ((piece + cols - 1) / cols) + (vocab - before * piece + cols - 1) / cols) * 2;
     xc = 0;
@@ -709,7 +710,7 @@ int vloss_tc_backward(Vloss& l, void* ws, bool want_dx, cudaStream_t st) {
   CUtensorMap a[6], g[6];
   int rc = f32 ? vt_gather<float>(l, base, st) : vt_gather<uint16_t>(l, base, st);
   if (rc == TKV_OK) rc = make_map_wide(&a[0], base, l.width, rows, kVtK, p.a_box, type);
-  if (rc == TKV_OK) rc = make_map_wide(&a[1], w, l.width, w_rows, kVtK, kVtCols / 2, type);
+  if (rc == TKV_OK) rc = make_map_wide(&a[1], w, l.width, w_rows, kVtK, p.cols / 2, type);
   if (rc == TKV_OK) rc = make_map_wide(&a[4], l.dl, room.piece, rows, 64, 32, type);
   if (rc == TKV_OK) rc = make_map_wide(&g[0], l.dl, room.piece, rows, kVtK, p.a_box, type);
   if (rc == TKV_OK) rc = make_map_wide(&g[1], w, l.width, w_rows, 64, kVtK, type);
