@@ -13,6 +13,7 @@ import torch.nn.functional as F
 from torch import nn
 
 from . import ops
+from .losses import expert_balance
 from .mixers import FusedProjection, as_f32
 
 
@@ -101,6 +102,17 @@ class SparseMLP(FeedForward):
         """Router logits in fp32, then ``(place, weight, src, offsets)``."""
         z = F.linear(x, self.router) if x.dtype == torch.float32 else torch.mm(x, self.router.t(), out_dtype=torch.float32)
         return ops.moe_route(z, as_f32(self, "correction"), self.identity, self.top, self.groups, self.keep, self.scale)
+
+    def balance(self, x, valid: Optional[torch.Tensor] = None):
+        """``(loss, counts)`` of this layer's routing of tokens ``x [tokens, width]`` (``valid``: those that are tokens, not padding), as
+        ``losses.expert_balance``: ``counts [experts + identity]`` are the tokens of each expert, the loss has a gradient for the router's
+        weight and for x."""
+        with torch.no_grad():
+            z = F.linear(x, self.router) if x.dtype == torch.float32 else torch.mm(x, self.router.t(), out_dtype=torch.float32)
+            choice = ops.moe_route_choice(z, as_f32(self, "correction"), self.identity, self.top, self.groups, self.keep, self.scale)[1]
+        if torch.is_grad_enabled() and (x.requires_grad or self.router.requires_grad):
+            z = F.linear(x.float(), self.router.float())
+        return expert_balance(z, choice, valid)
 
     def forward(self, x, status: Optional[torch.Tensor] = None):
         place, weight, src, offsets = self.route(x)

@@ -204,6 +204,12 @@ class HybridForCausalLM(HybridPreTrainedModel, TrimKVForCausalLM):
                        layers_out: Optional[list] = None) -> torch.Tensor:
         """One step of any requests of the batch: packed ids ``[sum(lengths)]`` -> fp32 logits ``[wanted, vocab]``.
         ``lengths`` None: one token per request.  ``want``: packed places (None: every token)."""
+        return self.head(self.packed_hidden(ids, cache, lengths, rows, want, layers_out))
+
+    @torch.no_grad()
+    def packed_hidden(self, ids: torch.Tensor, cache: HybridStateCache, lengths: Optional[Sequence[int]], rows: Optional[Sequence[int]] = None,
+                      want: Optional[Sequence[int]] = None, layers_out: Optional[list] = None) -> torch.Tensor:
+        """:meth:`forward_packed` up to the head: normed rows ``[wanted, width]`` in the model type."""
         if not ids.is_cuda:
             raise ops._lib.TrimKVNativeError("this model runs on CUDA tensors only (no CPU path)")
         batch = cache.begin(lengths, rows)
@@ -213,9 +219,9 @@ class HybridForCausalLM(HybridPreTrainedModel, TrimKVForCausalLM):
         at = None
         if want is not None:
             if len(want) == 0:
-                return stream.new_empty(0, self.config.vocab)
+                return self.lm_head.weight.new_empty(0, self.config.width)
             at = ops.ints_on(ids.device, list(want))
-        return self.head(self.model.final_norm(stream, at))
+        return self.model.final_norm(stream, at)
 
     def decode_step(self, ids: torch.Tensor, cache: HybridStateCache) -> torch.Tensor:
         """One token of every request of the batch, ids ``[B]`` on the device -> fp32 logits ``[B, vocab]``.  Recordable in a
@@ -224,9 +230,13 @@ class HybridForCausalLM(HybridPreTrainedModel, TrimKVForCausalLM):
         return self.head(self.model.final_norm(stream))
 
     def forward(self, input_ids=None, attention_mask=None, position_ids=None, past_key_values=None, inputs_embeds=None,
-                use_cache=None, cache_position=None, logits_to_keep=0, **kwargs):
+                use_cache=None, cache_position=None, logits_to_keep=0, labels=None, **kwargs):
         """HF call form.  ``attention_mask`` ``[B, >= S]`` marks the padding of unequal prompts, on either side; positions are
-        counted per request.  ``logits_to_keep=1``: every request's last token; 0: all places (zeros at padding)."""
+        counted per request.  ``logits_to_keep=1``: every request's last token; 0: all places (zeros at padding).
+
+        ``labels [B, S]`` (-100: does not count; or ``shift_labels``, already moved): the result has the ``loss`` of every token against the
+        label that follows it, as ``loss_of``; ``logits_to_keep=None`` then leaves the logits out.  The mixers record nothing for autograd:
+        the loss has a gradient for the head's weight and no further."""
         if input_ids is None or inputs_embeds is not None:
             raise ValueError("this model takes input_ids")
         cache = past_key_values if past_key_values is not None else self.new_cache(input_ids.device)
@@ -235,11 +245,12 @@ class HybridForCausalLM(HybridPreTrainedModel, TrimKVForCausalLM):
             cache.open(bsz)
         if cache._batch != bsz:
             raise ValueError(f"{bsz} rows for a cache of {cache._batch} requests")
-        step = self._fused_step_for(input_ids, cache, inputs_embeds, kwargs)
+        scored = labels is not None or kwargs.get("shift_labels") is not None
+        step = None if scored else self._fused_step_for(input_ids, cache, inputs_embeds, kwargs)
         if step is not None:
             logits = step(cache, input_ids, torch.zeros(1, dtype=torch.int64, device=input_ids.device))
             return CausalLMOutputWithPast(logits=logits[:, None, :], past_key_values=cache)
-        if width == 1:
+        if width == 1 and not scored:
             logits = self.forward_packed(input_ids.reshape(-1), cache, None)
             return CausalLMOutputWithPast(logits=logits[:, None, :], past_key_values=cache)
         live = None
@@ -251,6 +262,19 @@ class HybridForCausalLM(HybridPreTrainedModel, TrimKVForCausalLM):
         rows = [b for b in range(bsz) if lengths[b] > 0]  # a portion that is padding only for some requests
         ids = input_ids.reshape(-1) if live is None else input_ids[live]
         counts = [lengths[b] for b in rows]
+        if scored:
+            normed = self.packed_hidden(ids, cache, None if width == 1 else counts, None if width == 1 else rows)
+            loss = self._loss_of_packed(normed, live, labels, kwargs)
+            if logits_to_keep is None:
+                return CausalLMOutputWithPast(loss=loss, past_key_values=cache)
+            got = self.head(normed)
+            if live is None:
+                logits = got.view(bsz, width, -1)
+            else:
+                logits = got.new_zeros(bsz, width, got.shape[1])
+                logits[live] = got
+            logits = logits[:, slice(-logits_to_keep, None) if isinstance(logits_to_keep, int) else logits_to_keep]
+            return CausalLMOutputWithPast(loss=loss, logits=logits, past_key_values=cache)
         if logits_to_keep == 1:
             ends, at = [], -1
             for n in counts:
@@ -270,6 +294,18 @@ class HybridForCausalLM(HybridPreTrainedModel, TrimKVForCausalLM):
         elif logits_to_keep:
             logits = logits[:, -logits_to_keep:]
         return CausalLMOutputWithPast(logits=logits, past_key_values=cache)
+
+    def _loss_of_packed(self, normed, live, labels, kwargs):
+        """``loss_of`` for the packed tokens that ``live [B, S]`` (None: all) marks."""
+        ignore, given = kwargs.get("ignore_index"), kwargs.get("shift_labels")
+        ignore = -100 if ignore is None else ignore
+        target = given
+        if target is None:
+            target = F.pad(labels[:, 1:], (0, 1), value=ignore)
+            if live is not None:                          # what follows is padding
+                target = target.masked_fill(~F.pad(live[:, 1:], (0, 1), value=False), ignore)
+        target = target.reshape(-1) if live is None else target[live]
+        return self.loss_of(normed, None, kwargs.get("num_items_in_batch"), ignore, target)
 
     def _decode_step_cls(self):
         from .decoder import HybridDecodeStep

@@ -31,6 +31,8 @@ from transformers.modeling_outputs import BaseModelOutputWithPast, CausalLMOutpu
 
 from .attn import get_attention_interface, register_with_transformers
 from .cache_utils import TrimKVCache
+from .losses import linear_cross_entropy
+from .positions import RotaryPlan, apply_rotary
 
 register_with_transformers()
 
@@ -205,7 +207,7 @@ class TrimKVAttention(nn.Module):
             retention_weights = gate(hidden_states).transpose(1, 2)
         q, k, v = q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)
         cos, sin = position_embeddings
-        q, k = apply_rotary_pos_emb(q, k, cos, sin)
+        q, k = rotate(q, k, position_embeddings)
         if gate is not None and not gate.reads_hidden_states:
             retention_weights = gate(torch.cat([k, v], dim=-1)).transpose(1, 2)
         offset = past_key_values.get_seq_length(self.layer_idx)
@@ -251,18 +253,31 @@ class TrimKVDecoderLayer(nn.Module):
         return hidden_states + self.mlp(self.post_attention_layernorm(hidden_states))
 
 
+class RotaryTables(tuple):
+    """``(cos, sin)`` of a forward pass as the eager rotation takes them; ``turn`` holds what ``positions.apply_rotary`` takes instead,
+    ``(positions, freq, scale)``, or None."""
+
+    turn = None
+
+
 class RotaryEmbedding(nn.Module):
-    """cos/sin of the (default, unscaled) rotary embedding.  The inverse frequencies stay in fp32 whatever dtype the
+    """cos/sin of the rotary embedding.  The inverse frequencies stay in fp32 whatever dtype the
     model is cast to (they are not a registered buffer, so ``model.to(bfloat16)`` cannot round them), as they do when
-    the reference model is loaded through ``from_pretrained(torch_dtype=bfloat16)``."""
+    the reference model is loaded through ``from_pretrained(torch_dtype=bfloat16)``.
+
+    ``rope_parameters`` of long-context checkpoints (``rope_type`` linear, llama3, yarn, longrope, dynamic) are taken as
+    ``positions.RotaryPlan`` describes them, their angles in 64 bits; queries and keys of a prompt are then turned by
+    ``positions.apply_rotary``, one kernel with a gradient, rounded once.  The default embedding keeps the reference's order of
+    operations and roundings unless ``config.fused_rotary`` is set, which takes the kernel for it too."""
 
     def __init__(self, config):
         super().__init__()
         rp = getattr(config, "rope_parameters", None) or {}
-        kind = rp.get("rope_type", "default")
-        if kind != "default":
-            raise NotImplementedError(f"rope_type={kind!r} (only the default rotary embedding is built)")
         d = rotary_dim_of(config)
+        self.plan = RotaryPlan(d, rope_theta_of(config), dict(
+            rp, original_max_position_embeddings=rp.get("original_max_position_embeddings")
+            or getattr(config, "original_max_position_embeddings", None)), getattr(config, "max_position_embeddings", None))
+        self.config = config
         self._inv_freq = 1.0 / (rope_theta_of(config) ** (torch.arange(0, d, 2, dtype=torch.int64).float() / d))
         self._per_device = {}
 
@@ -275,10 +290,30 @@ class RotaryEmbedding(nn.Module):
 
     @torch.no_grad()
     def forward(self, x, position_ids):
-        inv = self.inv_freq_on(x.device)
-        freqs = position_ids[:, :, None].float() * inv[None, None, :]
+        plain = self.plan.kind == "default"
+        fused = x.is_cuda and (not plain or getattr(self.config, "fused_rotary", False))
+        freq, scale = self.plan.on(x.device, position_ids) if fused or not plain else (None, 1.0)
+        if plain:
+            inv = self.inv_freq_on(x.device)
+            freqs = position_ids[:, :, None].float() * inv[None, None, :]
+        else:
+            freqs = position_ids[:, :, None].double() * freq.double().sum(-1)
         emb = torch.cat((freqs, freqs), dim=-1)
-        return emb.cos().to(x.dtype), emb.sin().to(x.dtype)
+        cos, sin = emb.cos(), emb.sin()
+        if scale != 1.0:
+            cos, sin = cos * scale, sin * scale
+        out = RotaryTables((cos.to(x.dtype), sin.to(x.dtype)))
+        if fused:
+            out.turn = (position_ids, freq, scale)
+        return out
+
+
+def rotate(q, k, position_embeddings):
+    """Queries and keys ``[B, H, S, D]`` of a layer at the positions that ``RotaryEmbedding`` was given."""
+    turn = getattr(position_embeddings, "turn", None)
+    if turn is not None:
+        return apply_rotary(q, k, turn[0], turn[1], scale=turn[2])
+    return apply_rotary_pos_emb(q, k, *position_embeddings)
 
 
 class TrimKVPreTrainedModel(PreTrainedModel):
@@ -453,9 +488,22 @@ class TrimKVForCausalLM(TrimKVPreTrainedModel, GenerationMixin):
     def _fused_decode_covers(self) -> bool:
         return self.lm_head.weight.dtype in self.decode_dtypes and self._decode_step_cls().supports(self)
 
+    def loss_of(self, hidden_states, labels, num_items_in_batch=None, ignore_index=-100, shift_labels=None):
+        """Cross entropy of ``hidden_states [B, S, H]`` against the LM head, each token with the label that follows it (``labels [B, S]``;
+        ``shift_labels``: already moved), by ``losses.linear_cross_entropy``: no logits are made.  ``num_items_in_batch``: the sum over
+        the labels divided by that, as transformers' losses have it; else their mean."""
+        if shift_labels is None:
+            shift_labels = F.pad(labels[:, 1:], (0, 1), value=ignore_index)
+        loss = linear_cross_entropy(hidden_states, self.lm_head.weight, shift_labels, ignore_index=ignore_index,
+                                    reduction="mean" if num_items_in_batch is None else "sum")
+        return loss if num_items_in_batch is None else loss / num_items_in_batch
+
     def forward(self, input_ids=None, attention_mask=None, position_ids=None, past_key_values=None, inputs_embeds=None,
-                use_cache=None, cache_position=None, logits_to_keep=0, **kwargs):
-        step = self._fused_step_for(input_ids, past_key_values, inputs_embeds, kwargs)
+                use_cache=None, cache_position=None, logits_to_keep=0, labels=None, **kwargs):
+        """``labels [B, S]`` (-100: does not count): the result has the ``loss`` (``loss_of``), differentiable where the attention
+        implementation is (``"sdpa"``).  ``logits_to_keep``: the last so many places, or those of an index; 0 all, None no logits at all, which
+        with labels is what keeps a pass over a large vocabulary small."""
+        step = self._fused_step_for(input_ids, past_key_values, inputs_embeds, dict(kwargs, labels=labels))
         if step is not None:
             pos = cache_position[-1:] if cache_position is not None else torch.full(
                 (1,), past_key_values.get_seq_length(), device=input_ids.device)
@@ -465,9 +513,14 @@ class TrimKVForCausalLM(TrimKVPreTrainedModel, GenerationMixin):
         out = self.model(input_ids=input_ids, attention_mask=attention_mask, position_ids=position_ids,
                          past_key_values=past_key_values, inputs_embeds=inputs_embeds, use_cache=use_cache,
                          cache_position=cache_position)
-        sl = slice(-logits_to_keep, None) if isinstance(logits_to_keep, int) else logits_to_keep
-        logits = self.lm_head(out.last_hidden_state[:, sl, :])
-        res = CausalLMOutputWithPast(logits=logits, past_key_values=out.past_key_values)
+        loss = logits = None
+        if labels is not None:
+            loss = self.loss_of(out.last_hidden_state, labels, **{k: kwargs[k] for k in ("num_items_in_batch", "ignore_index", "shift_labels")
+                                                                  if kwargs.get(k) is not None})
+        if logits_to_keep is not None:
+            sl = slice(-logits_to_keep, None) if isinstance(logits_to_keep, int) else logits_to_keep
+            logits = self.lm_head(out.last_hidden_state[:, sl, :])
+        res = CausalLMOutputWithPast(loss=loss, logits=logits, past_key_values=out.past_key_values)
         res.last_hidden_state = out.last_hidden_state
         return res
 

@@ -797,7 +797,7 @@ def moe_route_choice(logits, correction, identity: int, top: int, groups: int, k
                               weight.data_ptr(), choice.data_ptr(), place.data_ptr(), src.data_ptr(), _ptr(counts), offsets.data_ptr(),
                               _stream(logits)), "tkv_moe_route")
     _count(2 if T > 128 else 1)
-    return place, choice, weight, src, offsets
+    return place, choice.view(T, top), weight, src, offsets
 
 
 def moe_gemm(a, w, offsets, out, src=None, act: str = "none", status=None) -> None:
