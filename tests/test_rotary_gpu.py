@@ -211,3 +211,13 @@ def test_gradient_of_the_gradient():
     v = torch.randn_like(q)
     back, = torch.autograd.grad(d, g, v)                            # of a linear map: the map itself
     _close(back, *_want(v, pos[None], freq, "half", 0.5))
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 elements of queries: tokens on either side of the border, and the last."""
+    heads, dim, tokens = 64, 256, 131072 + 50                          # 2^17 tokens are 2^31 elements
+    q = torch.empty(1, tokens, heads, dim, device="cuda", dtype=torch.bfloat16).normal_().transpose(1, 2)
+    pos, freq = torch.arange(tokens, device="cuda"), _table(64)
+    got, _ = apply_rotary(q, None, pos, freq)
+    for s in (slice(0, 3), slice(131072 - 3, 131072 + 3), slice(tokens - 2, tokens)):
+        _close(got[:, :, s], *_want(q[:, :, s], pos[None, s], freq, "half", 1.0))

@@ -88,7 +88,8 @@ def test_c_entries_refuse_before_any_launch(lib):
     assert fwd(stride=15) == fwd(red=3) == fwd(t=-1) == fwd(v=0) == fwd(h=0) == fwd(dt=3) == -1
     assert fwd(n=need() - 1) == -1 and b"workspace" in lib.tkv_last_error()
     assert fwd(ws=ctypes.c_void_p(p.value + 4)) == -1
-    assert fwd(t=1 << 25) == fwd(v=1 << 24) == -2
+    assert fwd(t=1 << 25) == fwd(v=1 << 24) == fwd(t=1 << 22, v=1 << 22) == -2
+    assert fwd(plan=ctypes.c_void_p(p.value + 4)) == -1 and b"aligned" in lib.tkv_last_error()
     bwd = lambda x=p, w=p, t=5, v=100, h=16, red=0, dx=p, dw=p, n=1 << 25, grad=p: lib.tkv_vloss_backward(  # noqa: E731
         x, 16, w, p, grad, 1, red, t, v, h, dx, dw, p, n, 0, None, None)
     assert bwd(x=None) == bwd(w=None) == bwd(grad=None) == bwd(dx=None, dw=None) == -1 and b"NULL" in lib.tkv_last_error()

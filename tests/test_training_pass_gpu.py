@@ -93,6 +93,10 @@ def test_loss_forms():
         assert abs(float(by) * 2 - float(base.loss)) <= 2.0 ** -20 * float(base.loss)
         moved = F.pad(labels[:, 1:], (0, 1), value=-100)
         assert torch.equal(model(input_ids=ids, labels=labels, shift_labels=moved, logits_to_keep=None).loss, base.loss)
+        assert torch.equal(model(input_ids=ids, shift_labels=moved, logits_to_keep=None).loss, base.loss)
+    with torch.inference_mode():
+        assert torch.equal(model(input_ids=ids, labels=labels, logits_to_keep=None).loss, base.loss)
+    with torch.no_grad():
         assert torch.equal(model(input_ids=ids).logits, base.logits) and model(input_ids=ids).loss is None
         other = model(input_ids=ids, labels=labels.masked_fill(labels < 0, 7), logits_to_keep=None, ignore_index=7).loss
         assert bool(other.isfinite())

@@ -2,6 +2,7 @@
 reductions, gradients."""
 import pytest
 import torch
+import torch.nn.functional as F
 
 from trimkv_b200 import linear_cross_entropy, ops
 
@@ -200,7 +201,7 @@ def test_large_logits_and_certain_tokens():
     _check(x * 300, w, y)
     x = w[y] * 500
     loss = linear_cross_entropy(x, w, y, reduction="none")
-    want = torch.nn.functional.cross_entropy(x.double() @ w.double().t(), y, reduction="none")
+    want = F.cross_entropy(x.double() @ w.double().t(), y, reduction="none")
     assert bool(((loss.double() - want).abs() <= 64 * 2.0 ** -23 * 500 * 4).all())
 
 
@@ -209,7 +210,7 @@ def test_gradient_against_differences(dtype):
     x, w, y = _inputs(20, 90, 16, dtype, sharp=False)
     x, w = x.requires_grad_(), w.requires_grad_()
     dx, dw = torch.autograd.grad(linear_cross_entropy(x, w, y, reduction="sum"), (x, w))
-    f = lambda a, b: float(torch.nn.functional.cross_entropy(a.double() @ b.double().t(), y, reduction="sum"))  # noqa: E731
+    f = lambda a, b: float(F.cross_entropy(a.double() @ b.double().t(), y, reduction="sum"))  # noqa: E731
     half = torch.finfo(dtype).eps / 2
     h = 2.0 ** -8
     with torch.no_grad():
@@ -276,3 +277,27 @@ def test_no_gradient_of_the_gradient():
     dx, = torch.autograd.grad(linear_cross_entropy(x, w, y), x, create_graph=True)
     with pytest.raises(RuntimeError):
         dx.sum().backward()
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 elements of weight (and of its gradient): what the last words and the first ones give."""
+    v, h = 140000, 16384
+    g = torch.Generator(device="cuda").manual_seed(0)
+    w = torch.empty(v, h, device="cuda", dtype=BF).normal_(0, h ** -0.5, generator=g).requires_grad_()
+    x = torch.randn(3, h, generator=g, device="cuda").to(BF).requires_grad_()
+    y = torch.tensor([v - 1, 0, v - 77], device="cuda")
+    loss = linear_cross_entropy(x, w, y, reduction="none")
+    with torch.no_grad():
+        s = torch.cat([x.double() @ w[i:i + 20000].double().t() for i in range(0, v, 20000)], 1)
+        want = F.cross_entropy(s, y, reduction="none")
+        assert bool(((loss.double() - want).abs() <= h * 2.0 ** -23 * 6 + 2.0 ** -16).all())
+    dx, dw = torch.autograd.grad(loss.sum(), (x, w))
+    with torch.no_grad():
+        d = torch.softmax(s, 1)
+        d[torch.arange(3), y] -= 1
+        for rows in (slice(0, 40), slice(v - 100, v), slice(131072 - 20, 131072 + 20)):          # 131072 * 16384 = 2^31
+            t = d[:, rows].t() @ x.double()
+            size = d[:, rows].abs().t() @ x.double().abs()
+            assert bool(((dw[rows].double() - t).abs() <= size * 2.0 ** -7 + 1e-30).all())
+        ex = sum(d[:, i:i + 20000] @ w[i:i + 20000].double() for i in range(0, v, 20000))
+        assert float((dx.double() - ex).norm()) <= 2.0 ** -7 * float(ex.norm())

@@ -218,7 +218,8 @@ __global__ void __launch_bounds__(kVgThreads, 2) vloss_any_kernel(const __grid_c
 
 // ------------------------------------------------------------------------------------------------ few tokens, fp32, CUDA cores
 // Bound by the weight's bytes: tiles of 64 words x 64 of the inner axis come by cp.async, kFewStages of them ahead, and are multiplied with
-// up to 32 tokens.  us of 8 tokens, 162637 words, width 3488, loss and both gradients: as three parts on the tensor cores 9875, so VL_FEW.
+// up to 32 tokens.  us of 8 tokens, 162637 words, width 3488, loss and both gradients: as three parts on the tensor cores 9875, so 1919;
+// scoring 3400 and 504.
 constexpr int kFewThreads = 256, kFewCols = 64, kFewK = 64, kFewPitch = kFewK + 4, kFewStages = 4;
 
 // 64 words a CTA: a lane has a word and, with three other warps, a quarter of every 64 of the inner axis.
@@ -672,7 +673,7 @@ template <typename... A> static int vl_launch(const char* what, void (*kernel)(A
 int vloss_plan_rows(const Vloss& p, const int64_t* labels, int64_t ignore, float* loss, cudaStream_t st) {
   return vl_launch("tkv_vloss_forward", vloss_plan_kernel, dim3(1), kPlanThreads, st, labels, ignore, p.tokens, p.vocab, p.plan, loss, p.status);
 }
-static bool use_few(const Vloss& p) { return few_shape(p.tokens, p.width, p.dtype) && aligned16(p.w) && aligned16(p.x) && p.x_stride % 4 == 0; }
+static bool use_few(const Vloss& p) { return few_shape(p.tokens, p.width, p.dtype) && aligned16(p.w) && aligned16(p.x) && p.x_stride % 4 == 0 && (p.dw == nullptr || aligned16(p.dw)); }
 static bool use_tc(const Vloss& p) { return !use_few(p) && vloss_tc_shape(p.tokens, p.vocab, p.width, p.dtype) && aligned16(p.w) && (p.dw == nullptr || aligned16(p.dw)); }
 static int64_t pad256(int64_t bytes) { return vl_round(bytes, 256); }
 static int64_t any_forward_bytes(int tokens, int64_t vocab) { return (int64_t)tokens * ((vocab + kFewCols - 1) / kFewCols) * 8; }
@@ -683,8 +684,8 @@ static int64_t any_backward_bytes(int tokens, int64_t vocab, int width, bool dx)
 static int check_sizes(const char* what, int64_t tokens, int64_t vocab, int width, int64_t x_stride, int dtype) {
   if (tokens < 0 || vocab < 1 || width < 1 || elem_size(dtype) == 0 || (tokens > 1 && x_stride < width))
     return fail(TKV_ERR_ARG, "%s: tokens=%lld vocab=%lld width=%d rows %lld apart dtype=%d", what, (long long)tokens, (long long)vocab, width, (long long)x_stride, dtype);
-  if (tokens > (1 << 24) || vocab > (1 << 23) || width > 65536)
-    return fail(TKV_ERR_UNSUPPORTED, "%s: tokens=%lld (at most 2^24) vocab=%lld (2^23) width=%d (65536)", what, (long long)tokens, (long long)vocab, width);
+  if (tokens > (1 << 24) || vocab > (1 << 23) || width > 65536 || tokens * vocab > ((int64_t)1 << 43))
+    return fail(TKV_ERR_UNSUPPORTED, "%s: tokens=%lld (at most 2^24) vocab=%lld (2^23; together 2^43) width=%d (65536)", what, (long long)tokens, (long long)vocab, width);
   return TKV_OK;
 }
 
@@ -712,6 +713,7 @@ extern "C" int tkv_vloss_forward(const void* x, int64_t x_stride, const void* w,
   if (rc0 != TKV_OK) return rc0;
   if (reduction < 0 || reduction > 2) return fail(TKV_ERR_ARG, "tkv_vloss_forward: reduction=%d", reduction);
   if (!plan || !workspace || (reduction && !reduced) || (tokens && (!x || !w || !labels || !loss))) return fail(TKV_ERR_ARG, "tkv_vloss_forward: NULL pointer argument");
+  if (((uintptr_t)plan & 7) != 0) return fail(TKV_ERR_ARG, "tkv_vloss_forward: the plan must be 8-byte aligned");
   if (!aligned16(workspace) || workspace_bytes < tkv_vloss_workspace_bytes(tokens, vocab, width, dtype, 0, 0))
     return fail(TKV_ERR_ARG, "tkv_vloss_forward: workspace of %lld bytes", (long long)workspace_bytes);
   cudaStream_t st = (cudaStream_t)stream;
@@ -750,6 +752,7 @@ extern "C" int tkv_vloss_backward(const void* x, int64_t x_stride, const void* w
     return TKV_OK;
   }
   if (!plan || !workspace || !w || !grad || (!dx && !dw) || !x) return fail(TKV_ERR_ARG, "tkv_vloss_backward: NULL pointer argument");
+  if (((uintptr_t)plan & 7) != 0) return fail(TKV_ERR_ARG, "tkv_vloss_backward: the plan must be 8-byte aligned");
   if (!aligned16(workspace) || workspace_bytes < tkv_vloss_workspace_bytes(tokens, vocab, width, dtype, 1, dx != nullptr))
     return fail(TKV_ERR_ARG, "tkv_vloss_backward: workspace of %lld bytes", (long long)workspace_bytes);
   if (dx && width % 8 == 0 && !aligned16(dx)) return fail(TKV_ERR_ARG, "tkv_vloss_backward: dx must be 16-byte aligned");

@@ -180,7 +180,7 @@ vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm->tmem_base)), "r"(512));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
   }
-  if (kMode != kVtGrads || p.want_dx) {                    // rows of A that no copy fills: zeros cost the products least power (1 token: 139 us, and VL_ZERO)
+  if (kMode != kVtGrads || p.want_dx) {                    // rows of A that no copy fills: zeros cost the products least power (us of 1 token: 146, so 125)
     const int kept = rank < p.a_ranks ? p.a_box * 128 : 0;
     for (int i = kept + tid * 16; i < kVtABytes; i += kVtThreads * 16)
       for (int st = 0; st < kVtStages; ++st) st16(base + st * kVtStage + i, make_uint4(0, 0, 0, 0));
@@ -543,7 +543,8 @@ static int vt_parts(int dtype) { return dtype == TKV_F32 ? 3 : 1; }
 
 static int64_t vt_rows(int tokens) { return vl_round(tokens, kVtRows); }
 // Columns of a tile: what a pair does in its rounds is rounds x columns, and a little per round; few rounds make it matter that the last
-// one is full.  us of one token, 151936 words, width 2048: 256 columns 106, by this rule (208) VL_ONE.
+// one is full.  us of the logits of one token, 151936 words, width 2048:
+// 256 columns 106.3, by this rule (208) 103.7.
 static int vt_tile_cols(int tokens, int64_t vocab, int step) {
   const int64_t mt = vt_rows(tokens) / kVtRows;
   if (mt * ((vocab + kVtCols - 1) / kVtCols) > 20 * kVtPairs) return kVtCols;

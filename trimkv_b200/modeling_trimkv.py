@@ -298,11 +298,10 @@ class RotaryEmbedding(nn.Module):
             freqs = position_ids[:, :, None].float() * inv[None, None, :]
         else:
             freqs = position_ids[:, :, None].double() * freq.double().sum(-1)
-        emb = torch.cat((freqs, freqs), dim=-1)
-        cos, sin = emb.cos(), emb.sin()
+        cos, sin = freqs.cos(), freqs.sin()
         if scale != 1.0:
             cos, sin = cos * scale, sin * scale
-        out = RotaryTables((cos.to(x.dtype), sin.to(x.dtype)))
+        out = RotaryTables(torch.cat((t, t), dim=-1) for t in (cos.to(x.dtype), sin.to(x.dtype)))
         if fused:
             out.turn = (position_ids, freq, scale)
         return out
@@ -503,7 +502,8 @@ class TrimKVForCausalLM(TrimKVPreTrainedModel, GenerationMixin):
         """``labels [B, S]`` (-100: does not count): the result has the ``loss`` (``loss_of``), differentiable where the attention
         implementation is (``"sdpa"``).  ``logits_to_keep``: the last so many places, or those of an index; 0 all, None no logits at all, which
         with labels is what keeps a pass over a large vocabulary small."""
-        step = self._fused_step_for(input_ids, past_key_values, inputs_embeds, dict(kwargs, labels=labels))
+        scored = labels if labels is not None else kwargs.get("shift_labels")
+        step = self._fused_step_for(input_ids, past_key_values, inputs_embeds, dict(kwargs, labels=scored))
         if step is not None:
             pos = cache_position[-1:] if cache_position is not None else torch.full(
                 (1,), past_key_values.get_seq_length(), device=input_ids.device)
@@ -514,7 +514,7 @@ class TrimKVForCausalLM(TrimKVPreTrainedModel, GenerationMixin):
                          past_key_values=past_key_values, inputs_embeds=inputs_embeds, use_cache=use_cache,
                          cache_position=cache_position)
         loss = logits = None
-        if labels is not None:
+        if scored is not None:
             loss = self.loss_of(out.last_hidden_state, labels, **{k: kwargs[k] for k in ("num_items_in_batch", "ignore_index", "shift_labels")
                                                                   if kwargs.get(k) is not None})
         if logits_to_keep is not None:

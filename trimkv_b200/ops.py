@@ -872,7 +872,7 @@ def vloss_forward(x, w, labels, ignore: int, reduction: int, status=None):
         ws = torch.empty(max(need, 0), dtype=torch.uint8, device=x.device)
         check(lib().tkv_vloss_forward(x.data_ptr(), x.stride(0), w.data_ptr(), labels.data_ptr(), ignore, t, v, h, reduction, loss.data_ptr(),
                                       _ptr(reduced), plan.data_ptr(), ws.data_ptr(), need, dt, _ptr(status), _stream(x)), "tkv_vloss_forward")
-    _count(3 + (reduction != 0))
+    _count(3 + (reduction != 0))                      # and one or two for every piece of the vocabulary beyond the first
     return loss, reduced, plan
 
 
