@@ -89,6 +89,11 @@ __device__ __forceinline__ void vt_arrive(uint32_t cluster_addr) {
 __device__ __forceinline__ void vt_raise(uint32_t cluster_addr) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(1) : "memory");
 }
+__device__ __forceinline__ float vt_max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 // kind::f16 of a pair: D fp32, M = 256, N = n; which operands lie across the inner axis.
 __device__ __forceinline__ uint32_t vt_idesc(int bf16, int a_mn, int b_mn, int n) {
   return (1u << 4) | ((uint32_t)bf16 << 7) | ((uint32_t)bf16 << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | (16u << 24);
@@ -159,7 +164,8 @@ template <typename T> __device__ __forceinline__ uint32_t vt_pack(float a, float
 
 // Maps: a, b of the logits (x, w, K-major), c: dL; of the gradients dL along and across (a, a2), w across (b), x across (b2), shares of dx
 // (c), dw (d).
-template <int kMode, typename T>
+// kDirect: a tile is one sum (no more than sum_steps stages).
+template <int kMode, typename T, bool kDirect>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kVtThreads, 1)
 vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_a2,
                 const __grid_constant__ CUtensorMap map_b2, const __grid_constant__ CUtensorMap map_c, const __grid_constant__ CUtensorMap map_d,
@@ -311,21 +317,28 @@ vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       const bool wanted = left > 0 && first < (kMode == kVtStats || t.dx ? tiles.n : kMode == kVtLogits ? (tiles.n + kVtK - 1) / kVtK * kVtK : (int)p.piece_cols);
       const int steps = t.steps * (p.parts == 1 ? 1 : kVtProducts);
       float v[kVtHalf];
+      if (!kDirect || steps == 0) {
 #pragma unroll
-      for (int i = 0; i < kVtHalf; ++i) v[i] = 0.f;
-      for (int k = 0; k < max(steps, 1); k += p.sum_steps) {
+        for (int i = 0; i < kVtHalf; ++i) v[i] = 0.f;
+      }
+      for (int k = 0; k < (kDirect ? 1 : max(steps, 1)); k += p.sum_steps) {
         const int buf = acc & 1;
         ok = (bool)__all_sync(0xffffffffu, mbar_wait_or_abort(&sm->acc_full[buf], (acc >> 1) & 1, abort_flag));
         if (!ok) break;
         tc_fence_after();
         const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + buf * kVtCols + c0;
         if (wanted && steps > 0) {                         // (columns beyond the last hold what was there: nobody reads them)
+          if constexpr (kDirect) {
 #pragma unroll
-          for (int c = 0; c < kVtHalf; c += 16) {
-            float u[16];
-            tmem_ld16(from + c, u);
+            for (int c = 0; c < kVtHalf; c += 32) tmem_ld32(from + c, v + c);
+          } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[c + i] += u[i];
+            for (int c = 0; c < kVtHalf; c += 16) {
+              float u[16];
+              tmem_ld16(from + c, u);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) v[c + i] += u[i];
+            }
           }
         }
         tc_fence_before();
@@ -353,27 +366,49 @@ vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 #pragma unroll
           for (int i = 0; i < kVtHalf; ++i) v[i] = i < left ? v[i] : -INFINITY;
         }
-        float top[4] = {v[0], v[1], v[2], v[3]}, sum[4] = {0.f, 0.f, 0.f, 0.f};
+        float top[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-        for (int i = 4; i < kVtHalf; ++i) top[i & 3] = fmaxf(top[i & 3], v[i]);
+        for (int i = 4; i < kVtHalf; i += 8) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            top[j] = i + 4 + j < kVtHalf ? vt_max3(top[j], v[i + j], v[i + 4 + j]) : fmaxf(top[j], v[i + j]);
+        }
         top[0] = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         const float at = top[0] == -INFINITY ? 0.f : top[0];
+        const float2 below = make_float2(-at, -at), one = make_float2(1.f, 1.f), by = make_float2(kLog2e, kLog2e), none = make_float2(-0.f, -0.f);
+        float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-        for (int i = 0; i < kVtHalf; ++i) sum[i & 3] += exp2_weight((v[i] - at) * kLog2e);
-        if (live) p.l.part[(int64_t)row * p.l.tiles + 2 * (p.tile0 + t.col0 / p.cols) + (c0 > 0)] = make_float2(top[0], (sum[0] + sum[1]) + (sum[2] + sum[3]));
+        for (int i = 0; i < kVtHalf; i += 2) {
+          const float2 d = fma2(fma2(make_float2(v[i], v[i + 1]), one, below), by, none);
+          sums[(i >> 1) & 1] = fma2(make_float2(exp2_weight(d.x), exp2_weight(d.y)), one, sums[(i >> 1) & 1]);
+        }
+        if (live) p.l.part[(int64_t)row * p.l.tiles + 2 * (p.tile0 + t.col0 / p.cols) + (c0 > 0)] = make_float2(top[0], (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y));
       } else if constexpr (kMode == kVtLogits) {
         const bool live = row < tiles.n;
         const int label = live ? (int)(p.l.plan.label[row] - p.v0 - t.col0) - c0 : -1;
         const float2 lse = live ? p.l.plan.lse[row] : make_float2(0.f, 0.f);
         const float g = live ? p.l.g[row] : 0.f;
+        const float2 below = make_float2(-lse.x, -lse.x), one = make_float2(1.f, 1.f), by = make_float2(kLog2e, kLog2e), less = make_float2(-lse.y, -lse.y),
+                     gg = make_float2(g, g), none = make_float2(-0.f, -0.f);
+        const bool whole = (bool)__all_sync(0xffffffffu, live) && left >= kVtHalf, label_here = (bool)__any_sync(0xffffffffu, (unsigned)label < (unsigned)kVtHalf);
 #pragma unroll
-        for (int i = 0; i < kVtHalf; ++i) {                // rows and columns that do not exist are zeros for the products to come
-          const float d = exp2_weight(fmaf(v[i] - lse.x, kLog2e, -lse.y)) - (i == label ? 1.f : 0.f);
-          v[i] = live && i < left ? g * d : 0.f;
-        }
-#pragma unroll
-        for (int c = 0; c < kVtHalf; c += 64) {
+        for (int c = 0; c < kVtHalf; c += 64) {            // (the second half is made while the first leaves)
           if (c0 + c >= p.cols) break;
+#pragma unroll
+          for (int i = c; i < c + 64; i += 2) {
+            const float2 d = fma2(fma2(make_float2(v[i], v[i + 1]), one, below), by, less);
+            const float2 e = fma2(make_float2(exp2_weight(d.x), exp2_weight(d.y)), gg, none);
+            v[i] = e.x;
+            v[i + 1] = e.y;
+          }
+          if (label_here) {
+#pragma unroll
+            for (int i = c; i < c + 64; ++i) v[i] -= i == label ? g : 0.f;
+          }
+          if (!whole) {
+#pragma unroll
+            for (int i = c; i < c + 64; ++i) v[i] = live && i < left ? v[i] : 0.f;   // rows and columns that do not exist are zeros for the products to come
+          }
 #pragma unroll
           for (int part = 0; part < (sizeof(T) == 4 ? 3 : 1); ++part) {
             uint32_t w[32];
@@ -629,16 +664,21 @@ static int vt_parts_of(const VtParams& p, const VtRoom& room, void* w, cudaStrea
                              reinterpret_cast<const float*>(p.l.w) + p.v0 * p.l.width, p.piece_cols * p.l.width, whole, reinterpret_cast<uint16_t*>(w), room.piece * p.l.width));
 }
 
-template <int kMode, typename T> static int vt_launch(const CUtensorMap* m, const VtParams& p, cudaStream_t st) {
+template <int kMode, typename T, bool kDirect> static int vt_launch(const CUtensorMap* m, const VtParams& p, cudaStream_t st) {
   static bool allowed[64] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && (dev < 0 || dev >= 64 || !allowed[dev])) {
-    e = cudaFuncSetAttribute(vloss_tc_kernel<kMode, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kVtSmemBytes);
+    e = cudaFuncSetAttribute(vloss_tc_kernel<kMode, T, kDirect>, cudaFuncAttributeMaxDynamicSharedMemorySize, kVtSmemBytes);
     if (e == cudaSuccess && dev >= 0 && dev < 64) allowed[dev] = true;
   }
-  if (e == cudaSuccess) e = launch_pdl(vloss_tc_kernel<kMode, T>, dim3(2 * kVtPairs), dim3(kVtThreads), (size_t)kVtSmemBytes, st, m[0], m[1], m[2], m[3], m[4], m[5], p);
+  if (e == cudaSuccess) e = launch_pdl(vloss_tc_kernel<kMode, T, kDirect>, dim3(2 * kVtPairs), dim3(kVtThreads), (size_t)kVtSmemBytes, st, m[0], m[1], m[2], m[3], m[4], m[5], p);
   return vt_check(e);
+}
+template <int kMode, typename T> static int vt_launch(const CUtensorMap* m, const VtParams& p, cudaStream_t st) {
+  // the longest tile: the width (logits), the piece and the tokens (gradients)
+  const int64_t inner = kMode == kVtGrads ? (p.piece_steps > vt_rows(p.l.tokens) / kVtK ? p.piece_steps : vt_rows(p.l.tokens) / kVtK) : (p.l.width + kVtK - 1) / kVtK;
+  return inner * (p.parts == 1 ? 1 : kVtProducts) <= p.sum_steps ? vt_launch<kMode, T, true>(m, p, st) : vt_launch<kMode, T, false>(m, p, st);
 }
 template <int kMode> static int vt_launch(const CUtensorMap* m, const VtParams& p, cudaStream_t st) {
   return p.l.dtype == TKV_BF16 ? vt_launch<kMode, __nv_bfloat16>(m, p, st) : p.l.dtype == TKV_F16 ? vt_launch<kMode, __half>(m, p, st) : vt_launch<kMode, float>(m, p, st);
