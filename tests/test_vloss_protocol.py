@@ -170,3 +170,50 @@ def test_the_simulation_finds_a_missing_wait(fault):
         except AssertionError:
             found += 1
     assert found > 10
+
+
+PAIRS = 74
+
+
+def _deal(dx, dw, extra):
+    """The tiles of every pair as VtTiles deals them out: dx tiles 0 .., dw tiles dx .."""
+    more = dx % PAIRS
+    fewer = PAIRS - more
+    extra = min(extra, dw // fewer) if more else 0
+    out = []
+    for pair in range(PAIRS):
+        mine, tile, turn = [], pair - PAIRS, 0
+        while True:
+            if tile + PAIRS < dx:
+                tile += PAIRS
+                mine.append(tile)
+                continue
+            tile = dx
+            own, j = 0 if pair < more else extra, turn
+            turn += 1
+            i = pair - more + fewer * j if j < own else extra * fewer + (pair + PAIRS - more) % PAIRS + PAIRS * (j - own)
+            if i >= dw:
+                break
+            mine.append(dx + i)
+        out.append(mine)
+    return out
+
+
+def test_every_tile_of_the_gradients_is_dealt_once_and_the_busiest_pair_is_known():
+    """And the work of the busiest pair is what vloss_rows_grad_kernel chooses the number of shares by."""
+    rng = random.Random(0)
+    for _ in range(1500):
+        dx = rng.choice([0, 1, 73, 74, 75, 128, rng.randrange(600)])
+        dw = rng.choice([0, 1, rng.randrange(50), rng.randrange(3000)])
+        cd, cw = rng.randrange(1, 500), rng.randrange(1, 200)
+        more = dx % PAIRS
+        fewer = PAIRS - more
+        x = min(cd // cw, dw // fewer) if more else 0
+        for extra in (x, x + rng.randrange(5)):                               # a last piece has fewer tiles than the choice was made for
+            assert sorted(t for mine in _deal(dx, dw, extra) for t in mine) == list(range(dx + dw))
+        worst = max(sum(cd if t < dx else cw for t in mine) for mine in _deal(dx, dw, x))
+        rest = dw - x * fewer
+        last = rest % PAIRS
+        busy = (dx // PAIRS + 1) * cd + (rest // PAIRS + (last > fewer)) * cw if more else 0
+        idle = dx // PAIRS * cd + (x + rest // PAIRS + (last > 0)) * cw
+        assert worst == max(busy, idle)

@@ -575,12 +575,13 @@ __global__ void __launch_bounds__(kSumThreads) vloss_sum_kernel(const float* los
 
 // Gradient of every counting row's loss, times a power of two that brings the largest to about 2^14: fp16 keeps what is small beside it
 // (a mean over many tokens makes all of them small), and exponents of bf16 and fp32 are only shifted.
-// And the shares of dx: the tiles of a launch are dealt out in turn, those of dx first; with s shares a tile of dx takes steps / s (and a
-// little for what it writes), one of dw the tokens' steps.  The s that makes the busiest worker's work least.
+// And how the gradients' tiles are dealt out: those of dx in turn; to the workers that got one fewer, x tiles of dw each that make up for it;
+// the others of dw in turn.  With s shares a tile of dx takes steps / s (and a little for what it writes), one of dw the tokens' steps: the s
+// that makes the busiest worker's work least.
 __global__ void __launch_bounds__(kSumThreads) vloss_rows_grad_kernel(const float* grad, int64_t stride, int reduction, VlossPlan plan, VlossWork work, float* g,
                                                                       float* scale, int* slots) {
   __shared__ float red[kSumThreads / 32];
-  __shared__ int cost[kVlMaxSlots];
+  __shared__ int cost[kVlMaxSlots], extra[kVlMaxSlots];
   grid_dependency_wait();
   grid_launch_dependents();
   const int n = plan.head[0], lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -590,18 +591,17 @@ __global__ void __launch_bounds__(kSumThreads) vloss_rows_grad_kernel(const floa
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (lane == 0) red[warp] = top;
-  {
-    const int s = warp + 1, mt = (n + work.rows - 1) / work.rows;                    // this warp looks at s shares
-    const int dx = work.dx ? mt * work.ht * s : 0, all = dx + (work.dw ? work.vt * work.ht : 0);
+  if (lane == 0) {
+    const int s = warp + 1, mt = (n + work.rows - 1) / work.rows, W = work.workers;  // this warp looks at s shares
+    const int dx = work.dx ? mt * work.ht * s : 0, dw = work.dw ? work.vt * work.ht : 0;
     const int dx_cost = (work.steps + s - 1) / s + 12, dw_cost = (n + work.step - 1) / work.step + 4;
-    int most = 0;
-    for (int w = lane; w < work.workers; w += 32) {
-      const int mine = dx > w ? (dx - w - 1) / work.workers + 1 : 0, total = all > w ? (all - w - 1) / work.workers + 1 : 0;
-      most = max(most, mine * dx_cost + (total - mine) * dw_cost);
-    }
-    most = __reduce_max_sync(0xffffffffu, most);
+    const int more = dx % W, fewer = W - more;                                       // workers with a tile of dx more than the others
+    const int x = more ? min(dx_cost / dw_cost, dw / fewer) : 0, rest = dw - x * fewer, last = rest % W;
+    const int with = more ? (dx / W + 1) * dx_cost + (rest / W + (last > fewer)) * dw_cost : 0;
+    const int without = dx / W * dx_cost + (x + rest / W + (last > 0)) * dw_cost;
     const bool fits = s == 1 || ((int64_t)s * ((n + work.acc_rows - 1) / work.acc_rows * work.acc_rows) <= (int64_t)work.room * work.tokens && work.steps >= 8 * s);
-    if (lane == 0) cost[warp] = fits ? most : INT32_MAX;
+    cost[warp] = fits ? max(with, without) : INT32_MAX;
+    extra[warp] = x;
   }
   __syncthreads();
 #pragma unroll
@@ -615,7 +615,8 @@ __global__ void __launch_bounds__(kSumThreads) vloss_rows_grad_kernel(const floa
     int best = 0;
     for (int i = 1; i < kVlMaxSlots; ++i)
       if (cost[i] < cost[best]) best = i;
-    *slots = best + 1;
+    slots[0] = best + 1;
+    slots[1] = extra[best];
   }
 }
 static_assert(kSumThreads / 32 == kVlMaxSlots, "a warp for every number of shares");

@@ -38,7 +38,7 @@ struct Vloss {
   // backward
   const float* g;                                          // [tokens] gradient of each counting row's loss, times g_scale
   const float* g_scale;                                    // [2] scale and its inverse
-  const int* slots;                                        // shares of dx
+  const int* slots;                                        // [2] shares of dx; tiles of dw that make up for a tile of dx fewer
   void* dl; int64_t piece;                                 // [tokens][piece]
   float* acc;                                              // [*slots][tokens that count, whole tiles of acc_rows][width] shares of dx
   int acc_rows;

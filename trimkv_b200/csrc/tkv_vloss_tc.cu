@@ -106,29 +106,40 @@ struct VtTile {
 };
 template <int kMode> struct VtTiles {
   const VtParams& p;
-  int n, tile, count, dx_count, mt, nt, ht, vt, slots, split;
-  __device__ __forceinline__ VtTiles(const VtParams& q, int pair) : p(q) {
+  int n, tile, count, mt, nt;
+  int pair, turn, dx_count, dw_count, ht, slots, split, more, extra;   // kVtGrads: see vloss_rows_grad_kernel
+  __device__ __forceinline__ VtTiles(const VtParams& q, int at) : p(q), pair(at) {
     n = q.l.plan.head[0];
     tile = pair - kVtPairs;
     mt = (n + kVtRows - 1) / kVtRows;
     if (kMode == kVtGrads) {
       ht = (q.l.width + kVtCols - 1) / kVtCols;
-      vt = (int)((q.piece_cols + kVtRows - 1) / kVtRows);
-      slots = *q.l.slots;
+      slots = q.l.slots[0];
       split = ((int)q.piece_steps + slots - 1) / slots;
       dx_count = q.want_dx ? mt * ht * slots : 0;
-      count = dx_count + (q.want_dw ? vt * ht : 0);
+      dw_count = q.want_dw ? (int)((q.piece_cols + kVtRows - 1) / kVtRows) * ht : 0;
+      more = dx_count % kVtPairs;
+      extra = more ? min(q.l.slots[1], dw_count / (kVtPairs - more)) : 0;   // (a last piece has fewer tiles)
+      turn = 0;
     } else {
       nt = (int)((q.piece_cols + q.cols - 1) / q.cols);
       count = mt * nt;
     }
   }
+  // The next tile of dx, or of dw from dx_count on; -1 after the last.
+  __device__ __forceinline__ int next_grad() {
+    if (tile + kVtPairs < dx_count) return tile += kVtPairs;
+    tile = dx_count;
+    const int fewer = kVtPairs - more, mine = pair < more ? 0 : extra, j = turn++;
+    const int i = j < mine ? pair - more + fewer * j : extra * fewer + (pair + kVtPairs - more) % kVtPairs + kVtPairs * (j - mine);
+    return i < dw_count ? dx_count + i : -1;
+  }
   __device__ __forceinline__ bool next(VtTile& t) {
-    tile += kVtPairs;
-    if (tile >= count) return false;
     if (kMode == kVtGrads) {
-      t.dx = tile < dx_count;
-      const int i = t.dx ? tile : tile - dx_count;
+      const int at = next_grad();
+      if (at < 0) return false;
+      t.dx = at < dx_count;
+      const int i = t.dx ? at : at - dx_count;
       t.col0 = i % ht * kVtCols;
       const int r = i / ht;
       if (t.dx) {
@@ -142,6 +153,8 @@ template <int kMode> struct VtTiles {
         t.steps = (n + kVtK - 1) / kVtK;
       }
     } else {
+      tile += kVtPairs;
+      if (tile >= count) return false;
       const int per = kVtGroup * nt, g = tile / per, r = tile - g * per, rows = min(kVtGroup, mt - g * kVtGroup);
       t.dx = t.slot = t.step0 = 0;
       t.row0 = (g * kVtGroup + r % rows) * kVtRows;
