@@ -301,3 +301,65 @@ def test_offsets_beyond_32_bits():
             assert bool(((dw[rows].double() - t).abs() <= size * 2.0 ** -7 + 1e-30).all())
         ex = sum(d[:, i:i + 20000] @ w[i:i + 20000].double() for i in range(0, v, 20000))
         assert float((dx.double() - ex).norm()) <= 2.0 ** -7 * float(ex.norm())
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("t", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("v,h", [(1, 8), (3, 248), (4, 256), (5, 264), (31, 520), (33, 2048), (9000, 1000), (40000, 512), (700, 4096), (70, 16384)])
+def test_a_handful_of_tokens(dtype, t, v, h):
+    """Logits on the CUDA cores where a handful of tokens has not too many columns: rows, runs of columns and words that end inside a
+    warp's four; every second token ignored too."""
+    x, w, y = _inputs(t, v, h, dtype)
+    loss, _, _ = _check(x, w, y)
+    half = torch.where(torch.arange(t, device="cuda") % 2 == 0, torch.full_like(y, -100), y)
+    again, _, _ = _check(x, w, half)
+    assert torch.equal(again[1::2], loss[1::2])                  # a token's loss does not depend on its neighbours'
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_a_handful_of_tokens_of_odd_places(dtype):
+    x, w, y = _inputs(4, 1000, 256, dtype)
+    want = linear_cross_entropy(x, w, y, reduction="none")
+    wide = torch.full((4, 300), float("nan"), device="cuda", dtype=dtype)
+    wide[:, 3:259] = x
+    assert torch.equal(linear_cross_entropy(wide[:, 3:259], w, y, reduction="none"), want)
+    x[2, 5] = float("nan")                                       # one token's NaN is its own
+    got = linear_cross_entropy(x, w, y, reduction="none")
+    assert torch.equal(got.isnan(), torch.tensor([False, False, True, False], device="cuda")) and torch.equal(got[[0, 1, 3]], want[[0, 1, 3]])
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("t,v,h", [(1, 4000, 64), (3, 50, 200), (60, 9000, 136), (256, 30000, 72)])
+def test_the_label_entry_loses_nothing(dtype, reduction, t, v, h):
+    """The label's entry of dL counts in full: no rounding of it to 16 bits in dx, nor, up to 256 tokens of which no 32 words have more than
+    eight as their labels, in dw.  Every other entry is rounded once, sums and the last rounding are those of _check."""
+    x, w, y = _inputs(t, v, h, dtype)
+    if t > 8:
+        y = torch.arange(t, device="cuda") * 7 % v
+        assert int(torch.bincount(y // 32).max()) <= 8
+    xg, wg = x.clone().requires_grad_(), w.clone().requires_grad_()
+    grad = 0.5 + torch.rand(t, device="cuda") if reduction == "none" else torch.tensor(0.7, device="cuda")
+    dx, dw = torch.autograd.grad(linear_cross_entropy(xg, wg, y, reduction=reduction), (xg, wg), grad)
+    g = (grad if reduction == "none" else grad.expand(t) / t).double()[:, None]
+    xd, wd = x.double(), w.double()
+    p = torch.softmax(xd @ wd.t(), 1)
+    own = torch.zeros_like(p).scatter_(1, y[:, None], 1.0)
+    d, others = (p - own) * g, p * (1 - own) * g
+    half = torch.finfo(dtype).eps / 2
+    logit = h * 2.0 ** -23 * float((xd.abs() @ wd.abs().t()).max())
+    soft = 2 * logit + 2.0 ** -20 * (2 + float(-p.gather(1, y[:, None]).log().min()))
+    for got, want, size, rounded, whole, n in ((dx, d @ wd, (p * g) @ wd.abs(), others @ wd.abs(), d.abs() @ wd.abs(), v),
+                                               (dw, d.t() @ xd, (p * g).t() @ xd.abs(), others.t() @ xd.abs(), d.abs().t() @ xd.abs(), t)):
+        tol = size * 2 * soft + rounded * half * 1.01 + whole * (n + h) * 2.0 ** -23 + want.abs() * half * 1.01 + torch.finfo(dtype).smallest_normal
+        if dtype == HF:                                          # entries below fp16's smallest normal number, beside a largest of at least 2^13
+            tol = tol + 2.0 ** -38 * float(g.max()) * (wd if n == v else xd).abs().sum(0)
+        assert bool(((got.double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("t", [40, 256, 300])
+def test_one_label_for_all(dtype, t):
+    x, w, y = _inputs(t, 600, 136, dtype)
+    _check(x, w, torch.full_like(y, 77))
+    _check(x, w, 64 + y % 32)

@@ -45,6 +45,19 @@ template <int V> __device__ __forceinline__ void load_vec(const __nv_bfloat16* p
     for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
   }
 }
+template <int V> __device__ __forceinline__ void load_vec(const __half* p, float* v) {
+  if constexpr (V == 1) {
+    v[0] = __half2float(p[0]);
+  } else {
+    const uint4 r = ld16(p);
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      v[2 * i] = h.x; v[2 * i + 1] = h.y;
+    }
+  }
+}
 template <int V> __device__ __forceinline__ void store_vec(__nv_bfloat16* p, const float* v) {
   if constexpr (V == 1) {
     p[0] = __float2bfloat16_rn(v[0]);

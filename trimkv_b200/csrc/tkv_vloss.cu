@@ -609,9 +609,14 @@ __global__ void __launch_bounds__(kSumThreads) vloss_rows_grad_kernel(const floa
   int e = 0;
   if (top > 0.f && top < INFINITY) e = min(max(14 - ilogbf(top), -100), 100);
   const float s = ldexpf(1.f, e);
-  for (int i = threadIdx.x; i < n; i += kSumThreads) g[i] = grad[(int64_t)plan.rows[i] * stride] * by * s;
+  float same = 1.f;                                        // a gradient that all tokens share is multiplied in at the end: g is then a power of two
+  if (stride == 0 && top > 0.f && top < INFINITY) same = ldexpf(top, -ilogbf(top));
+  for (int i = threadIdx.x; i < n; i += kSumThreads) {
+    const float v = grad[(int64_t)plan.rows[i] * stride] * by * s;
+    g[i] = same == 1.f ? v : copysignf(ldexpf(1.f, ilogbf(v)), v);
+  }
   if (threadIdx.x == 0) {
-    scale[0] = s; scale[1] = ldexpf(1.f, -e);
+    scale[0] = s; scale[1] = ldexpf(same, -e);
     int best = 0;
     for (int i = 1; i < kVlMaxSlots; ++i)
       if (cost[i] < cost[best]) best = i;
@@ -640,6 +645,8 @@ template <typename T> __global__ void __launch_bounds__(kDxThreads) vloss_dx_ker
   const float back = p.plan.head[2] ? __int_as_float(0x7fffffff) : p.g_scale[1];
   T* out = dx + (int64_t)t * p.width;
   if (p.width % 8 == 0) {
+    const float rest = live && p.rest ? p.rest[lo] : 0.f;
+    const T* w = reinterpret_cast<const T*>(p.w) + (int64_t)(live ? p.plan.label[lo] : 0) * p.width;
     for (int c = threadIdx.x * 8; c < p.width; c += kDxThreads * 8) {
       float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       if (live)
@@ -649,6 +656,12 @@ template <typename T> __global__ void __launch_bounds__(kDxThreads) vloss_dx_ker
 #pragma unroll
           for (int e = 0; e < 8; ++e) s[e] += v[e];
         }
+      if (rest != 0.f) {
+        float v[8];
+        load_vec<8>(w + c, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] += rest * v[e];
+      }
       alignas(16) T e[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(s[i] * back);
@@ -703,7 +716,7 @@ extern "C" int64_t tkv_vloss_workspace_bytes(int64_t tokens, int64_t vocab, int 
     const int64_t tc = vloss_tc_bytes(t, vocab, width, dtype, backward != 0, want_dx != 0);
     n = n > tc ? n : tc;
   }
-  return 512 + pad256((int64_t)t * 4) + n;
+  return 512 + (backward ? 2 : 1) * pad256((int64_t)t * 4) + n;
 }
 
 extern "C" int tkv_vloss_forward(const void* x, int64_t x_stride, const void* w, const int64_t* labels, int64_t ignore, int64_t tokens,
@@ -762,9 +775,10 @@ extern "C" int tkv_vloss_backward(const void* x, int64_t x_stride, const void* w
   p.plan = vloss_plan(const_cast<int32_t*>(plan), tokens); p.status = status; p.dw = dw;
   float* scale = reinterpret_cast<float*>(workspace);
   float* g = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + 512);
-  char* rest = reinterpret_cast<char*>(g) + pad256(tokens * 4);
+  char* rest = reinterpret_cast<char*>(g) + 2 * pad256(tokens * 4);
   p.g = g; p.g_scale = scale; p.slots = reinterpret_cast<int*>(scale) + 2;
   const bool tc = use_tc(p);
+  if (tc && dtype != TKV_F32) p.rest = reinterpret_cast<float*>(reinterpret_cast<char*>(g) + pad256(tokens * 4));
   const int64_t piece = any_piece(p.tokens, vocab);
   const int room = any_slots(p.tokens, width);
   const bool few = use_few(p);

@@ -40,6 +40,7 @@ struct Vloss {
   const float* g_scale;                                    // [2] scale and its inverse
   const int* slots;                                        // [2] shares of dx; tiles of dw that make up for a tile of dx fewer
   void* dl; int64_t piece;                                 // [tokens][piece]
+  float* rest;                                             // [tokens] what rounding dL to 16 bits took from the label's entry (vloss_tc_backward)
   float* acc;                                              // [*slots][tokens that count, whole tiles of acc_rows][width] shares of dx
   int acc_rows;
   void* dw;

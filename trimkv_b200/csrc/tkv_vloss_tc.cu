@@ -33,6 +33,15 @@ constexpr int kVtHalf = kVtCols / 2;                       // columns of a warp 
 // logit of 40 whose products are all positive, width 4096, bf16: one sum -5.4e-6; sums of 16 stages -1.3e-6, of 8 -5.6e-7, of 4 -2.8e-7.
 // ms of 8192 x 151936 x 2048 with both gradients: 14.6, 14.7, 15.2, 16.4; us of 1500 tokens scored: 600, 620, 655, 710.
 constexpr int kVtSum = 16;
+// In fp32 half as many.  RMS error of the gradients of 300 tokens, width 1024, 32768 words: 1.4e-6 (dx) and 1.0e-6 (dw) with 16, 7e-7 and 5.5e-7
+// with 8 (fp32 products on the CUDA cores: 1.0e-6 and 5.4e-7), 3.8e-7 and 3.0e-7 with 4; us of the pass 780, 805, 900.
+constexpr int kVtSum32 = 8;
+// The label's entry of dL, g (p - 1), is most of its row, and what rounding it to 16 bits takes away does not average out: all of a row of
+// dx, and of dw's row of the label, is off by it.  It is kept (Vloss::rest) and goes back in where those rows are finished, w[label] rest into
+// dx, x rest into dw.  For dw every warp of 32 rows looks through the tokens' labels, up to kVtExact tokens and the first kVtExactHits of them:
+// RMS error of dw of 256 tokens, bf16, with a gradient for each token 1.7e-3 (the rounding of dw itself) for 168 us, without it 2.3e-3; 4096
+// tokens would take 1600 us for 1330.  A word that is many tokens' label averages their roundings (256 tokens of one word, all put back: 590 us).
+constexpr int kVtExact = 256, kVtExactHits = 8;
 
 enum { kVtStats, kVtLogits, kVtGrads };
 
@@ -55,6 +64,7 @@ struct VtParams {
   int want_dx, want_dw, more;                              // kVtGrads
   int64_t piece_steps;                                     // stages of a whole piece
   int sum_steps;                                           // stages that are added up in TMEM
+  const void* xc;                                          // the rows of x that count
 };
 
 // The parts that product c takes of A and of B; with one part there is product 5 alone.
@@ -415,8 +425,13 @@ vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             v[i + 1] = e.y;
           }
           if (label_here) {
+            float mine = 0.f;
 #pragma unroll
-            for (int i = c; i < c + 64; ++i) v[i] -= i == label ? g : 0.f;
+            for (int i = c; i < c + 64; ++i) {
+              v[i] -= i == label ? g : 0.f;
+              mine = i == label ? v[i] : mine;
+            }
+            if (sizeof(T) == 2 && (unsigned)(label - c) < 64u && label < left) p.l.rest[row] = mine - round_as<T>(mine);
           }
           if (!whole) {
 #pragma unroll
@@ -436,6 +451,30 @@ vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         }
       } else {
         const float back = t.dx ? 1.f : p.l.g_scale[1];
+        if constexpr (sizeof(T) == 2) {
+          if (!t.dx && tiles.n <= kVtExact) {
+            int room = kVtExactHits;
+            for (int i0 = 0; i0 < tiles.n && room > 0; i0 += 32) {
+              const int y = i0 + lane < tiles.n ? (int)(p.l.plan.label[i0 + lane] - p.v0 - first) : -1;
+              for (unsigned hits = __ballot_sync(0xffffffffu, (unsigned)y < 32u); hits != 0 && room > 0; hits &= hits - 1, --room) {
+                const int j = __ffs(hits) - 1, i = i0 + j, who = __shfl_sync(0xffffffffu, y, j);
+                const T* x = reinterpret_cast<const T*>(p.xc) + (int64_t)i * p.l.width + t.col0 + c0;
+                if (lane == who) {
+                  const float r = p.l.rest[i];
+#pragma unroll
+                  for (int c = 0; c < kVtHalf; c += 8) {
+                    if (c >= left) break;
+                    float u[8];
+                    load_vec<8>(x + c, u);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[c + e] += r * u[e];
+                  }
+                }
+                __syncwarp();
+              }
+            }
+          }
+        }
         if (t.dx || sizeof(T) == 4) {                      // a share's rows are whole tiles
 #pragma unroll
           for (int c = 0; c < kVtHalf; c += 32) {
@@ -589,6 +628,15 @@ __global__ void __launch_bounds__(kVtGatherThreads) vloss_first_kernel(const int
 bool vloss_tc_shape(int tokens, int64_t vocab, int width, int dtype) { return elem_size(dtype) != 0 && width % 8 == 0 && tokens > 0; }
 static int vt_parts(int dtype) { return dtype == TKV_F32 ? 3 : 1; }
 
+// ---------------------------------------------------------------------------------------------- a handful of tokens, CUDA cores
+// Logits of up to four tokens in 16 bits, bound by the weight's bytes: a warp takes four words at a time, a lane eight columns of every 256 of
+// each, and keeps the largest logit and the sum of one of the 4 kR (word, token) pairs while it goes through the vocabulary, so that a CTA
+// writes one pair of numbers for a token.  us of 151936 words, width 2048, 1, 2 and 4 tokens: 96, 98, 110; on the tensor cores, whose tiles
+// have two rows in 256 that count, 113, 116, 121.  8 tokens would take 273 for 123: 8 x 311e6 products are more than the bytes.
+// One run of columns requested ahead 117 (1 token), two 98, three 96; three CTAs an SM, with fewer registers, 103 to 227.
+constexpr int kVwThreads = 256, kVwWords = 4, kVwCols = 256, kVwCtas = 2, kVwGrid = 148 * kVwCtas, kVwTokens = 4;
+constexpr int kVwValues = 16384, kVwBytes = 2 * kVwValues * 4;   // x in shared memory: tokens up to a power of two, whole runs of 256 columns
+
 static int64_t vt_rows(int tokens) { return vl_round(tokens, kVtRows); }
 // Columns of a tile: what a pair does in its rounds is rounds x columns, and a little per round; few rounds make it matter that the last
 // one is full.  us of the logits of one token, 151936 words, width 2048:
@@ -650,7 +698,7 @@ struct VtRoom {
     dl = w + (parts == 3 ? pad(3 * piece * width * 2) : 0);
     acc = dl + (backward ? pad(parts * rows * piece * 2) : 0);
     part = acc + (backward && dx ? pad((int64_t)vt_slots(tokens, width) * rows * width * 4) : 0);
-    bytes = part + (backward ? 0 : pad((int64_t)tokens * tiles * 8));
+    bytes = part + (backward ? 0 : pad((int64_t)tokens * (tiles > kVwGrid ? tiles : kVwGrid) * 8));
   }
 };
 int64_t vloss_tc_bytes(int tokens, int64_t vocab, int width, int dtype, bool backward, bool dx) { return 1024 + VtRoom(tokens, vocab, width, dtype, backward, dx).bytes; }
@@ -697,9 +745,141 @@ template <int kMode> static int vt_launch(const CUtensorMap* m, const VtParams& 
   return p.l.dtype == TKV_BF16 ? vt_launch<kMode, __nv_bfloat16>(m, p, st) : p.l.dtype == TKV_F16 ? vt_launch<kMode, __half>(m, p, st) : vt_launch<kMode, float>(m, p, st);
 }
 
+// Sums over the lanes of N values a lane, in lane l that of value l N / 32: every exchange over O lanes halves what is left to a lane.
+template <int N, int O = 16> __device__ __forceinline__ float vw_sums(float (&v)[N], int lane) {
+  if constexpr (N == 1) {
+    float s = v[0];
+#pragma unroll
+    for (int o = O; o >= 1; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return s;
+  } else {
+    float u[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const float mine = lane & O ? v[N / 2 + i] : v[i], other = lane & O ? v[i] : v[N / 2 + i];
+      u[i] = mine + __shfl_xor_sync(0xffffffffu, other, O);
+    }
+    return vw_sums<N / 2, O / 2>(u, lane);
+  }
+}
+__device__ __forceinline__ void vw_floats(const uint4& r, float2* v, __nv_bfloat16) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+}
+__device__ __forceinline__ void vw_floats(const uint4& r, float2* v, __half) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+}
+// A largest value and the sum of the weights beside it, joined with another's.
+__device__ __forceinline__ float2 vw_join(float2 a, float2 b) {
+  const float top = fmaxf(a.x, b.x);
+  return make_float2(top, a.y * vl_weight(a.x, top) + b.y * vl_weight(b.x, top));
+}
+
+template <typename T, int kR> __global__ void __launch_bounds__(kVwThreads, kVwCtas) vloss_words_kernel(const __grid_constant__ Vloss p, const T* xc) {
+  extern __shared__ __align__(16) float4 vw_x[];            // [token][half of eight columns][eight columns], zeros behind the last
+  __shared__ float2 join[kVwThreads];
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int n = p.plan.head[0], lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int chunks = (p.width + kVwCols - 1) / kVwCols, eights = chunks * 32;
+  for (int i = threadIdx.x; i < kR * eights; i += kVwThreads) {
+    const int r = i / eights, c = i - r * eights;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (r < n && c * 8 < p.width) load_vec<8>(xc + (int64_t)r * p.width + c * 8, v);
+    vw_x[(r * 2 + 0) * eights + c] = make_float4(v[0], v[1], v[2], v[3]);
+    vw_x[(r * 2 + 1) * eights + c] = make_float4(v[4], v[5], v[6], v[7]);
+  }
+  __syncthreads();
+  constexpr int kEach = 32 / (kVwWords * kR);              // lanes with the same word and token
+  const int at = lane / kEach, r = at % kR, j = at / kR;
+  const int64_t label = r < n ? p.plan.label[r] : -1;
+  float2 mine = make_float2(-INFINITY, 0.f);
+  const T* w = reinterpret_cast<const T*>(p.w);
+  constexpr int kVwAhead = kR <= 2 ? 3 : 2;
+  // Eight columns of four words, kVwAhead of them requested before they are used: across the end of a row too.
+  const int64_t step = (int64_t)gridDim.x * (kVwThreads / 32) * kVwWords;
+  int64_t v0 = ((int64_t)blockIdx.x * (kVwThreads / 32) + warp) * kVwWords, v_in = v0;
+  const T* row[kVwWords];
+  int c_in = 0, c = 0;
+  auto rows = [&]() {
+#pragma unroll
+    for (int i = 0; i < kVwWords; ++i) row[i] = w + min(v_in + i, p.vocab - 1) * p.width + lane * 8;
+  };
+  rows();
+  uint4 ahead[kVwAhead][kVwWords];
+  auto fetch = [&](uint4 (&to)[kVwWords]) {
+    const bool in = v_in < p.vocab && c_in * kVwCols + lane * 8 < p.width;
+#pragma unroll
+    for (int i = 0; i < kVwWords; ++i) to[i] = in ? ld16_stream(row[i] + c_in * kVwCols) : make_uint4(0, 0, 0, 0);
+    if (++c_in == chunks) { c_in = 0; v_in += step; rows(); }
+  };
+#pragma unroll
+  for (int b = 0; b < kVwAhead; ++b) fetch(ahead[b]);
+  float2 acc[kVwWords * kR];
+#pragma unroll
+  for (int i = 0; i < kVwWords * kR; ++i) acc[i] = make_float2(0.f, 0.f);
+  while (v0 < p.vocab) {
+#pragma unroll
+    for (int b = 0; b < kVwAhead; ++b) {
+      if (v0 >= p.vocab) break;
+      float2 f[kVwWords][4];
+#pragma unroll
+      for (int i = 0; i < kVwWords; ++i) vw_floats(ahead[b][i], f[i], T());
+      fetch(ahead[b]);
+#pragma unroll
+      for (int t = 0; t < kR; ++t) {
+        const float4 x0 = vw_x[(t * 2 + 0) * eights + c * 32 + lane], x1 = vw_x[(t * 2 + 1) * eights + c * 32 + lane];
+#pragma unroll
+        for (int i = 0; i < kVwWords; ++i) {
+          float2& s = acc[i * kR + t];
+          s = fma2(make_float2(x0.x, x0.y), f[i][0], s);
+          s = fma2(make_float2(x0.z, x0.w), f[i][1], s);
+          s = fma2(make_float2(x1.x, x1.y), f[i][2], s);
+          s = fma2(make_float2(x1.z, x1.w), f[i][3], s);
+        }
+      }
+      if (++c < chunks) continue;
+      float sums[kVwWords * kR];
+#pragma unroll
+      for (int i = 0; i < kVwWords * kR; ++i) {
+        sums[i] = acc[i].x + acc[i].y;
+        acc[i] = make_float2(0.f, 0.f);
+      }
+      const float s = vw_sums(sums, lane);
+      if (v0 + j < p.vocab) {
+        if (v0 + j == label && lane % kEach == 0) p.mine[r] = s;
+        mine = vw_join(mine, make_float2(s, 1.f));
+      }
+      c = 0;
+      v0 += step;
+    }
+  }
+  join[threadIdx.x] = mine;
+  __syncthreads();
+  if (threadIdx.x < n) {                                   // (n <= kR)
+    float2 all = make_float2(-INFINITY, 0.f);
+    for (int i = 0; i < kVwThreads / 32 * kVwWords; ++i) all = vw_join(all, join[(i / kVwWords) * 32 + ((i % kVwWords) * kR + threadIdx.x) * kEach]);
+    p.part[(int64_t)threadIdx.x * p.tiles + blockIdx.x] = all;
+  }
+}
+
+static bool vw_shape(int tokens, int width, int dtype) { return dtype != TKV_F32 && tokens <= kVwTokens && (int64_t)tokens * width <= kVwValues; }
+template <typename T, int kR> static int vw_launch(const Vloss& p, const void* xc, cudaStream_t st) {
+  const int bytes = kR * ((p.width + kVwCols - 1) / kVwCols) * kVwCols * 4;
+  cudaError_t e = cudaFuncSetAttribute(vloss_words_kernel<T, kR>, cudaFuncAttributeMaxDynamicSharedMemorySize, kVwBytes);
+  if (e == cudaSuccess) e = launch_pdl(vloss_words_kernel<T, kR>, dim3((unsigned)p.tiles), dim3(kVwThreads), (size_t)bytes, st, p, reinterpret_cast<const T*>(xc));
+  return vt_check(e);
+}
+template <typename T> static int vw_launch(const Vloss& p, const void* xc, cudaStream_t st) {
+  return p.tokens == 1 ? vw_launch<T, 1>(p, xc, st) : p.tokens == 2 ? vw_launch<T, 2>(p, xc, st) : vw_launch<T, 4>(p, xc, st);
+}
+
 static char* vt_align(void* p) { return reinterpret_cast<char*>(((uintptr_t)p + 1023) & ~(uintptr_t)1023); }
 
-static VtParams vt_params(const Vloss& l, const VtRoom& room) {
+static VtParams vt_params(const Vloss& l, const VtRoom& room, const void* base) {
   VtParams p = {};
   p.l = l;
   p.cols = room.cols;
@@ -708,7 +888,8 @@ static VtParams vt_params(const Vloss& l, const VtRoom& room) {
   p.parts = vt_parts(l.dtype);
   p.rows = (int)room.rows;
   p.w_rows = (int)room.piece;
-  p.sum_steps = kVtSum;
+  p.sum_steps = p.parts == 1 ? kVtSum : kVtSum32;
+  p.xc = base;
   return p;
 }
 static void vt_piece_at(VtParams* p, const VtRoom& room, int64_t v0) {
@@ -731,8 +912,13 @@ int vloss_tc_forward(Vloss& l, const int64_t* labels, int64_t ignore, float* los
     if (rc == TKV_OK) rc = f32 ? vt_gather<float>(l, base, st) : vt_gather<uint16_t>(l, base, st);
   }
   l.part = reinterpret_cast<float2*>(base + room.part);
+  if (vw_shape(l.tokens, l.width, l.dtype)) {
+    const int64_t groups = (l.vocab + kVwThreads / 32 * kVwWords - 1) / (kVwThreads / 32 * kVwWords);
+    l.tiles = (int)(groups < kVwGrid ? groups : kVwGrid);
+    return rc != TKV_OK ? rc : l.dtype == TKV_BF16 ? vw_launch<__nv_bfloat16>(l, base, st) : vw_launch<__half>(l, base, st);
+  }
   l.tiles = room.tiles;
-  VtParams p = vt_params(l, room);
+  VtParams p = vt_params(l, room, base);
   const int type = f32 ? TKV_BF16 : l.dtype;
   const void* w = f32 ? (const void*)(base + room.w) : l.w;
   CUtensorMap m[6];
@@ -754,7 +940,7 @@ int vloss_tc_backward(Vloss& l, void* ws, bool want_dx, cudaStream_t st) {
   const bool f32 = l.dtype == TKV_F32;
   l.dl = base + room.dl;
   l.acc = reinterpret_cast<float*>(base + room.acc);
-  VtParams p = vt_params(l, room);
+  VtParams p = vt_params(l, room, base);
   p.want_dx = want_dx;
   p.want_dw = l.dw != nullptr;
   p.piece_steps = room.piece / kVtK;
@@ -779,7 +965,7 @@ int vloss_tc_backward(Vloss& l, void* ws, bool want_dx, cudaStream_t st) {
   for (int64_t v0 = 0; v0 < l.vocab && rc == TKV_OK; v0 += room.piece) {
     vt_piece_at(&p, room, v0);
     rc = vt_parts_of(p, room, base + room.w, st);
-    p.sum_steps = kVtSum;
+    p.sum_steps = f32 ? kVtSum32 : kVtSum;
     if (rc == TKV_OK) rc = vt_launch<kVtLogits>(a, p, st);
     if (!f32) p.sum_steps = INT32_MAX;                     // gradients that are rounded to 8 or 11 bits in the end
     if (rc == TKV_OK) rc = vt_launch<kVtGrads>(g, p, st);
