@@ -363,3 +363,14 @@ def test_one_label_for_all(dtype, t):
     x, w, y = _inputs(t, 600, 136, dtype)
     _check(x, w, torch.full_like(y, 77))
     _check(x, w, 64 + y % 32)
+
+
+@pytest.mark.parametrize("t", [33, 50, 64, 65])
+def test_some_tokens_of_a_large_fp32_head(t):
+    x, w, y = _inputs(t, 131072 + 7, 1024, SF, keep=0.9)
+    loss, dx, _ = _check(x, w, y)
+    wide = torch.zeros(t, 1027, device="cuda")
+    wide[:, 1:1025] = x                                          # rows of another alignment: another form
+    logit = 1024 * 2.0 ** -23 * float((x.double().abs() @ w.double().abs().t()).max())
+    again = linear_cross_entropy(wide[:, 1:1025], w, y, reduction="none")
+    assert bool(((again - loss).abs() <= 2 * (2 * logit + 2.0 ** -20 * (2 + float(loss.detach().max())))).all())

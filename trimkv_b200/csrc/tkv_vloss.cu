@@ -218,20 +218,22 @@ __global__ void __launch_bounds__(kVgThreads, 2) vloss_any_kernel(const __grid_c
 
 // ------------------------------------------------------------------------------------------------ few tokens, fp32, CUDA cores
 // Bound by the weight's bytes: tiles of 64 words x 64 of the inner axis come by cp.async, kFewStages of them ahead, and are multiplied with
-// up to 32 tokens.  us of 8 tokens, 162637 words, width 3488, loss and both gradients: as three parts on the tensor cores 9875, so 1919;
-// scoring 3400 and 504.
+// up to 32 tokens.  us of 8 tokens, 162637 words, width 3488, loss and both gradients: as three parts on the tensor cores 9200, so 1750;
+// scoring 3600 and 430 (5.3 TB/s).  32 tokens, bound by the products: 4230 and 1155.
 constexpr int kFewThreads = 256, kFewCols = 64, kFewK = 64, kFewPitch = kFewK + 4, kFewStages = 4;
 
-// 64 words a CTA: a lane has a word and, with three other warps, a quarter of every 64 of the inner axis.
+// 64 words a CTA: a warp has all of them, two a lane, up to 16 tokens and a part of every 64 of the inner axis.  (Every value of a token
+// that comes out of shared memory is used for two words; with one word a lane those loads took as long as the products.)
 template <int kR, int kMode> __global__ void __launch_bounds__(kFewThreads) vloss_few_kernel(const __grid_constant__ Vloss p, const float* w, int64_t col0, int64_t cols) {
   extern __shared__ __align__(16) float few_s[];
   constexpr int kStage = (kFewCols + kR) * kFewPitch;
   grid_dependency_wait();
   grid_launch_dependents();
-  const int n = p.plan.head[0], r0 = blockIdx.y * kR, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quarter = warp & 3;
+  const int n = p.plan.head[0], r0 = blockIdx.y * kR, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (r0 >= n) return;
-  const int word = (warp >> 2) * 32 + lane, steps = (p.width + kFewK - 1) / kFewK;
-  float* join = few_s;                                     // [quarter][token][word], when the stages are done with
+  constexpr int kRows = kR > 8 ? kR / 2 : kR, kSplit = kFewThreads / 32 * kRows / kR, kPart = kFewK / kSplit;
+  const int part = warp % kSplit, first = warp / kSplit * kRows, steps = (p.width + kFewK - 1) / kFewK;
+  float* join = few_s;                                     // [part][token][word], when the stages are done with
   // A thread fetches the same four columns of the same rows of every stage: words i0 + 16 i, then tokens.
   const int i0 = threadIdx.x >> 4, k0 = 4 * (threadIdx.x & 15);
   constexpr int kMine = kFewCols / 16 + (kR + 15) / 16;
@@ -264,30 +266,34 @@ template <int kR, int kMode> __global__ void __launch_bounds__(kFewThreads) vlos
   for (int i = 0; i < kFewStages - 1; ++i) fetch();
   int slot = 0;
   {
-    float2 acc[kR][2];
+    float2 acc[kRows][2];
 #pragma unroll
-    for (int r = 0; r < kR; ++r) acc[r][0] = acc[r][1] = make_float2(0.f, 0.f);
+    for (int r = 0; r < kRows; ++r) acc[r][0] = acc[r][1] = make_float2(0.f, 0.f);
     for (int step = 0; step < steps; ++step) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kFewStages - 2) : "memory");
       __syncthreads();                                     // this stage is there, and everyone is done with the one that is fetched into
       fetch();
-      const float* stage = few_s + slot * kStage + quarter * (kFewK / 4);
+      const float* stage = few_s + slot * kStage + part * kPart;
       slot = slot + 1 == kFewStages ? 0 : slot + 1;
 #pragma unroll
-      for (int k = 0; k < kFewK / 4; k += 4) {
-        const float4 f = *reinterpret_cast<const float4*>(stage + word * kFewPitch + k);
+      for (int k = 0; k < kPart; k += 4) {
+        const float4 f0 = *reinterpret_cast<const float4*>(stage + lane * kFewPitch + k), f1 = *reinterpret_cast<const float4*>(stage + (lane + 32) * kFewPitch + k);
 #pragma unroll
-        for (int r = 0; r < kR; ++r) {
-          const float4 y = *reinterpret_cast<const float4*>(stage + (kFewCols + r) * kFewPitch + k);
-          acc[r][0] = fma2(make_float2(y.x, y.y), make_float2(f.x, f.y), acc[r][0]);
-          acc[r][1] = fma2(make_float2(y.z, y.w), make_float2(f.z, f.w), acc[r][1]);
+        for (int r = 0; r < kRows; ++r) {
+          const float4 y = *reinterpret_cast<const float4*>(stage + (kFewCols + first + r) * kFewPitch + k);
+          acc[r][0] = fma2(make_float2(y.x, y.y), make_float2(f0.x, f0.y), acc[r][0]);
+          acc[r][1] = fma2(make_float2(y.x, y.y), make_float2(f1.x, f1.y), acc[r][1]);
+          acc[r][0] = fma2(make_float2(y.z, y.w), make_float2(f0.z, f0.w), acc[r][0]);
+          acc[r][1] = fma2(make_float2(y.z, y.w), make_float2(f1.z, f1.w), acc[r][1]);
         }
       }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < kR; ++r) join[(quarter * kR + r) * kFewCols + word] = (acc[r][0].x + acc[r][0].y) + (acc[r][1].x + acc[r][1].y);
+    for (int r = 0; r < kRows; ++r)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) join[(part * kR + first + r) * kFewCols + lane + 32 * h] = acc[r][h].x + acc[r][h].y;
     __syncthreads();
     for (int r = warp; r < kR && r0 + r < n; r += kFewThreads / 32) {
       const int t = r0 + r;
@@ -297,7 +303,9 @@ template <int kR, int kMode> __global__ void __launch_bounds__(kFewThreads) vlos
       for (int h = 0; h < 2; ++h) {
         const int at = lane + 32 * h;
         c[h] = (int64_t)blockIdx.x * kFewCols + at;
-        s[h] = (join[r * kFewCols + at] + join[(kR + r) * kFewCols + at]) + (join[(2 * kR + r) * kFewCols + at] + join[(3 * kR + r) * kFewCols + at]);
+        s[h] = join[r * kFewCols + at];
+#pragma unroll
+        for (int i = 1; i < kSplit; ++i) s[h] += join[(i * kR + r) * kFewCols + at];
       }
       const int64_t label = p.plan.label[t] - col0;
       if constexpr (kMode == kVgStats) {
@@ -335,9 +343,11 @@ template <int kR> __global__ void __launch_bounds__(kFewShareThreads) vloss_few_
   const int64_t each = ((words + slots - 1) / slots + 3) / 4 * 4, first = blockIdx.z * each, last = min(words, first + each);
   const int c = blockIdx.x * kFewShareCols + 4 * t;
   const bool mine = c < p.width;
-  float2 acc[kR][2];
+  float2 acc[kR / 2][4];                                   // tokens in pairs: their dL comes out of shared memory as the instruction wants it
 #pragma unroll
-  for (int r = 0; r < kR; ++r) acc[r][0] = acc[r][1] = make_float2(0.f, 0.f);
+  for (int r = 0; r < kR / 2; ++r)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[r][e] = make_float2(0.f, 0.f);
   for (int64_t v0 = first; v0 < last; v0 += 4 * kFewWords) {
     __syncthreads();
     for (int i = threadIdx.x; i < 4 * kFewWords * kR; i += kFewShareThreads) {
@@ -353,13 +363,17 @@ template <int kR> __global__ void __launch_bounds__(kFewShareThreads) vloss_few_
 #pragma unroll
       for (int i = 0; i < 8; ++i) f[i] = k + i < left ? *reinterpret_cast<const float4*>(at + (int64_t)(k + i) * p.width) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < 8; ++i) {
+        const float2 fx = make_float2(f[i].x, f[i].x), fy = make_float2(f[i].y, f[i].y), fz = make_float2(f[i].z, f[i].z), fw = make_float2(f[i].w, f[i].w);
 #pragma unroll
-        for (int r = 0; r < kR; ++r) {
-          const float d = ds[quarter][k + i][r];
-          acc[r][0] = fma2(make_float2(f[i].x, f[i].y), make_float2(d, d), acc[r][0]);
-          acc[r][1] = fma2(make_float2(f[i].z, f[i].w), make_float2(d, d), acc[r][1]);
+        for (int r = 0; r < kR / 2; ++r) {
+          const float2 d = *reinterpret_cast<const float2*>(&ds[quarter][k + i][2 * r]);
+          acc[r][0] = fma2(fx, d, acc[r][0]);
+          acc[r][1] = fma2(fy, d, acc[r][1]);
+          acc[r][2] = fma2(fz, d, acc[r][2]);
+          acc[r][3] = fma2(fw, d, acc[r][3]);
         }
+      }
     }
   }
   for (int part = 0; part < 4; ++part) {                   // threads 32 part .. + 31 of every quarter, the quarters in order
@@ -370,7 +384,8 @@ template <int kR> __global__ void __launch_bounds__(kFewShareThreads) vloss_few_
 #pragma unroll
         for (int r = 0; r < kR; ++r) {
           float4* to = reinterpret_cast<float4*>(&join[r][4 * (t & 31)]);
-          float4 s = make_float4(acc[r][0].x, acc[r][0].y, acc[r][1].x, acc[r][1].y);
+          const float2* a = acc[r / 2];
+          float4 s = r % 2 == 0 ? make_float4(a[0].x, a[1].x, a[2].x, a[3].x) : make_float4(a[0].y, a[1].y, a[2].y, a[3].y);
           if (q > 0) { s.x += to->x; s.y += to->y; s.z += to->z; s.w += to->w; }
           if (q < 3) { *to = s; continue; }
           if (!mine || r0 + r >= n) continue;
@@ -396,33 +411,43 @@ template <int kR> __global__ void __launch_bounds__(kFewOutThreads) vloss_few_ou
     const int r = i / kFewWords, k = i - r * kFewWords;
     ds[k][r] = r < n && k < left ? reinterpret_cast<const float*>(p.dl)[r * p.piece + first + k] : 0.f;
   }
-  float4 x[kR];
+  float2 x[kR / 2][4];                                     // tokens in pairs
 #pragma unroll
-  for (int r = 0; r < kR; ++r)
-    x[r] = r < n && c < p.width ? *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.x) + (int64_t)p.plan.rows[r] * p.x_stride + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int r = 0; r < kR; r += 2) {
+    float4 a[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      a[i] = r + i < n && c < p.width ? *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.x) + (int64_t)p.plan.rows[r + i] * p.x_stride + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+    x[r / 2][0] = make_float2(a[0].x, a[1].x);
+    x[r / 2][1] = make_float2(a[0].y, a[1].y);
+    x[r / 2][2] = make_float2(a[0].z, a[1].z);
+    x[r / 2][3] = make_float2(a[0].w, a[1].w);
+  }
   __syncthreads();
   if (c >= p.width) return;
   const float back = p.g_scale[1];
   float* out = reinterpret_cast<float*>(p.dw) + (v0 + first) * p.width + c;
   for (int k = 0; k < left; ++k) {
-    float2 a = make_float2(0.f, 0.f), b = a;
+    float2 a[4];
 #pragma unroll
-    for (int r = 0; r < kR; ++r) {
-      const float d = ds[k][r];
-      a = fma2(make_float2(x[r].x, x[r].y), make_float2(d, d), a);
-      b = fma2(make_float2(x[r].z, x[r].w), make_float2(d, d), b);
+    for (int e = 0; e < 4; ++e) a[e] = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int r = 0; r < kR / 2; ++r) {
+      const float2 d = *reinterpret_cast<const float2*>(&ds[k][2 * r]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) a[e] = fma2(x[r][e], d, a[e]);
     }
-    *reinterpret_cast<float4*>(out + (int64_t)k * p.width) = make_float4(a.x * back, a.y * back, b.x * back, b.y * back);
+    *reinterpret_cast<float4*>(out + (int64_t)k * p.width) = make_float4((a[0].x + a[0].y) * back, (a[1].x + a[1].y) * back, (a[2].x + a[2].y) * back, (a[3].x + a[3].y) * back);
   }
 }
 
-// Where they are used: fp32, rows of x and w in vectors of 16 bytes, few enough tokens that a pass over w for each 32 of them costs less
+// Where they are used (see use_few_forward too): fp32, rows of x and w in vectors of 16 bytes, few enough tokens that a pass over w for each 32 of them costs less
 // than what taking w apart does.
 static bool few_shape(int tokens, int width, int dtype) { return dtype == TKV_F32 && width % 8 == 0 && tokens > 0 && tokens <= 32; }
 static int few_rows(int tokens) { return tokens <= 8 ? 8 : tokens <= 16 ? 16 : 32; }
 template <int kR, int kMode> static int few_launch(const Vloss& p, const float* w, int64_t col0, int64_t cols, cudaStream_t st) {
   constexpr int kBytes = kFewStages * (kFewCols + kR) * kFewPitch * 4;
-  static_assert(4 * kR * kFewCols * 4 <= kBytes, "the quarters are joined where the stages were");
+  static_assert(8 * kR * kFewCols * 4 <= kBytes, "the parts are joined where the stages were");
   const int64_t tiles = (cols + kFewCols - 1) / kFewCols;
   static bool allowed[64] = {};
   int dev = 0;
@@ -688,6 +713,11 @@ int vloss_plan_rows(const Vloss& p, const int64_t* labels, int64_t ignore, float
   return vl_launch("tkv_vloss_forward", vloss_plan_kernel, dim3(1), kPlanThreads, st, labels, ignore, p.tokens, p.vocab, p.plan, loss, p.status);
 }
 static bool use_few(const Vloss& p) { return few_shape(p.tokens, p.width, p.dtype) && aligned16(p.w) && aligned16(p.x) && p.x_stride % 4 == 0 && (p.dw == nullptr || aligned16(p.dw)); }
+// Scoring of up to 64 tokens in two passes over a large w: us of 64 tokens, 162637 words, width 3488, in two passes 2230, on the tensor cores
+// 3600; of 60000 words, width 2048, 540 and 590; of 32768, width 1024, whose parts stay in L2, 186 and 135.
+static bool use_few_forward(const Vloss& p) {
+  return use_few(p) || (p.dtype == TKV_F32 && p.width % 8 == 0 && p.tokens <= 64 && p.vocab * p.width >= (int64_t)1 << 27 && aligned16(p.w) && aligned16(p.x) && p.x_stride % 4 == 0);
+}
 static bool use_tc(const Vloss& p) { return !use_few(p) && vloss_tc_shape(p.tokens, p.vocab, p.width, p.dtype) && aligned16(p.w) && (p.dw == nullptr || aligned16(p.dw)); }
 static int64_t pad256(int64_t bytes) { return vl_round(bytes, 256); }
 static int64_t any_forward_bytes(int tokens, int64_t vocab) { return (int64_t)tokens * ((vocab + kFewCols - 1) / kFewCols) * 8; }
@@ -737,12 +767,12 @@ extern "C" int tkv_vloss_forward(const void* x, int64_t x_stride, const void* w,
   p.mine = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + 512);
   void* rest = reinterpret_cast<char*>(p.mine) + pad256(tokens * 4);
   int rc;
-  if (tokens && use_tc(p)) {
+  if (tokens && !use_few_forward(p) && use_tc(p)) {
     rc = vloss_tc_forward(p, labels, ignore, loss, rest, st);
   } else {
     rc = vloss_plan_rows(p, labels, ignore, loss, st);
     p.part = reinterpret_cast<float2*>(rest);
-    const bool few = use_few(p);
+    const bool few = use_few_forward(p);
     const int tile = few ? kFewCols : kVgTile;
     p.tiles = (int)((vocab + tile - 1) / tile);
     if (rc == TKV_OK && tokens)
