@@ -81,7 +81,7 @@ def test_c_entries_refuse_before_any_launch(lib):
     need = lambda t=5, v=100, h=16, dt=0, back=0, dx=0: lib.tkv_vloss_workspace_bytes(t, v, h, dt, back, dx)  # noqa: E731
     assert need() > 0 and need(back=1, dx=1) > need(back=1) > 0
     assert need(t=-1) == need(v=0) == need(h=0) == need(dt=3) == need(t=(1 << 24) + 1) == need(v=(1 << 23) + 1) == need(h=65537) == -1
-    assert lib.tkv_vloss_plan_words(5) == 24
+    assert lib.tkv_vloss_plan_words(5) == 29
     fwd = lambda x=p, stride=16, t=5, v=100, h=16, red=1, loss=p, out=p, plan=p, ws=p, n=1 << 15, dt=0: lib.tkv_vloss_forward(  # noqa: E731
         x, stride, p, p, -100, t, v, h, red, loss, out, plan, ws, n, dt, None, None)
     assert fwd(x=None) == fwd(loss=None) == fwd(out=None) == fwd(plan=None) == fwd(ws=None) == -1 and b"NULL" in lib.tkv_last_error()

@@ -374,3 +374,37 @@ def test_some_tokens_of_a_large_fp32_head(t):
     logit = 1024 * 2.0 ** -23 * float((x.double().abs() @ w.double().abs().t()).max())
     again = linear_cross_entropy(wide[:, 1:1025], w, y, reduction="none")
     assert bool(((again - loss).abs() <= 2 * (2 * logit + 2.0 ** -20 * (2 + float(loss.detach().max())))).all())
+
+
+@pytest.mark.parametrize("dtype,t,v,h", [(BF, 1, 5000, 2048), (HF, 4, 9000, 2048), (BF, 5, 9000, 2048), (BF, 300, 9000, 2048), (SF, 20, 5000, 1024),
+                                         (SF, 40, 131072, 1024), (SF, 70, 5000, 1024)])
+def test_nearly_certain_tokens(dtype, t, v, h):
+    """Logits near 60 and 1 - p from 1e-5 to 1e-2: g (p - 1) of the label is as exact as the sum of the other words' p, whichever forms of the
+    products the forward and the backward pass took: their differences of 2^-20 of a logit act on the p of other words alone."""
+    g = torch.Generator(device="cuda").manual_seed(t + v)
+    w = (torch.randn(v, h, generator=g, device="cuda") * h ** -0.5).to(dtype)
+    y = torch.randint(0, v, (t,), generator=g, device="cuda")
+    rest = 10 ** (-5 + 3 * torch.rand(t, generator=g, device="cuda"))
+    base = torch.rand(t, h, generator=g, device="cuda") * w[y].float().sign() * 0.6       # products of one sign: what a cut is worst for
+    x = base
+    for _ in range(6):                                           # along w[y] until the label has the probability wanted
+        s = x.to(dtype).double() @ w.double().t()
+        others = torch.logsumexp(s.scatter(1, y[:, None], -float("inf")), 1)
+        gap = -torch.log(rest.double()) - (s.gather(1, y[:, None])[:, 0] - others)
+        x = x + (gap / (w[y].double() ** 2).sum(1))[:, None].float() * w[y].float()
+    x = x.to(dtype)
+    xd, wd = x.double(), w.double()
+    p = torch.softmax(xd @ wd.t(), 1)
+    own = torch.zeros_like(p).scatter_(1, y[:, None], 1.0)
+    tail = (p * (1 - own)).sum(1)
+    assert float(tail.max()) < 0.05 and float(tail.min()) > 1e-7
+    xg = x.clone().requires_grad_()
+    dx = torch.autograd.grad(linear_cross_entropy(xg, w, y, reduction="sum"), xg)[0]
+    want = -tail[:, None] * wd[y] + (p * (1 - own)) @ wd
+    half = torch.finfo(dtype).eps / 2
+    logit = h * 2.0 ** -23 * float((xd.abs() @ wd.abs().t()).max())
+    soft = 2 * logit + 2.0 ** -20
+    # the label's entry: the others' sum, off by soft, and p itself, a few roundings of numbers up to 1; the other entries: soft and one rounding
+    tol = (tail * 2 * soft + 2.0 ** -21)[:, None] * wd[y].abs() + (p * (1 - own)) @ wd.abs() * (2 * soft + half * 1.01) + want.abs() * half * 1.01
+    tol = tol + torch.finfo(dtype).smallest_normal + (2.0 ** -38 * wd.abs().sum(0) if dtype == HF else 0)
+    assert bool(((dx.double() - want).abs() <= tol).all()), float(((dx.double() - want).abs() / tol).max())

@@ -195,11 +195,11 @@ __global__ void __launch_bounds__(kVgThreads, 2) vloss_any_kernel(const __grid_c
     } else if (live) {
       if constexpr (kMode == kVgLogitGrad) {
         const float2 lse = p.l.plan.lse[row];
-        const float g = p.l.g[row];
+        const float g = p.l.g[row], own = p.l.plan.own[row];
         const int64_t label = (int64_t)p.l.plan.label[row] - p.col0;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (col[j] < p.n) reinterpret_cast<float*>(p.l.dl)[row * p.l.piece + col[j]] = g * (exp2f(fmaf(v[j] - lse.x, kLog2e, -lse.y)) - (col[j] == label ? 1.f : 0.f));
+          if (col[j] < p.n) reinterpret_cast<float*>(p.l.dl)[row * p.l.piece + col[j]] = g * (col[j] == label ? own : exp2f(fmaf(v[j] - lse.x, kLog2e, -lse.y)));
       } else if constexpr (kMode == kVgShare) {
         float* out = p.l.acc + ((int64_t)blockIdx.z * count + row) * p.n;
 #pragma unroll
@@ -321,10 +321,10 @@ template <int kR, int kMode> __global__ void __launch_bounds__(kFewThreads) vlos
         if (lane == 0) p.part[(int64_t)t * p.tiles + blockIdx.x] = make_float2(top, sum);
       } else {
         const float2 lse = p.plan.lse[t];
-        const float g = p.g[t];
+        const float g = p.g[t], own = p.plan.own[t];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-          if (c[h] < cols) reinterpret_cast<float*>(p.dl)[t * p.piece + c[h]] = g * (exp2f(fmaf(s[h] - lse.x, kLog2e, -lse.y)) - (c[h] == label ? 1.f : 0.f));
+          if (c[h] < cols) reinterpret_cast<float*>(p.dl)[t * p.piece + c[h]] = g * (c[h] == label ? own : exp2f(fmaf(s[h] - lse.x, kLog2e, -lse.y)));
       }
     }
   }
@@ -574,7 +574,9 @@ __global__ void __launch_bounds__(kJoinThreads) vloss_join_kernel(Vloss p, float
 #pragma unroll
     for (int w = 0; w < kJoinThreads / 32; ++w) sum += red[1][w];
     p.plan.lse[row] = make_float2(all, log2f(sum));
-    loss[p.plan.rows[row]] = p.plan.head[2] ? __int_as_float(0x7fffffff) : (all - p.mine[row]) + logf(sum);   // maximum and label first: they are often the same number
+    const float l = (all - p.mine[row]) + logf(sum);       // maximum and label first: they are often the same number
+    p.plan.own[row] = expm1f(-l);
+    loss[p.plan.rows[row]] = p.plan.head[2] ? __int_as_float(0x7fffffff) : l;
   }
 }
 
@@ -735,7 +737,7 @@ static int check_sizes(const char* what, int64_t tokens, int64_t vocab, int widt
 
 }  // namespace tkv
 
-extern "C" int64_t tkv_vloss_plan_words(int64_t tokens) { return 4 + 4 * (tokens > 0 ? tokens : 0); }
+extern "C" int64_t tkv_vloss_plan_words(int64_t tokens) { return 4 + 5 * (tokens > 0 ? tokens : 0); }
 
 extern "C" int64_t tkv_vloss_workspace_bytes(int64_t tokens, int64_t vocab, int width, int dtype, int backward, int want_dx) {
   using namespace tkv;

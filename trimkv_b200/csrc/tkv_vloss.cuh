@@ -14,12 +14,13 @@ namespace tkv {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kVlRowTile = 256;                            // workspaces hold whole tiles of rows
 
-// int32 words: [0] tokens that count, [1] is 1 if a label was out of range, [2] if a wait ran out, then lse (two fp32), rows and labels of the tokens that count.
+// int32 words: [0] tokens that count, [1] is 1 if a label was out of range, [2] if a wait ran out, then of the tokens that count lse (two fp32), rows,
+// labels, and p - 1 of the label (fp32), which the gradients take from here: near 1 - p = 0 it is lost in a logit made again by another form.
 struct VlossPlan {
-  int32_t* head; float2* lse; int32_t* rows; int32_t* label;
+  int32_t* head; float2* lse; int32_t* rows; int32_t* label; float* own;
 };
 inline __host__ __device__ VlossPlan vloss_plan(int32_t* p, int64_t tokens) {
-  return {p, reinterpret_cast<float2*>(p + 4), p + 4 + 2 * tokens, p + 4 + 3 * tokens};
+  return {p, reinterpret_cast<float2*>(p + 4), p + 4 + 2 * tokens, p + 4 + 3 * tokens, reinterpret_cast<float*>(p + 4 + 4 * tokens)};
 }
 
 // exp(x - top) of a logit or a maximum x <= top; nothing counts for nothing where there is no maximum yet.

@@ -425,12 +425,9 @@ vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             v[i + 1] = e.y;
           }
           if (label_here) {
-            float mine = 0.f;
+            const float mine = live ? g * p.l.plan.own[row] : 0.f;
 #pragma unroll
-            for (int i = c; i < c + 64; ++i) {
-              v[i] -= i == label ? g : 0.f;
-              mine = i == label ? v[i] : mine;
-            }
+            for (int i = c; i < c + 64; ++i) v[i] = i == label ? mine : v[i];
             if (sizeof(T) == 2 && (unsigned)(label - c) < 64u && label < left) p.l.rest[row] = mine - round_as<T>(mine);
           }
           if (!whole) {
@@ -784,6 +781,7 @@ template <typename T, int kR> __global__ void __launch_bounds__(kVwThreads, kVwC
   grid_dependency_wait();
   grid_launch_dependents();
   const int n = p.plan.head[0], lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (n == 0) return;                                      // nothing counts: nobody reads the parts
   const int chunks = (p.width + kVwCols - 1) / kVwCols, eights = chunks * 32;
   for (int i = threadIdx.x; i < kR * eights; i += kVwThreads) {
     const int r = i / eights, c = i - r * eights;

@@ -42,8 +42,9 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: tor
     shape of ``labels``), ``"sum"``, or ``"mean"`` over the labels that are not ``ignore_index`` (NaN where there are none, as in
     ``torch.nn.functional.cross_entropy``).  Ignored tokens cost nothing; their rows are not read and get a gradient of zeros.  A label
     outside the vocabulary makes its token's loss NaN, leaves the token out of the gradients and is recorded in ``status``
-    (``ops.new_status``).  Differentiable in hidden and weight; gradients are accumulated in fp32 and rounded once, with dL rounded to the
-    inputs' type for the products, as a product of stored logits would have it."""
+    (``ops.new_status``).  Differentiable in hidden and weight; gradients are accumulated in fp32 and rounded once, with the
+    gradients of the logits rounded to the inputs' type for the products (the label's, the largest of a token, counts in full for hidden,
+    and for weight up to 256 tokens)."""
     if reduction not in ops.VLOSS_REDUCTIONS:
         raise ValueError(f"reduction {reduction!r}: one of {sorted(ops.VLOSS_REDUCTIONS)}")
     if weight.dim() != 2 or hidden.dim() < 1 or hidden.shape[-1] != weight.shape[1] or labels.shape != hidden.shape[:-1]:
