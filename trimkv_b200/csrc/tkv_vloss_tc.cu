@@ -36,6 +36,9 @@ constexpr int kVtSum = 16;
 // In fp32 half as many.  RMS error of the gradients of 300 tokens, width 1024, 32768 words: 1.4e-6 (dx) and 1.0e-6 (dw) with 16, 7e-7 and 5.5e-7
 // with 8 (fp32 products on the CUDA cores: 1.0e-6 and 5.4e-7), 3.8e-7 and 3.0e-7 with 4; us of the pass 780, 805, 900.
 constexpr int kVtSum32 = 8;
+// Scoring up to kVtSumFew tokens too, whose losses average nothing: of 7 tokens, width 1024, the mean off by 6e-7 for 1.3e-6; us of 9 tokens,
+// 151936 words, width 2048, 126 for 118.  64 tokens would take 133 for 122, 256 tokens 162 for 157.
+constexpr int kVtSumFew = 32;
 // The label's entry of dL, g (p - 1), is most of its row, and what rounding it to 16 bits takes away does not average out: all of a row of
 // dx, and of dw's row of the label, is off by it.  It is kept (Vloss::rest) and goes back in where those rows are finished, w[label] rest into
 // dx, x rest into dw.  For dw every warp of 32 rows looks through the tokens' labels, up to kVtExact tokens and the first kVtExactHits of them:
@@ -917,6 +920,7 @@ int vloss_tc_forward(Vloss& l, const int64_t* labels, int64_t ignore, float* los
   }
   l.tiles = room.tiles;
   VtParams p = vt_params(l, room, base);
+  if (l.tokens <= kVtSumFew) p.sum_steps = kVtSum32;
   const int type = f32 ? TKV_BF16 : l.dtype;
   const void* w = f32 ? (const void*)(base + room.w) : l.w;
   CUtensorMap m[6];
