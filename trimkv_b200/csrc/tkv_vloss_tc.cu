@@ -30,15 +30,13 @@ constexpr int kVtGroup = 32;                               // row tiles that sha
 constexpr int kVtPairs = 74;
 constexpr int kVtHalf = kVtCols / 2;                       // columns of a warp of the epilogue
 // Stages that are added up in TMEM (1024 of the inner axis): the tensor cores cut what they add to an accumulator.  Relative error of a
-// logit of 40 whose products are all positive, width 4096, bf16: one sum -5.4e-6; sums of 16 stages -1.3e-6, of 8 -5.6e-7, of 4 -2.8e-7.
+// logit of 40 whose products are all positive, width 4096, bf16: one sum -5.4e-6; sums of 16 stages -1.3e-6, of 8 -5.6e-7, of 4 -2.8e-7
+// (before vt_up puts the mean of that back).
 // ms of 8192 x 151936 x 2048 with both gradients: 14.6, 14.7, 15.2, 16.4; us of 1500 tokens scored: 600, 620, 655, 710.
 constexpr int kVtSum = 16;
-// In fp32 half as many.  RMS error of the gradients of 300 tokens, width 1024, 32768 words: 1.4e-6 (dx) and 1.0e-6 (dw) with 16, 7e-7 and 5.5e-7
-// with 8 (fp32 products on the CUDA cores: 1.0e-6 and 5.4e-7), 3.8e-7 and 3.0e-7 with 4; us of the pass 780, 805, 900.
+// In fp32 half as many.  RMS error of the gradients of 300 tokens, width 1024, 32768 words, with 16 stages: 8.4e-7 (dx) and 8.9e-7 (dw), with 8
+// 4.6e-7 and 3.3e-7 (fp32 products on the CUDA cores: 1.0e-6 and 5.4e-7); us of the pass 785 to 840 both.
 constexpr int kVtSum32 = 8;
-// Scoring up to kVtSumFew tokens too, whose losses average nothing: of 7 tokens, width 1024, the mean off by 6e-7 for 1.3e-6; us of 9 tokens,
-// 151936 words, width 2048, 126 for 118.  64 tokens would take 133 for 122, 256 tokens 162 for 157.
-constexpr int kVtSumFew = 32;
 // The label's entry of dL, g (p - 1), is most of its row, and what rounding it to 16 bits takes away does not average out: all of a row of
 // dx, and of dw's row of the label, is off by it.  It is kept (Vloss::rest) and goes back in where those rows are finished, w[label] rest into
 // dx, x rest into dw.  For dw every warp of 32 rows looks through the tokens' labels, up to kVtExact tokens and the first kVtExactHits of them:
@@ -69,6 +67,12 @@ struct VtParams {
   int sum_steps;                                           // stages that are added up in TMEM
   const void* xc;                                          // the rows of x that count
 };
+
+// What a sum of so many stages is multiplied by.  Each of its 4 additions a stage cuts half a unit of what is there on average, 2^-24 / m of a
+// number of mantissa m, in the mean over m 2^-24 / (2 ln 2), and over a sum that grows evenly half of that for every addition.  The sum
+// of the means is known, so it is put back: it is the same for all tokens, and a mean over them would keep it.  (16 stages: 1.4e-6; measured on
+// products of one sign 1.3e-6.)  Mean loss of 300 tokens, widths 512 to 4096, off by 2 to 8e-7 of itself without, by 0.1 to 2e-7 with it.
+__device__ __forceinline__ float vt_up(int stages) { return 1.f + (float)(4 * stages) * (0.36067376f / 16777216.f); }
 
 // The parts that product c takes of A and of B; with one part there is product 5 alone.
 constexpr int kVtProducts = 6;
@@ -358,12 +362,13 @@ vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 #pragma unroll
             for (int c = 0; c < kVtHalf; c += 32) tmem_ld32(from + c, v + c);
           } else {
+            const float up = vt_up(min(p.sum_steps, steps - k));
 #pragma unroll
             for (int c = 0; c < kVtHalf; c += 16) {
               float u[16];
               tmem_ld16(from + c, u);
 #pragma unroll
-              for (int i = 0; i < 16; ++i) v[c + i] += u[i];
+              for (int i = 0; i < 16; ++i) v[c + i] = fmaf(u[i], up, v[c + i]);
             }
           }
         }
@@ -378,6 +383,7 @@ vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         if (kMode == kVtStats && row < tiles.n) p.l.part[(int64_t)row * p.l.tiles + 2 * (p.tile0 + t.col0 / p.cols) + (c0 > 0)] = make_float2(-INFINITY, 0.f);
         continue;
       }
+      const float up = kDirect ? vt_up(steps) : 1.f;       // (other sums have it already)
       if constexpr (kMode == kVtStats) {
         const bool live = row < tiles.n;
         const int label = live ? (int)(p.l.plan.label[row] - p.v0 - t.col0) - c0 : -1;
@@ -385,7 +391,7 @@ vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
           float mine = 0.f;
 #pragma unroll
           for (int i = 0; i < kVtHalf; ++i) mine = i == label ? v[i] : mine;
-          p.l.mine[row] = mine;
+          p.l.mine[row] = mine * up;
         }
         __syncwarp();
         if (left < kVtHalf) {
@@ -400,12 +406,13 @@ vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             top[j] = i + 4 + j < kVtHalf ? vt_max3(top[j], v[i + j], v[i + 4 + j]) : fmaxf(top[j], v[i + j]);
         }
         top[0] = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        top[0] *= up;
         const float at = top[0] == -INFINITY ? 0.f : top[0];
-        const float2 below = make_float2(-at, -at), one = make_float2(1.f, 1.f), by = make_float2(kLog2e, kLog2e), none = make_float2(-0.f, -0.f);
+        const float2 below = make_float2(-at, -at), one = make_float2(1.f, 1.f), ups = make_float2(up, up), by = make_float2(kLog2e, kLog2e), none = make_float2(-0.f, -0.f);
         float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
         for (int i = 0; i < kVtHalf; i += 2) {
-          const float2 d = fma2(fma2(make_float2(v[i], v[i + 1]), one, below), by, none);
+          const float2 d = fma2(fma2(make_float2(v[i], v[i + 1]), ups, below), by, none);
           sums[(i >> 1) & 1] = fma2(make_float2(exp2_weight(d.x), exp2_weight(d.y)), one, sums[(i >> 1) & 1]);
         }
         if (live) p.l.part[(int64_t)row * p.l.tiles + 2 * (p.tile0 + t.col0 / p.cols) + (c0 > 0)] = make_float2(top[0], (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y));
@@ -414,7 +421,7 @@ vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         const int label = live ? (int)(p.l.plan.label[row] - p.v0 - t.col0) - c0 : -1;
         const float2 lse = live ? p.l.plan.lse[row] : make_float2(0.f, 0.f);
         const float g = live ? p.l.g[row] : 0.f;
-        const float2 below = make_float2(-lse.x, -lse.x), one = make_float2(1.f, 1.f), by = make_float2(kLog2e, kLog2e), less = make_float2(-lse.y, -lse.y),
+        const float2 below = make_float2(-lse.x, -lse.x), ups = make_float2(up, up), by = make_float2(kLog2e, kLog2e), less = make_float2(-lse.y, -lse.y),
                      gg = make_float2(g, g), none = make_float2(-0.f, -0.f);
         const bool whole = (bool)__all_sync(0xffffffffu, live) && left >= kVtHalf, label_here = (bool)__any_sync(0xffffffffu, (unsigned)label < (unsigned)kVtHalf);
 #pragma unroll
@@ -422,7 +429,7 @@ vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
           if (c0 + c >= p.cols) break;
 #pragma unroll
           for (int i = c; i < c + 64; i += 2) {
-            const float2 d = fma2(fma2(make_float2(v[i], v[i + 1]), one, below), by, less);
+            const float2 d = fma2(fma2(make_float2(v[i], v[i + 1]), ups, below), by, less);
             const float2 e = fma2(make_float2(exp2_weight(d.x), exp2_weight(d.y)), gg, none);
             v[i] = e.x;
             v[i + 1] = e.y;
@@ -920,7 +927,6 @@ int vloss_tc_forward(Vloss& l, const int64_t* labels, int64_t ignore, float* los
   }
   l.tiles = room.tiles;
   VtParams p = vt_params(l, room, base);
-  if (l.tokens <= kVtSumFew) p.sum_steps = kVtSum32;
   const int type = f32 ? TKV_BF16 : l.dtype;
   const void* w = f32 ? (const void*)(base + room.w) : l.w;
   CUtensorMap m[6];
