@@ -626,7 +626,7 @@ __global__ void __launch_bounds__(kSumThreads) vloss_rows_grad_kernel(const floa
     const int x = more ? min(dx_cost / dw_cost, dw / fewer) : 0, rest = dw - x * fewer, last = rest % W;
     const int with = more ? (dx / W + 1) * dx_cost + (rest / W + (last > fewer)) * dw_cost : 0;
     const int without = dx / W * dx_cost + (x + rest / W + (last > 0)) * dw_cost;
-    const bool fits = s == 1 || ((int64_t)s * ((n + work.acc_rows - 1) / work.acc_rows * work.acc_rows) <= (int64_t)work.room * work.tokens && work.steps >= 8 * s);
+    const bool fits = s == 1 || (s <= work.most && (int64_t)s * ((n + work.acc_rows - 1) / work.acc_rows * work.acc_rows) <= (int64_t)work.room * work.tokens && work.steps >= 8 * s);
     cost[warp] = fits ? max(with, without) : INT32_MAX;
     extra[warp] = x;
   }
@@ -814,9 +814,9 @@ extern "C" int tkv_vloss_backward(const void* x, int64_t x_stride, const void* w
   const int64_t piece = any_piece(p.tokens, vocab);
   const int room = any_slots(p.tokens, width);
   const bool few = use_few(p);
-  const VlossWork work = few ? VlossWork{148, p.tokens <= 8 ? 8 : 16, 1, (width + kFewShareCols - 1) / kFewShareCols, 0, (int)((piece + kFewWords - 1) / kFewWords), kFewWords, room, p.tokens, dx != nullptr, false}
+  const VlossWork work = few ? VlossWork{148, p.tokens <= 8 ? 8 : 16, 1, (width + kFewShareCols - 1) / kFewShareCols, 0, (int)((piece + kFewWords - 1) / kFewWords), kFewWords, room, p.tokens, room, dx != nullptr, false}
                        : tc ? vloss_tc_work(p.tokens, vocab, width, dtype, dx != nullptr, dw != nullptr)
-                            : VlossWork{2 * 148, kVgTile, 1, (width + kVgTile - 1) / kVgTile, 0, (int)((piece + kVgK - 1) / kVgK), kVgK, room, p.tokens, dx != nullptr, false};
+                            : VlossWork{2 * 148, kVgTile, 1, (width + kVgTile - 1) / kVgTile, 0, (int)((piece + kVgK - 1) / kVgK), kVgK, room, p.tokens, room, dx != nullptr, false};
   int rc = vl_launch("tkv_vloss_backward", vloss_rows_grad_kernel, dim3(1), kSumThreads, st, grad, grad_stride, reduction, p.plan, work, g, scale,
                      reinterpret_cast<int*>(scale) + 2);
   if (rc != TKV_OK) return rc;

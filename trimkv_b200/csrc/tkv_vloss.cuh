@@ -51,8 +51,9 @@ inline int64_t vl_round(int64_t n, int64_t to) { return (n + to - 1) / to * to; 
 
 constexpr int kVlMaxSlots = 32;
 // What a launch of the gradients has to share out, for the choice of the shares of dx: workers, rows of a tile and what rows
-// of a share are rounded to, tiles of the width and of a piece, steps of a piece, elements of a step, room for shares of `tokens` rows.
-struct VlossWork { int workers, rows, acc_rows, ht, vt, steps, step, room, tokens; bool dx, dw; };
+// of a share are rounded to, tiles of the width and of a piece, steps of a piece, elements of a step, room for shares of `tokens` rows (fewer
+// rows that count leave room for more shares), and the most shares that the launches compute: the grid's, where it has a block for each.
+struct VlossWork { int workers, rows, acc_rows, ht, vt, steps, step, room, tokens, most; bool dx, dw; };
 
 int vloss_plan_rows(const Vloss& p, const int64_t* labels, int64_t ignore, float* loss, cudaStream_t st);
 

@@ -685,7 +685,7 @@ static int vt_slots(int tokens, int width) {
 VlossWork vloss_tc_work(int tokens, int64_t vocab, int width, int dtype, bool want_dx, bool want_dw) {
   const int64_t piece = vt_piece(tokens, vocab, width, dtype);
   return {kVtPairs, kVtRows, kVtRows, (width + kVtCols - 1) / kVtCols, (int)((piece + kVtRows - 1) / kVtRows), (int)(piece / kVtK), kVtK, vt_slots(tokens, width), (int)vt_rows(tokens),
-          want_dx, want_dw};
+          kVlMaxSlots, want_dx, want_dw};
 }
 
 // What lies where in a workspace.
