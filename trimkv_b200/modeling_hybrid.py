@@ -263,7 +263,8 @@ class HybridForCausalLM(HybridPreTrainedModel, TrimKVForCausalLM):
         ids = input_ids.reshape(-1) if live is None else input_ids[live]
         counts = [lengths[b] for b in rows]
         if scored:
-            normed = self.packed_hidden(ids, cache, None if width == 1 else counts, None if width == 1 else rows)
+            each = width == 1 and live is None            # a token of every request of the batch
+            normed = self.packed_hidden(ids, cache, None if each else counts, None if each else rows)
             loss = self._loss_of_packed(normed, live, labels, kwargs)
             if logits_to_keep is None:
                 return CausalLMOutputWithPast(loss=loss, past_key_values=cache)
