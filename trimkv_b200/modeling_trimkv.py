@@ -278,7 +278,9 @@ class RotaryEmbedding(nn.Module):
             rp, original_max_position_embeddings=rp.get("original_max_position_embeddings")
             or getattr(config, "original_max_position_embeddings", None)), getattr(config, "max_position_embeddings", None))
         self.config = config
-        self._inv_freq = 1.0 / (rope_theta_of(config) ** (torch.arange(0, d, 2, dtype=torch.int64).float() / d))
+        # from_pretrained builds models on "meta", where this table would have no values and, being no buffer, never get any
+        where = "cpu" if torch.get_default_device().type == "meta" else None
+        self._inv_freq = 1.0 / (rope_theta_of(config) ** (torch.arange(0, d, 2, dtype=torch.int64, device=where).float() / d))
         self._per_device = {}
 
     def inv_freq_on(self, device):

@@ -113,7 +113,8 @@ class RotaryPlan:
         self.original = p.get("original_max_position_embeddings") or max_positions
         if self.kind in ("llama3", "yarn", "longrope", "dynamic") and not self.original:
             raise ValueError(f"rope_type={self.kind!r} without original_max_position_embeddings")
-        f = self.base ** (-torch.arange(0, dims, 2, dtype=torch.float64) / max(dims, 1))
+        # On the CPU whatever the default device is: checkpoints are loaded into models that were built on "meta", where tables have no values.
+        f = self.base ** (-torch.arange(0, dims, 2, dtype=torch.float64, device="cpu") / max(dims, 1))
         self.factor = float(p.get("factor") or 1.0)
         self._tables = [getattr(self, f"_{self.kind}")(f, p, max_positions)]
         if self.kind == "longrope":
@@ -155,13 +156,13 @@ class RotaryPlan:
         if p.get("truncate", True):
             lo, hi = math.floor(lo), math.ceil(hi)
         lo, hi = max(lo, 0), min(hi, self.dims - 1)
-        ramp = ((torch.arange(self.dims // 2, dtype=torch.float64) - lo) / ((hi - lo) or 0.001)).clamp(0, 1)
+        ramp = ((torch.arange(self.dims // 2, dtype=torch.float64, device="cpu") - lo) / ((hi - lo) or 0.001)).clamp(0, 1)
         return f / factor * ramp + f * (1 - ramp)
 
     def _longrope(self, f, p, max_positions):
         out = []
         for key in ("short_factor", "long_factor"):
-            by = torch.tensor([float(x) for x in p[key]], dtype=torch.float64)
+            by = torch.tensor([float(x) for x in p[key]], dtype=torch.float64, device="cpu")
             if by.shape != f.shape:
                 raise ValueError(f"{key} has {by.numel()} numbers for {f.numel()} pairs")
             out.append(f / by)
