@@ -274,9 +274,10 @@ class RotaryEmbedding(nn.Module):
         super().__init__()
         rp = getattr(config, "rope_parameters", None) or {}
         d = rotary_dim_of(config)
+        # the configuration's own attribute (where Phi-3's checkpoints have it) goes before the key
         self.plan = RotaryPlan(d, rope_theta_of(config), dict(
-            rp, original_max_position_embeddings=rp.get("original_max_position_embeddings")
-            or getattr(config, "original_max_position_embeddings", None)), getattr(config, "max_position_embeddings", None))
+            rp, original_max_position_embeddings=getattr(config, "original_max_position_embeddings", None)
+            or rp.get("original_max_position_embeddings")), getattr(config, "max_position_embeddings", None))
         self.config = config
         # from_pretrained builds models on "meta", where this table would have no values and, being no buffer, never get any
         where = "cpu" if torch.get_default_device().type == "meta" else None

@@ -90,7 +90,8 @@ class RotaryPlan:
       that with ``mscale`` and ``mscale_all_dim``);
     * ``longrope``: divided by ``short_factor`` or, where the sequence is longer than the original length, ``long_factor`` (a number per
       pair); scaled by ``attention_factor`` (default ``sqrt(1 + ln(factor) / ln(original))``);
-    * ``dynamic``: for sequences longer than ``original`` the base grows with the length.
+    * ``dynamic``: for sequences longer than ``max_positions`` the base grows with the length (``original_max_position_embeddings`` counts
+      only where ``max_positions`` is not given, as in transformers).
 
     ``on(device, positions)`` is the table and the scale; where it depends on the length, that is the largest position plus one, and it is
     chosen on the device (recordable in a CUDA graph)."""
@@ -111,6 +112,8 @@ class RotaryPlan:
         if missing:
             raise ValueError(f"rope_type={self.kind!r} without {missing}")
         self.original = p.get("original_max_position_embeddings") or max_positions
+        if self.kind == "dynamic":
+            self.original = max_positions or self.original
         if self.kind in ("llama3", "yarn", "longrope", "dynamic") and not self.original:
             raise ValueError(f"rope_type={self.kind!r} without original_max_position_embeddings")
         # On the CPU whatever the default device is: checkpoints are loaded into models that were built on "meta", where tables have no values.
