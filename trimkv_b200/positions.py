@@ -9,6 +9,7 @@ import math
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import ops
 
@@ -16,14 +17,25 @@ LAYOUTS = {"half": 0, "pairs": 1}
 
 
 class _Rotary(torch.autograd.Function):
-    """The gradient of a turn is the turn back, with the same scale; its gradient in turn is the turn itself."""
+    """The gradient of a turn is the turn back, with the same scale; its gradient in turn is the turn itself.  A turn is linear: tangents are
+    turned like what they belong to."""
 
     @staticmethod
     def forward(ctx, q, k, positions, freq, layout, inverse, scale):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(positions, freq)
+        ctx.save_for_forward(positions, freq)
         ctx.how = layout, inverse, scale
+        ctx.shapes = tuple(None if t is None else t.shape for t in (q, k))
         return ops.rotary(q, k, positions, freq, layout, inverse, scale)
+
+    @staticmethod
+    def jvp(ctx, *tangents):
+        positions, freq = ctx.saved_tensors
+        turn, given = _Rotary.apply if torch.is_grad_enabled() else ops.rotary, tangents[0] if tangents[0] is not None else tangents[1]
+        turned = turn(*tangents[:2], positions, freq, *ctx.how)
+        # where only one of the two has a tangent, the other's is zero (an output's may not be left out)
+        return tuple(given.new_zeros(shape) if out is None and shape is not None else out for out, shape in zip(turned, ctx.shapes))
 
     @staticmethod
     def backward(ctx, dq, dk):
@@ -36,6 +48,10 @@ class _Rotary(torch.autograd.Function):
         return dq, dk, None, None, None, None, None
 
 
+def _has_tangent(t: torch.Tensor) -> bool:
+    return forward_ad.unpack_dual(t).tangent is not None
+
+
 def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, freq: torch.Tensor, *, layout: str = "half",
                  scale: float = 1.0) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """``q [B, Hq, S, D]`` and ``k [B, Hkv, S, D]`` (or None) turned by their positions, as new tensors of the same type.
@@ -44,7 +60,7 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     position) as a high and a low part; the first ``2 * pairs`` elements of a head turn and are multiplied by ``scale``, the others are
     copied.  ``layout``: ``"half"`` turns element i with ``pairs + i``, ``"pairs"`` element 2i with 2i + 1.  Angles are exact to fp32 at
     any position, and a result is rounded once.  Any strides; the results are stored token by token (``[B, S, H, D]`` in memory).
-    Differentiable in q and k."""
+    Differentiable in q and k, in either mode."""
     how = LAYOUTS.get(layout)
     if how is None:
         raise ValueError(f"layout {layout!r}: one of {sorted(LAYOUTS)}")
@@ -66,7 +82,7 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
         raise ValueError(f"frequencies {freq.dtype} {tuple(pairs)}: want contiguous fp32 [pairs, 2] with at most {d // 2} pairs")
     if positions.device != device or freq.device != device:
         raise ValueError(f"queries on {device}, positions on {positions.device}, frequencies on {freq.device}")
-    if (q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled():
+    if ((q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled()) or _has_tangent(q) or (k is not None and _has_tangent(k)):
         return _Rotary.apply(q, k, positions, freq, how, False, float(scale))
     return ops.rotary(q, k, positions, freq, how, False, float(scale))
 
