@@ -66,6 +66,17 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: tor
     return loss.view(labels.shape) if reduction == "none" and labels.dim() != 1 else loss
 
 
+def logits_cross_entropy(logits: torch.Tensor, labels: torch.Tensor, *, ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
+    """:func:`linear_cross_entropy` where the logits ``[..., V]`` are there already, in elementary operations on any device: the same loss and
+    reductions, ignored rows not counted whatever is in them, NaN for labels outside the vocabulary."""
+    live = labels != ignore_index
+    counts = live & (labels >= 0) & (labels < logits.shape[-1])
+    z = logits.to(torch.promote_types(logits.dtype, torch.float32)).masked_fill(~counts[..., None], 0.0)
+    at = labels.long().masked_fill(~counts, 0)
+    loss = (z.logsumexp(-1) - z.gather(-1, at[..., None])[..., 0]).masked_fill(~live, 0.0).masked_fill(live & ~counts, float("nan"))
+    return loss if reduction == "none" else loss.sum() if reduction == "sum" else loss.sum() / counts.sum()
+
+
 class _ExpertBalance(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, choice, valid):

@@ -198,6 +198,9 @@ class HybridForCausalLM(HybridPreTrainedModel, TrimKVForCausalLM):
         w = self.lm_head.weight
         return F.linear(normed, w) if w.dtype == torch.float32 else torch.mm(normed, w.t(), out_dtype=torch.float32)
 
+    def _head_is_its_weight(self) -> bool:
+        return True                                       # see head: nothing else of the module is read
+
     @torch.no_grad()
     def forward_packed(self, ids: torch.Tensor, cache: HybridStateCache, lengths: Optional[Sequence[int]],
                        rows: Optional[Sequence[int]] = None, want: Optional[Sequence[int]] = None,

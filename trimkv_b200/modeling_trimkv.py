@@ -31,7 +31,7 @@ from transformers.modeling_outputs import BaseModelOutputWithPast, CausalLMOutpu
 
 from .attn import get_attention_interface, register_with_transformers
 from .cache_utils import TrimKVCache
-from .losses import linear_cross_entropy
+from .losses import linear_cross_entropy, logits_cross_entropy
 from .positions import RotaryPlan, apply_rotary
 
 register_with_transformers()
@@ -490,14 +490,25 @@ class TrimKVForCausalLM(TrimKVPreTrainedModel, GenerationMixin):
     def _fused_decode_covers(self) -> bool:
         return self.lm_head.weight.dtype in self.decode_dtypes and self._decode_step_cls().supports(self)
 
-    def loss_of(self, hidden_states, labels, num_items_in_batch=None, ignore_index=-100, shift_labels=None):
+    def _head_is_its_weight(self) -> bool:
+        """Whether the LM head is the product with ``lm_head.weight`` and nothing else: no bias, no other module in its place (an adapter, a
+        parametrization), no hooks, no weight of another tensor class."""
+        h = self.lm_head
+        return (type(h) is nn.Linear and h.bias is None and type(h.weight) in (nn.Parameter, torch.Tensor) and "forward" not in h.__dict__
+                and not (h._forward_hooks or h._forward_pre_hooks or h._backward_hooks or h._backward_pre_hooks))
+
+    def loss_of(self, hidden_states, labels, num_items_in_batch=None, ignore_index=-100, shift_labels=None, logits=None):
         """Cross entropy of ``hidden_states [B, S, H]`` against the LM head, each token with the label that follows it (``labels [B, S]``;
-        ``shift_labels``: already moved), by ``losses.linear_cross_entropy``: no logits are made.  ``num_items_in_batch``: the sum over
-        the labels divided by that, as transformers' losses have it; else their mean."""
+        ``shift_labels``: already moved), by ``losses.linear_cross_entropy``: no logits are made.  A head that is more than its weight is
+        called, and the loss taken from its logits (``logits``: those of all places, where they are there already).
+        ``num_items_in_batch``: the sum over the labels divided by that, as transformers' losses have it; else their mean."""
         if shift_labels is None:
             shift_labels = F.pad(labels[:, 1:], (0, 1), value=ignore_index)
-        loss = linear_cross_entropy(hidden_states, self.lm_head.weight, shift_labels, ignore_index=ignore_index,
-                                    reduction="mean" if num_items_in_batch is None else "sum")
+        how = dict(ignore_index=ignore_index, reduction="mean" if num_items_in_batch is None else "sum")
+        if logits is None and self._head_is_its_weight():
+            loss = linear_cross_entropy(hidden_states, self.lm_head.weight, shift_labels, **how)
+        else:
+            loss = logits_cross_entropy(self.lm_head(hidden_states) if logits is None else logits, shift_labels, **how)
         return loss if num_items_in_batch is None else loss / num_items_in_batch
 
     def forward(self, input_ids=None, attention_mask=None, position_ids=None, past_key_values=None, inputs_embeds=None,
@@ -516,13 +527,15 @@ class TrimKVForCausalLM(TrimKVPreTrainedModel, GenerationMixin):
         out = self.model(input_ids=input_ids, attention_mask=attention_mask, position_ids=position_ids,
                          past_key_values=past_key_values, inputs_embeds=inputs_embeds, use_cache=use_cache,
                          cache_position=cache_position)
-        loss = logits = None
+        loss = logits = whole = None
         if scored is not None:
-            loss = self.loss_of(out.last_hidden_state, labels, **{k: kwargs[k] for k in ("num_items_in_batch", "ignore_index", "shift_labels")
-                                                                  if kwargs.get(k) is not None})
+            if not self._head_is_its_weight():
+                whole = self.lm_head(out.last_hidden_state)            # once, for the loss and the logits
+            loss = self.loss_of(out.last_hidden_state, labels, logits=whole, **{
+                k: kwargs[k] for k in ("num_items_in_batch", "ignore_index", "shift_labels") if kwargs.get(k) is not None})
         if logits_to_keep is not None:
             sl = slice(-logits_to_keep, None) if isinstance(logits_to_keep, int) else logits_to_keep
-            logits = self.lm_head(out.last_hidden_state[:, sl, :])
+            logits = self.lm_head(out.last_hidden_state[:, sl, :]) if whole is None else whole[:, sl, :]
         res = CausalLMOutputWithPast(loss=loss, logits=logits, past_key_values=out.past_key_values)
         res.last_hidden_state = out.last_hidden_state
         return res
