@@ -6,6 +6,7 @@ from torch import nn
 from torch.nn.utils import parametrize
 
 import trimkv_b200 as t
+from tests.host_emulation import on_device
 from trimkv_b200 import modeling_trimkv
 from trimkv_b200.losses import logits_cross_entropy
 
@@ -129,7 +130,7 @@ def test_a_plain_head_takes_the_weight(monkeypatch):
         return hidden.sum()
     monkeypatch.setattr(modeling_trimkv, "linear_cross_entropy", fused)
     model = _model()
-    hidden = torch.zeros(2, 5, 128)
+    hidden = on_device(torch.zeros(2, 5, 128))
     model.loss_of(hidden, torch.ones(2, 5, dtype=torch.int64))
     assert seen == [((2, 5, 128), (131, 128), dict(ignore_index=-100, reduction="mean"))]
 

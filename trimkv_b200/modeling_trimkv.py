@@ -497,15 +497,19 @@ class TrimKVForCausalLM(TrimKVPreTrainedModel, GenerationMixin):
         return (type(h) is nn.Linear and h.bias is None and type(h.weight) in (nn.Parameter, torch.Tensor) and "forward" not in h.__dict__
                 and not (h._forward_hooks or h._forward_pre_hooks or h._backward_hooks or h._backward_pre_hooks))
 
+    def _fused_loss_covers(self, hidden_states) -> bool:
+        """Whether ``losses.linear_cross_entropy`` has a form for the loss of these rows: on CUDA, of a type that the kernels take."""
+        return hidden_states.is_cuda and hidden_states.dtype in (torch.bfloat16, torch.float16, torch.float32) and self._head_is_its_weight()
+
     def loss_of(self, hidden_states, labels, num_items_in_batch=None, ignore_index=-100, shift_labels=None, logits=None):
         """Cross entropy of ``hidden_states [B, S, H]`` against the LM head, each token with the label that follows it (``labels [B, S]``;
-        ``shift_labels``: already moved), by ``losses.linear_cross_entropy``: no logits are made.  A head that is more than its weight is
-        called, and the loss taken from its logits (``logits``: those of all places, where they are there already).
+        ``shift_labels``: already moved), by ``losses.linear_cross_entropy``: no logits are made.  A head that is more than its weight, on
+        the CPU any head, is called, and the loss taken from its logits (``logits``: those of all places, where they are there already).
         ``num_items_in_batch``: the sum over the labels divided by that, as transformers' losses have it; else their mean."""
         if shift_labels is None:
             shift_labels = F.pad(labels[:, 1:], (0, 1), value=ignore_index)
         how = dict(ignore_index=ignore_index, reduction="mean" if num_items_in_batch is None else "sum")
-        if logits is None and self._head_is_its_weight():
+        if logits is None and self._fused_loss_covers(hidden_states):
             loss = linear_cross_entropy(hidden_states, self.lm_head.weight, shift_labels, **how)
         else:
             loss = logits_cross_entropy(self.lm_head(hidden_states) if logits is None else logits, shift_labels, **how)
@@ -529,7 +533,7 @@ class TrimKVForCausalLM(TrimKVPreTrainedModel, GenerationMixin):
                          cache_position=cache_position)
         loss = logits = whole = None
         if scored is not None:
-            if not self._head_is_its_weight():
+            if not self._fused_loss_covers(out.last_hidden_state):
                 whole = self.lm_head(out.last_hidden_state)            # once, for the loss and the logits
             loss = self.loss_of(out.last_hidden_state, labels, logits=whole, **{
                 k: kwargs[k] for k in ("num_items_in_batch", "ignore_index", "shift_labels") if kwargs.get(k) is not None})
