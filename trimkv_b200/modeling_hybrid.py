@@ -307,7 +307,8 @@ class HybridForCausalLM(HybridPreTrainedModel, TrimKVForCausalLM):
         if target is None:
             target = F.pad(labels[:, 1:], (0, 1), value=ignore)
             if live is not None:                          # what follows is padding
-                target = target.masked_fill(~F.pad(live[:, 1:], (0, 1), value=False), ignore)
+                target = target.to(live.device).masked_fill(~F.pad(live[:, 1:], (0, 1), value=False), ignore)
+        target = target.to(normed.device)
         target = target.reshape(-1) if live is None else target[live]
         return self.loss_of(normed, None, kwargs.get("num_items_in_batch"), ignore, target)
 

@@ -508,6 +508,7 @@ class TrimKVForCausalLM(TrimKVPreTrainedModel, GenerationMixin):
         ``num_items_in_batch``: the sum over the labels divided by that, as transformers' losses have it; else their mean."""
         if shift_labels is None:
             shift_labels = F.pad(labels[:, 1:], (0, 1), value=ignore_index)
+        shift_labels = shift_labels.to(hidden_states.device)             # labels of a data loader may still be on the CPU
         how = dict(ignore_index=ignore_index, reduction="mean" if num_items_in_batch is None else "sum")
         if logits is None and self._fused_loss_covers(hidden_states):
             loss = linear_cross_entropy(hidden_states, self.lm_head.weight, shift_labels, **how)
