@@ -655,12 +655,24 @@ static_assert(kSumThreads / 32 == kVlMaxSlots, "a warp for every number of share
 
 constexpr int kDxThreads = 256;
 
+// Where a wait ran out, tiles of dw are missing: all of it becomes NaN.
+template <typename T> __device__ __forceinline__ void vl_spoil(const VlossPlan& plan, T* dw, int64_t n) {
+  if (dw == nullptr || plan.head[2] == 0) return;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) dw[i] = from_f32<T>(__int_as_float(0x7fffffff));
+}
+template <typename T> __global__ void __launch_bounds__(kDxThreads) vloss_spoil_kernel(Vloss p) {
+  grid_dependency_wait();
+  grid_launch_dependents();
+  vl_spoil(p.plan, reinterpret_cast<T*>(p.dw), p.vocab * p.width);
+}
+
 // dx: the shares of a row added up in order, in the caller's type and place; zeros for tokens that do not count.  The rows of the plan are
 // in order, so a token finds itself there by halving.
 template <typename T> __global__ void __launch_bounds__(kDxThreads) vloss_dx_kernel(Vloss p, T* dx) {
   grid_dependency_wait();
   grid_launch_dependents();
   const int t = blockIdx.x, n = p.plan.head[0];
+  vl_spoil(p.plan, reinterpret_cast<T*>(p.dw), p.vocab * p.width);
   int lo = 0, hi = n;
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
@@ -709,6 +721,11 @@ template <typename... A> static int vl_launch(const char* what, void (*kernel)(A
   cudaError_t e = launch_pdl(kernel, grid, dim3(threads), 0, st, args...);
   if (e != cudaSuccess) return fail(TKV_ERR_LAUNCH, "%s: %s", what, cudaGetErrorString(e));
   return check_launch(what);
+}
+
+template <typename T> static int vloss_finish(const Vloss& p, void* dx, cudaStream_t st) {
+  if (dx) return vl_launch("tkv_vloss_backward", vloss_dx_kernel<T>, dim3((unsigned)p.tokens), kDxThreads, st, p, (T*)dx);
+  return vl_launch("tkv_vloss_backward", vloss_spoil_kernel<T>, dim3(148), kDxThreads, st, p);
 }
 
 int vloss_plan_rows(const Vloss& p, const int64_t* labels, int64_t ignore, float* loss, cudaStream_t st) {
@@ -830,8 +847,7 @@ extern "C" int tkv_vloss_backward(const void* x, int64_t x_stride, const void* w
     rc = dtype == TKV_F32 ? vloss_any_backward<float>(p, dx != nullptr, room, few, st)
                           : dtype == TKV_BF16 ? vloss_any_backward<__nv_bfloat16>(p, dx != nullptr, room, false, st) : vloss_any_backward<__half>(p, dx != nullptr, room, false, st);
   }
-  if (rc != TKV_OK || dx == nullptr) return rc;
-  if (dtype == TKV_F32) return vl_launch("tkv_vloss_backward", vloss_dx_kernel<float>, dim3((unsigned)tokens), kDxThreads, st, p, (float*)dx);
-  if (dtype == TKV_BF16) return vl_launch("tkv_vloss_backward", vloss_dx_kernel<__nv_bfloat16>, dim3((unsigned)tokens), kDxThreads, st, p, (__nv_bfloat16*)dx);
-  return vl_launch("tkv_vloss_backward", vloss_dx_kernel<__half>, dim3((unsigned)tokens), kDxThreads, st, p, (__half*)dx);
+  if (rc != TKV_OK) return rc;
+  if (dtype == TKV_F32) return vloss_finish<float>(p, dx, st);
+  return dtype == TKV_BF16 ? vloss_finish<__nv_bfloat16>(p, dx, st) : vloss_finish<__half>(p, dx, st);
 }

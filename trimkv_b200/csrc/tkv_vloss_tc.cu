@@ -15,7 +15,7 @@
 // is left out is below 2^-24 of a product.  w is taken apart a piece of the vocabulary at a time, so that its parts stay in L2.
 //
 // Copies of both CTAs complete on the even CTA's barriers; it issues the products; their completion is told to both.  Every wait is
-// bounded; a CTA whose wait runs out records TKV_DEV_TIMEOUT, in the plan too (losses and dx become NaN), and tells its neighbour; both
+// bounded; a CTA whose wait runs out records TKV_DEV_TIMEOUT, in the plan too (losses, dx and dw become NaN), and tells its neighbour; both
 // drain and free their TMEM.
 #include <cuda.h>
 #include "tkv_vloss.cuh"

@@ -887,7 +887,7 @@ def vloss_backward(x, w, plan, grad, reduction: int, want_dx: bool, want_dw: boo
         check(lib().tkv_vloss_backward(x.data_ptr(), x.stride(0), w.data_ptr(), plan.data_ptr(), grad.data_ptr(),
                                        grad.stride(0) if grad.dim() else 0, reduction, t, v, h, _ptr(dx), _ptr(dw), ws.data_ptr(), need, dt,
                                        _ptr(status), _stream(x)), "tkv_vloss_backward")
-    _count(2 + want_dx + want_dw)
+    _count(3 + want_dw)
     return dx, dw
 
 
