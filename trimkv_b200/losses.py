@@ -34,6 +34,10 @@ class _LinearCrossEntropy(torch.autograd.Function):
         return dx, dw, None, None, None, None
 
 
+def _autocast(t: torch.Tensor) -> torch.Tensor:
+    return t.to(torch.get_autocast_dtype(t.device.type)) if t.is_floating_point() and t.dtype != torch.float64 else t
+
+
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, *, ignore_index: int = -100,
                          reduction: str = "mean", status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``cross_entropy(hidden @ weight.T, labels)`` in fp32 without the logits: ``hidden [..., H]``, ``weight [V, H]``, ``labels [...]``.
@@ -44,13 +48,16 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: tor
     outside the vocabulary makes its token's loss NaN, leaves the token out of the gradients and is recorded in ``status``
     (``ops.new_status``).  Differentiable in hidden and weight; gradients are accumulated in fp32 and rounded once, with the
     gradients of the logits rounded to the inputs' type for the products (the label's, the largest of a token, counts in full for hidden,
-    and for weight up to 256 tokens)."""
+    and for weight up to 256 tokens).  Under autocast hidden and weight are taken in its type, as
+    ``torch.nn.functional.linear`` takes them."""
     if reduction not in ops.VLOSS_REDUCTIONS:
         raise ValueError(f"reduction {reduction!r}: one of {sorted(ops.VLOSS_REDUCTIONS)}")
     if weight.dim() != 2 or hidden.dim() < 1 or hidden.shape[-1] != weight.shape[1] or labels.shape != hidden.shape[:-1]:
         raise ValueError(f"hidden {tuple(hidden.shape)}, weight {tuple(weight.shape)}, labels {tuple(labels.shape)}")
     if weight.shape[0] == 0 or weight.shape[1] == 0:
         raise ValueError(f"an empty weight {tuple(weight.shape)}")
+    if torch.is_autocast_enabled(hidden.device.type):
+        hidden, weight = (_autocast(t) for t in (hidden, weight))
     ops.dtype_code(hidden.dtype)
     if weight.dtype != hidden.dtype:
         raise TypeError(f"hidden rows in {hidden.dtype}, weight in {weight.dtype}")
