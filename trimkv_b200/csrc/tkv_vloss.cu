@@ -61,6 +61,7 @@ struct VgProduct {
   int64_t m, n, k;                                         // where the token axis is one of them, at most *count of it
   const int32_t* count;
   int token_axis;                                          // 0: m, 2: k
+  int mt;                                                  // tiles along m; blockIdx.x goes through them, then along n
   int64_t col0;                                            // column 0 is this of the vocabulary
   int split; int64_t split_len;                            // kVgShare: most shares; the whole of k
   int more;                                                // shares are added to what is there
@@ -119,7 +120,8 @@ __global__ void __launch_bounds__(kVgThreads, 2) vloss_any_kernel(const __grid_c
   grid_launch_dependents();
   const int64_t count = *p.count;
   const int64_t m = p.token_axis == 0 ? min(p.m, count) : p.m, kend = p.token_axis == 2 ? min(p.k, count) : p.k;
-  const int64_t m0 = (int64_t)blockIdx.x * kVgTile, n0 = (int64_t)blockIdx.y * kVgTile;
+  const int n_tile = (int)blockIdx.x / p.mt;
+  const int64_t m0 = (int64_t)((int)blockIdx.x - n_tile * p.mt) * kVgTile, n0 = (int64_t)n_tile * kVgTile;
   int64_t split_len = p.split_len;
   if (kMode == kVgShare) {                                 // as many shares as the device chose, of the grid's
     const int64_t slots = *p.l.slots;
@@ -191,7 +193,7 @@ __global__ void __launch_bounds__(kVgThreads, 2) vloss_any_kernel(const __grid_c
       for (int j = 0; j < 8; ++j) sum += col[j] < p.n ? vl_weight(v[j], top) : 0.f;
 #pragma unroll
       for (int o = 8; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (live && tx == 0) p.l.part[row * p.l.tiles + blockIdx.y] = make_float2(top, sum);
+      if (live && tx == 0) p.l.part[row * p.l.tiles + n_tile] = make_float2(top, sum);
     } else if (live) {
       if constexpr (kMode == kVgLogitGrad) {
         const float2 lse = p.l.plan.lse[row];
@@ -481,10 +483,12 @@ static int few_share_launch(const Vloss& p, const float* w, int64_t words, int r
   return e == cudaSuccess ? check_launch("tkv_vloss") : fail(TKV_ERR_LAUNCH, "tkv_vloss: %s", cudaGetErrorString(e));
 }
 
-template <typename TA, bool kAK, typename TB, bool kBK, int kMode, typename TOut> static int vg_launch(const VgProduct& p, cudaStream_t st) {
+template <typename TA, bool kAK, typename TB, bool kBK, int kMode, typename TOut> static int vg_launch(VgProduct p, cudaStream_t st) {
+  // (2^43 logits are below 2^30 tiles; the other products have fewer)
   const int64_t mt = (p.m + kVgTile - 1) / kVgTile, nt = (p.n + kVgTile - 1) / kVgTile;
-  if (nt > 65535 || mt > INT32_MAX) return fail(TKV_ERR_UNSUPPORTED, "tkv_vloss: %lld x %lld tiles", (long long)mt, (long long)nt);
-  cudaError_t e = launch_pdl(vloss_any_kernel<TA, kAK, TB, kBK, kMode, TOut>, dim3((unsigned)mt, (unsigned)nt, p.split), dim3(kVgThreads), 0, st, p);
+  if (mt * nt > INT32_MAX) return fail(TKV_ERR_UNSUPPORTED, "tkv_vloss: %lld x %lld tiles", (long long)mt, (long long)nt);
+  p.mt = (int)mt;
+  cudaError_t e = launch_pdl(vloss_any_kernel<TA, kAK, TB, kBK, kMode, TOut>, dim3((unsigned)(mt * nt), 1, p.split), dim3(kVgThreads), 0, st, p);
   if (e != cudaSuccess) return fail(TKV_ERR_LAUNCH, "tkv_vloss: %s", cudaGetErrorString(e));
   return check_launch("tkv_vloss");
 }
