@@ -738,12 +738,16 @@ int vloss_plan_rows(const Vloss& p, const int64_t* labels, int64_t ignore, float
 static bool use_few(const Vloss& p) { return few_shape(p.tokens, p.width, p.dtype) && aligned16(p.w) && aligned16(p.x) && p.x_stride % 4 == 0 && (p.dw == nullptr || aligned16(p.dw)); }
 // Scoring of up to 64 tokens in two passes over a large w: us of 64 tokens, 162637 words, width 3488, in two passes 2230, on the tensor cores
 // 3600; of 60000 words, width 2048, 540 and 590; of 32768, width 1024, whose parts stay in L2, 186 and 135.
+constexpr int kFewForward = 64;
 static bool use_few_forward(const Vloss& p) {
-  return use_few(p) || (p.dtype == TKV_F32 && p.width % 8 == 0 && p.tokens <= 64 && p.vocab * p.width >= (int64_t)1 << 27 && aligned16(p.w) && aligned16(p.x) && p.x_stride % 4 == 0);
+  return use_few(p) || (p.dtype == TKV_F32 && p.width % 8 == 0 && p.tokens <= kFewForward && p.vocab * p.width >= (int64_t)1 << 27 && aligned16(p.w) && aligned16(p.x) && p.x_stride % 4 == 0);
 }
 static bool use_tc(const Vloss& p) { return !use_few(p) && vloss_tc_shape(p.tokens, p.vocab, p.width, p.dtype) && aligned16(p.w) && (p.dw == nullptr || aligned16(p.dw)); }
 static int64_t pad256(int64_t bytes) { return vl_round(bytes, 256); }
-static int64_t any_forward_bytes(int tokens, int64_t vocab) { return (int64_t)tokens * ((vocab + kFewCols - 1) / kFewCols) * 8; }
+static int64_t any_forward_bytes(int tokens, int64_t vocab, int dtype) {
+  const int tile = dtype == TKV_F32 && tokens <= kFewForward ? kFewCols : kVgTile;   // the narrower tiles where they may run
+  return (int64_t)tokens * ((vocab + tile - 1) / tile) * 8;
+}
 static int64_t any_backward_bytes(int tokens, int64_t vocab, int width, bool dx) {
   const int64_t piece = any_piece(tokens, vocab);
   return pad256((int64_t)tokens * piece * 4) + (dx ? (int64_t)any_slots(tokens, width) * tokens * width * 4 : 0);
@@ -764,7 +768,7 @@ extern "C" int64_t tkv_vloss_workspace_bytes(int64_t tokens, int64_t vocab, int 
   using namespace tkv;
   if (check_sizes("tkv_vloss_workspace_bytes", tokens, vocab, width, width, dtype) != TKV_OK) return -1;
   const int t = (int)tokens;
-  int64_t n = backward ? any_backward_bytes(t, vocab, width, want_dx != 0) : any_forward_bytes(t, vocab);
+  int64_t n = backward ? any_backward_bytes(t, vocab, width, want_dx != 0) : any_forward_bytes(t, vocab, dtype);
   if (vloss_tc_shape(t, vocab, width, dtype)) {            // which form runs is known with the addresses: room for either
     const int64_t tc = vloss_tc_bytes(t, vocab, width, dtype, backward != 0, want_dx != 0);
     n = n > tc ? n : tc;

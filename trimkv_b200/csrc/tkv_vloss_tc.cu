@@ -688,6 +688,8 @@ VlossWork vloss_tc_work(int tokens, int64_t vocab, int width, int dtype, bool wa
           kVlMaxSlots, want_dx, want_dw};
 }
 
+static bool vw_shape(int tokens, int width, int dtype) { return dtype != TKV_F32 && tokens <= kVwTokens && (int64_t)tokens * width <= kVwValues; }
+
 // What lies where in a workspace.
 struct VtRoom {
   int64_t rows, piece, xc, w, dl, acc, part, bytes;        // bytes from the start
@@ -705,7 +707,7 @@ struct VtRoom {
     dl = w + (parts == 3 ? pad(3 * piece * width * 2) : 0);
     acc = dl + (backward ? pad(parts * rows * piece * 2) : 0);
     part = acc + (backward && dx ? pad((int64_t)vt_slots(tokens, width) * rows * width * 4) : 0);
-    bytes = part + (backward ? 0 : pad((int64_t)tokens * (tiles > kVwGrid ? tiles : kVwGrid) * 8));
+    bytes = part + (backward ? 0 : pad((int64_t)tokens * (vw_shape(tokens, width, dtype) && kVwGrid > tiles ? kVwGrid : tiles) * 8));
   }
 };
 int64_t vloss_tc_bytes(int tokens, int64_t vocab, int width, int dtype, bool backward, bool dx) { return 1024 + VtRoom(tokens, vocab, width, dtype, backward, dx).bytes; }
@@ -874,7 +876,6 @@ template <typename T, int kR> __global__ void __launch_bounds__(kVwThreads, kVwC
   }
 }
 
-static bool vw_shape(int tokens, int width, int dtype) { return dtype != TKV_F32 && tokens <= kVwTokens && (int64_t)tokens * width <= kVwValues; }
 template <typename T, int kR> static int vw_launch(const Vloss& p, const void* xc, cudaStream_t st) {
   const int bytes = kR * ((p.width + kVwCols - 1) / kVwCols) * kVwCols * 4;
   cudaError_t e = cudaFuncSetAttribute(vloss_words_kernel<T, kR>, cudaFuncAttributeMaxDynamicSharedMemorySize, kVwBytes);
