@@ -37,6 +37,11 @@ constexpr int kVtSum = 16;
 // In fp32 half as many.  RMS error of the gradients of 300 tokens, width 1024, 32768 words, with 16 stages: 8.4e-7 (dx) and 8.9e-7 (dw), with 8
 // 4.6e-7 and 3.3e-7 (fp32 products on the CUDA cores: 1.0e-6 and 5.4e-7); us of the pass 785 to 840 both.
 constexpr int kVtSum32 = 8;
+// Gradients in 16 bits: sums of 4096 of the tokens or words.  In one sum of any length, whose products come to be far below it, dw of 32768, 2^17
+// and 2^21 tokens with products of one sign was -2.0e-4, -8.3e-4 and -1.3e-2 of itself off in the mean, all of it to one side (rounding to fp16
+// is 2.4e-4 in the mean, either way); with 256 stages -8e-5, 128 -4e-5, 64 -2e-5 at every length.  us of dx and dw of 4096 x 30000 x 2048:
+// 1008, 1010, 1011, 1011; of 8192 x 151936 x 2048 10.8 ms with any.
+constexpr int kVtSumGrad = 64;
 // The label's entry of dL, g (p - 1), is most of its row, and what rounding it to 16 bits takes away does not average out: all of a row of
 // dx, and of dw's row of the label, is off by it.  It is kept (Vloss::rest) and goes back in where those rows are finished, w[label] rest into
 // dx, x rest into dw.  For dw every warp of 32 rows looks through the tokens' labels, up to kVtExact tokens and the first kVtExactHits of them:
@@ -976,7 +981,7 @@ int vloss_tc_backward(Vloss& l, void* ws, bool want_dx, cudaStream_t st) {
     rc = vt_parts_of(p, room, base + room.w, st);
     p.sum_steps = f32 ? kVtSum32 : kVtSum;
     if (rc == TKV_OK) rc = vt_launch<kVtLogits>(a, p, st);
-    if (!f32) p.sum_steps = INT32_MAX;                     // gradients that are rounded to 8 or 11 bits in the end
+    if (!f32) p.sum_steps = kVtSumGrad;
     if (rc == TKV_OK) rc = vt_launch<kVtGrads>(g, p, st);
   }
   return rc;
