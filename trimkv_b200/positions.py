@@ -193,7 +193,8 @@ class RotaryPlan:
     def _on(self, device) -> list:
         held = self._held.get(device)
         if held is None:
-            held = self._held[device] = [split_frequencies(t).to(device) for t in self._tables]
+            with torch.inference_mode(False):             # kept beyond this call: a training pass saves them for its gradients
+                held = self._held[device] = [split_frequencies(t).to(device) for t in self._tables]
         return held
 
     def on(self, device, positions: torch.Tensor) -> Tuple[torch.Tensor, float]:
