@@ -65,6 +65,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: tor
         raise TypeError(f"labels of {labels.dtype}: want int32 or int64")
     if not hidden.device == weight.device == labels.device:
         raise ValueError(f"hidden rows on {hidden.device}, weight on {weight.device}, labels on {labels.device}")
+    if status is not None and (status.dtype != torch.int32 or status.numel() < 1 or status.device != hidden.device):
+        raise ValueError(f"status {status.dtype} {tuple(status.shape)} on {status.device}: want int32 on {hidden.device}, as ops.new_status gives it")
     x = hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])
     if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
         x = x.contiguous()
