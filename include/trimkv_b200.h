@@ -679,8 +679,8 @@ int tkv_rotary(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_ss, void* q_
  * tkv_vloss_backward: grad is the gradient of the loss of every token (reduction 0; grad_stride elements apart) or of the reduced number;
  * dx [tokens, width] and dw [vocab, width] dense, in the type of x and w, either may be NULL.
  * Workspaces (16-byte aligned): tkv_vloss_workspace_bytes, -1 for sizes that are refused (more than 2^24 tokens, 2^23 words, 2^43 logits or
- * a width of 65536).  The plan is 8-byte aligned.  A wait inside a kernel that runs out sets TKV_DEV_TIMEOUT and makes losses, or dx and dw,
- * NaN. */
+ * a width of 65536); of a backward pass up to 500 MB and the rows once more, beyond 16384 tokens 16 KB a token (fp32: 12 KB) and the rows
+ * once more.  The plan is 8-byte aligned.  A wait inside a kernel that runs out sets TKV_DEV_TIMEOUT and makes losses, or dx and dw, NaN. */
 int64_t tkv_vloss_plan_words(int64_t tokens);
 int64_t tkv_vloss_workspace_bytes(int64_t tokens, int64_t vocab, int width, int dtype, int backward, int want_dx);
 int tkv_vloss_forward(const void* x, int64_t x_stride, const void* w, const int64_t* labels, int64_t ignore, int64_t tokens,

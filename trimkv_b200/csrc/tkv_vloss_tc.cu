@@ -35,7 +35,7 @@ constexpr int kVtHalf = kVtCols / 2;                       // columns of a warp 
 // ms of 8192 x 151936 x 2048 with both gradients: 14.6, 14.7, 15.2, 16.4; us of 1500 tokens scored: 600, 620, 655, 710.
 constexpr int kVtSum = 16;
 // In fp32 half as many.  RMS error of the gradients of 300 tokens, width 1024, 32768 words, with 16 stages: 8.4e-7 (dx) and 8.9e-7 (dw), with 8
-// 4.6e-7 and 3.3e-7 (fp32 products on the CUDA cores: 1.0e-6 and 5.4e-7); us of the pass 785 to 840 both.
+// 4.6e-7 and 3.3e-7 (fp32 products on the CUDA cores: 1.0e-6 and 5.4e-7); us of the pass's kernels 620 and 636.
 constexpr int kVtSum32 = 8;
 // Gradients in 16 bits: sums of 4096 of the tokens or words.  In one sum of any length, whose products come to be far below it, dw of 32768, 2^17
 // and 2^21 tokens with products of one sign was -2.0e-4, -8.3e-4 and -1.3e-2 of itself off in the mean, all of it to one side (rounding to fp16
@@ -224,7 +224,7 @@ vloss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm->tmem_base)), "r"(512));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
   }
-  if (kMode != kVtGrads || p.want_dx) {                    // rows of A that no copy fills: zeros cost the products least power (us of 1 token: 146, so 125)
+  if (kMode != kVtGrads || p.want_dx) {                    // rows of A that no copy fills: zeros cost the products least power (us of 5 tokens of 151936 x 2048 scored: 122, so 118)
     const int kept = rank < p.a_ranks ? p.a_box * 128 : 0;
     for (int i = kept + tid * 16; i < kVtABytes; i += kVtThreads * 16)
       for (int st = 0; st < kVtStages; ++st) st16(base + st * kVtStage + i, make_uint4(0, 0, 0, 0));
@@ -646,16 +646,15 @@ static int vt_parts(int dtype) { return dtype == TKV_F32 ? 3 : 1; }
 // ---------------------------------------------------------------------------------------------- a handful of tokens, CUDA cores
 // Logits of up to four tokens in 16 bits, bound by the weight's bytes: a warp takes four words at a time, a lane eight columns of every 256 of
 // each, and keeps the largest logit and the sum of one of the 4 kR (word, token) pairs while it goes through the vocabulary, so that a CTA
-// writes one pair of numbers for a token.  us of 151936 words, width 2048, 1, 2 and 4 tokens: 96, 98, 110; on the tensor cores, whose tiles
-// have two rows in 256 that count, 113, 116, 121.  8 tokens would take 273 for 123: 8 x 311e6 products are more than the bytes.
+// writes one pair of numbers for a token.  us of 151936 words, width 2048, 1, 2 and 4 tokens: 96, 98, 110; on the tensor cores,
+// where these few no longer go, 113, 116, 121.  8 tokens would take 273 here for 118 there: 8 x 311e6 products are more than the bytes.
 // One run of columns requested ahead 117 (1 token), two 98, three 96; three CTAs an SM, with fewer registers, 103 to 227.
 constexpr int kVwThreads = 256, kVwWords = 4, kVwCols = 256, kVwCtas = 2, kVwGrid = 148 * kVwCtas, kVwTokens = 4;
 constexpr int kVwValues = 16384, kVwBytes = 2 * kVwValues * 4;   // x in shared memory: tokens up to a power of two, whole runs of 256 columns
 
 static int64_t vt_rows(int tokens) { return vl_round(tokens, kVtRows); }
 // Columns of a tile: what a pair does in its rounds is rounds x columns, and a little per round; few rounds make it matter that the last
-// one is full.  us of the logits of one token, 151936 words, width 2048:
-// 256 columns 106.3, by this rule (208) 103.7.
+// one is full.  us of 5 tokens scored, 151936 words, width 2048: 256 columns 120.3, by this rule (208) 118.3.
 static int vt_tile_cols(int tokens, int64_t vocab, int step) {
   const int64_t mt = vt_rows(tokens) / kVtRows;
   if (mt * ((vocab + kVtCols - 1) / kVtCols) > 20 * kVtPairs) return kVtCols;
@@ -668,8 +667,8 @@ static int vt_tile_cols(int tokens, int64_t vocab, int step) {
   return best;
 }
 static int vt_a_box(int tokens) { return tokens >= 128 ? 128 : (int)vl_round(tokens, 8); }
-// The vocabulary in equal pieces: of at most 256 MB of dL where that is not fewer than 8192 words; fp32: of at most 96 MB of parts of w too,
-// and not fewer than 2048 words.
+// The vocabulary in equal pieces: of at most 256 MB of dL where that is not fewer than 8192 words (so from 16385 tokens on dL is larger, 16 KB a
+// token); fp32: of at most 96 MB of parts of w too, and not fewer than 2048 words (from 21846 tokens on dL is 12 KB a token).
 static int64_t vt_piece(int tokens, int64_t vocab, int width, int dtype) {
   int64_t n = ((int64_t)256 << 20) / (2 * vt_parts(dtype) * vt_rows(tokens));
   int64_t least = 8192;

@@ -48,7 +48,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: tor
     outside the vocabulary makes its token's loss NaN, leaves the token out of the gradients and is recorded in ``status``
     (``ops.new_status``).  Differentiable in hidden and weight; gradients are accumulated in fp32 and rounded once, with the
     gradients of the logits rounded to the inputs' type for the products (the label's, the largest of a token, counts in full for hidden,
-    and for weight up to 256 tokens).  Under autocast hidden and weight are taken in its type, as
+    and for weight up to 256 tokens, the first eight of every 32 neighbouring words).  Under autocast hidden and weight are taken in its type, as
     ``torch.nn.functional.linear`` takes them."""
     if reduction not in ops.VLOSS_REDUCTIONS:
         raise ValueError(f"reduction {reduction!r}: one of {sorted(ops.VLOSS_REDUCTIONS)}")
