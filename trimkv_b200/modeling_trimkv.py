@@ -267,8 +267,9 @@ class RotaryEmbedding(nn.Module):
 
     ``rope_parameters`` of long-context checkpoints (``rope_type`` linear, llama3, yarn, longrope, dynamic) are taken as
     ``positions.RotaryPlan`` describes them, their angles in 64 bits; queries and keys of a prompt are then turned by
-    ``positions.apply_rotary``, one kernel with a gradient, rounded once.  The default embedding keeps the reference's order of
-    operations and roundings unless ``config.fused_rotary`` is set, which takes the kernel for it too."""
+    ``positions.apply_rotary``, one kernel with a gradient, rounded once (the fused decode step takes cos and sin as tables of the model's
+    type).  The default embedding keeps the reference's order of operations and roundings unless ``config.fused_rotary`` is set, which
+    takes the kernel for it too."""
 
     def __init__(self, config):
         super().__init__()
